@@ -25,6 +25,8 @@ MAX_NMS_LIMIT = 4096
 MAX_GT = 4096
 MAX_LAYERS = 8
 STATIC_SCRATCH_BYTES = 4 << 20
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
+MAX_TOP = 1024
 
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
@@ -81,6 +83,12 @@ SIGNATURES = {
     "ssdbox_prepare_gt": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "ssdbox_widerface_rows": (_i, [_vp, _vp, _vp, _i, _i, _vp, _vp]),
     "ssdbox_ssd_loss": (_i, [_vp, _vp, _vp, _i, _i64, _i, _i, _f, _vp, _vp, _vp]),
+    "ssdbox_linear_cross_entropy_workspace": (_i, [_i64, _i64, _i64, _i64, _i, _f, _i, _i, ctypes.POINTER(ctypes.c_size_t)]),
+    "ssdbox_linear_cross_entropy": (_i, [_vp, _vp, _i64, _vp, _i64, _vp, _i, _i64, _i64, _i64, _i, _f, _f, _vp, _vp, _vp, _vp,
+                                         _vp, ctypes.c_size_t]),
+    "ssdbox_distill_topk_workspace": (_i, [_i64, _i64, _i, ctypes.POINTER(ctypes.c_size_t)]),
+    "ssdbox_distill_topk": (_i, [_vp, _vp, _i64, _i64, _i64, _i, _vp, _vp, _i, _i, _vp, _f, _vp, _vp, _vp, _vp,
+                                 ctypes.c_size_t]),
     "ssdbox_selftest": (_i, [_vp, _pf, _pf, _pf, _pf, _i]),
 }
 

@@ -8,6 +8,7 @@ equal that loop image by image.
 Arrays may be numpy arrays, tf.Tensors, anything exporting __dlpack__, or torch tensors; PyTorch
 is touched only in the last case (runtime.Session).
 """
+import ctypes
 import functools
 
 import numpy as np
@@ -246,3 +247,198 @@ def ssd_loss_batch(y_true, y_pred, neg_pos_ratio=3, n_neg_min=0, alpha=1.0, retu
     if return_grad:
         res += (sess.get(grad, family),)
     return res[0] if len(res) == 1 else res
+
+
+# ------------------------------------------------------------------ losses of large classifiers
+def _device_of(*arrays):
+    """The GPU of the first CUDA tensor among the arguments, or None: such a call runs where its data is."""
+    for x in arrays:
+        if _is_torch_tensor(x) and x.is_cuda:
+            return int(x.device.index)
+    return None
+
+
+def _session(context, *arrays):
+    """A session on the device the arrays are on; torch tensors on two GPUs are refused."""
+    device = _device_of(*arrays)
+    if context is not None and device is not None and device != context.device:
+        raise ValueError("the context runs on GPU %d, the arrays are on GPU %d" % (context.device, device))
+    for x in arrays:
+        if _is_torch_tensor(x) and x.is_cuda and int(x.device.index) != device:
+            raise ValueError("arrays on GPU %d and GPU %d" % (device, int(x.device.index)))
+    return Session(*arrays, context=context, device=device)
+
+
+def _float_rows(sess, x, name, max_ld=None):
+    """A float32 / float16 / bfloat16 array as rows of its last axis: (array, family, rows, row stride,
+    SSDBOX_DTYPE code, type).  Rows of a CUDA tensor may lie further apart than they are long."""
+    if _is_torch_tensor(x):
+        torch = _torch()
+        code = {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16,
+                torch.bfloat16: _lib.DTYPE_BF16}.get(x.dtype)
+        if code is None:
+            raise ValueError("%s must be float32, float16 or bfloat16, got %s" % (name, x.dtype))
+        if x.dim() < 2:
+            raise ValueError("%s must have at least 2 dimensions, got shape %s" % (name, tuple(x.shape)))
+        t = x.detach()
+        if not t.is_cuda or t.device.index != sess.device:
+            t = t.to("cuda:%d" % sess.device)
+        width = int(t.shape[-1])
+        rows = 1
+        for s in t.shape[:-1]:
+            rows *= int(s)
+        if rows and width:
+            try:
+                t = t.view(rows, width)
+            except RuntimeError:
+                t = t.reshape(rows, width)
+            if (t.stride(1) != 1 and width > 1) or (rows > 1 and not width <= t.stride(0) <= (max_ld or 1 << 62)):
+                t = t.contiguous()
+            ld = int(t.stride(0)) if rows > 1 else width
+        else:
+            t, ld = t.reshape(rows, width), width
+        return t, "torch", rows, ld, code, t.dtype
+    dtype = np.dtype(getattr(x, "dtype", np.float32)) if not _is_tf_tensor(x) else np.dtype(x.dtype.as_numpy_dtype)
+    if dtype not in (np.dtype(np.float32), np.dtype(np.float16)):
+        raise ValueError("%s must be float32 or float16 (or a torch bfloat16 tensor), got %s" % (name, dtype))
+    t, family = sess.put(x, dtype if not sess.use_torch else None)
+    if len(t.shape) < 2:
+        raise ValueError("%s must have at least 2 dimensions, got shape %s" % (name, tuple(t.shape)))
+    rows = 1
+    for s in t.shape[:-1]:
+        rows *= int(s)
+    code = _lib.DTYPE_F32 if dtype == np.dtype(np.float32) else _lib.DTYPE_F16
+    return t, family, rows, int(t.shape[-1]), code, (t.dtype if sess.use_torch else dtype)
+
+
+def _integers(sess, x, name, shape):
+    """An int32 or int64 array of the given shape, dense on the device: (array, bytes a value)."""
+    if _is_torch_tensor(x):
+        torch = _torch()
+        t = x.detach()
+        if t.dtype not in (torch.int32, torch.int64):
+            if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
+                raise ValueError("%s must be integers, got %s" % (name, t.dtype))
+            t = t.to(torch.int64)
+        if not t.is_cuda or t.device.index != sess.device:
+            t = t.to("cuda:%d" % sess.device)
+        t = t.contiguous()
+        if tuple(t.shape) != tuple(shape):
+            raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
+        return t, t.element_size()
+    a = x.numpy() if _is_tf_tensor(x) else np.asarray(x)
+    if a.dtype.kind not in "iu":
+        raise ValueError("%s must be integers, got %s" % (name, a.dtype))
+    if tuple(a.shape) != tuple(shape):
+        raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), a.shape))
+    if a.dtype != np.int32:
+        if a.dtype == np.uint64 and a.size and int(a.max()) > np.iinfo(np.int64).max:
+            raise ValueError("%s do not fit int64" % name)
+        a = a.astype(np.int64)
+    return sess.from_host(a), a.dtype.itemsize
+
+
+def _row_floats(sess, x, name, shape):
+    """A float32 array of the given shape on the device, or None."""
+    if x is None:
+        return None
+    t, _ = sess.put(x.detach() if _is_torch_tensor(x) else x, np.float32)
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
+    return t
+
+
+def _aligned(t, ld, width):
+    """The same rows starting at a 16-byte boundary."""
+    if t.data_ptr() % 16 == 0:
+        return t, ld
+    return t.clone(memory_format=_torch().contiguous_format), width
+
+
+@_on_context_stream
+def linear_cross_entropy_batch(hidden, weight, labels, logit_scale=1.0, label_smoothing=0.0, grad_loss=None,
+                               return_grad=False, weight_grad=True, context=None):
+    """Softmax cross entropy of a linear head over many classes; the logits are never stored whole.
+
+    hidden (..., D) and weight (V,D) of one type (float32, float16, bfloat16); labels (...) int32 or
+    int64.  logits = logit_scale * hidden weight^T.  A negative label leaves its row out: loss 0, no
+    gradient, its hidden values unused.  A label >= V gives loss NaN and no gradient.
+    Returns the (...) float32 loss per row; with return_grad also the gradients with respect to
+    hidden and weight, in their types, of sum(grad_loss * loss), or of mean(loss) over all rows when
+    grad_loss (...) is None (weight_grad=False: a frozen head, the hidden rows' gradient alone).
+    The tensors' autograd graph is not extended: the gradients are what the call returns.
+    """
+    sess = _session(context, hidden, weight, labels, grad_loss)
+    ctx = sess.ctx
+    lead = tuple(int(s) for s in hidden.shape[:-1])
+    h, family, rows, ld_h, code, dtype = _float_rows(sess, hidden, "hidden")
+    w, _, classes, ld_w, code_w, _ = _float_rows(sess, weight, "weight", 1 << 21)
+    if code != code_w:
+        raise ValueError("hidden and weight must have one type")
+    dim = int(h.shape[-1])
+    if len(weight.shape) != 2 or int(w.shape[-1]) != dim:
+        raise ValueError("weight must have shape (V, %d), got %s" % (dim, tuple(weight.shape)))
+    if classes == 0 or dim == 0:
+        raise ValueError("a head needs classes and values, got shape %s" % (tuple(weight.shape),))
+    if sess.use_torch:
+        w, ld_w = _aligned(w, ld_w, dim)
+    lab, label_bytes = _integers(sess, labels, "labels", lead)
+    g = _row_floats(sess, grad_loss, "grad_loss", lead) if return_grad else None
+    lib, need = ctx.lib, ctypes.c_size_t()
+    _lib.check(lib.ssdbox_linear_cross_entropy_workspace(
+        rows, classes, dim, ld_w, code, float(label_smoothing), int(bool(return_grad)),
+        int(bool(return_grad and weight_grad)), ctypes.byref(need)))
+    loss = sess.empty(lead)
+    gh = sess.empty(lead + (dim,), dtype) if return_grad else None
+    gw = sess.empty((classes, dim), dtype) if return_grad and weight_grad else None
+    work = sess.empty((need.value,), np.uint8)
+    _lib.check(lib.ssdbox_linear_cross_entropy(
+        ctx.handle, _ptr(h), ld_h, _ptr(w), ld_w, _ptr(lab), label_bytes, rows, classes, dim, code,
+        float(logit_scale), float(label_smoothing), _ptr(g), _ptr(loss), _ptr(gh), _ptr(gw), _ptr(work), need.value))
+    res = (sess.get(loss, family),)
+    if return_grad:
+        res += (sess.get(gh, family),)
+        if weight_grad:
+            res += (sess.get(gw, family),)
+    return res[0] if len(res) == 1 else res
+
+
+@_on_context_stream
+def distill_topk_batch(logits, teacher_values, teacher_index, temperature=1.0, teacher_lse=None, grad_loss=None,
+                       return_grad=False, context=None):
+    """Distillation from a teacher's top logits.
+
+    logits (..., V) of the student (float32, float16, bfloat16), such as the class columns of the
+    heads' output; teacher_values (..., K) the teacher's largest logits, teacher_index (..., K) their
+    classes (int32 or int64; an index outside [0, V) or a value of -inf is padding).  With
+    p = softmax(logits / temperature), the (...) float32 loss per row is temperature^2 KL(q || p):
+      teacher_lse None: q = softmax(teacher_values / temperature);
+      teacher_lse (...), the log-sum-exp of all the teacher's logits / temperature:
+      q = exp(teacher_values / temperature - teacher_lse), and the classes without an entry form one
+      bucket of both.
+    A row without an entry has loss 0 and no gradient.  With return_grad also the (..., V) gradient
+    in the logits' type of sum(grad_loss * loss), or of mean(loss) when grad_loss (...) is None.
+    The tensors' autograd graph is not extended: the gradient is what the call returns.
+    """
+    sess = _session(context, logits, teacher_values, teacher_index, teacher_lse, grad_loss)
+    ctx = sess.ctx
+    z, family, rows, ld, code, dtype = _float_rows(sess, logits, "logits")
+    lead, classes = tuple(int(s) for s in logits.shape[:-1]), int(z.shape[-1])
+    if classes == 0:
+        raise ValueError("logits have no classes: shape %s" % (tuple(logits.shape),))
+    if len(teacher_values.shape) != len(lead) + 1:
+        raise ValueError("teacher_values must have shape %s + (K,), got %s" % (lead, tuple(teacher_values.shape)))
+    top = int(teacher_values.shape[-1])
+    values = _row_floats(sess, teacher_values, "teacher_values", lead + (top,))
+    index, index_bytes = _integers(sess, teacher_index, "teacher_index", lead + (top,))
+    lse = _row_floats(sess, teacher_lse, "teacher_lse", lead)
+    g = _row_floats(sess, grad_loss, "grad_loss", lead) if return_grad else None
+    lib, need = ctx.lib, ctypes.c_size_t()
+    _lib.check(lib.ssdbox_distill_topk_workspace(rows, classes, code, ctypes.byref(need)))
+    loss = sess.empty(lead)
+    grad = sess.empty(lead + (classes,), dtype) if return_grad else None
+    work = sess.empty((need.value,), np.uint8) if need.value else None
+    _lib.check(lib.ssdbox_distill_topk(
+        ctx.handle, _ptr(z), ld, rows, classes, code, _ptr(values), _ptr(index), index_bytes, top, _ptr(lse),
+        float(temperature), _ptr(g), _ptr(loss), _ptr(grad), _ptr(work), need.value))
+    return (sess.get(loss, family), sess.get(grad, family)) if return_grad else sess.get(loss, family)

@@ -1,0 +1,798 @@
+// Cross entropy of a linear head over many classes, with its gradients, without the logits being kept.
+//
+//   z = s H W^T (rows x classes), l = label, eps = label smoothing, V = classes
+//   nll = log sum_v exp z_v - z_l,   loss = (1 - eps) nll + eps (log sum_v exp z_v - mean_v z_v)
+//   d_nv = g_n s (p_nv - eps / V - (1 - eps) [v = l]),   dH = d W,   dW = d^T H
+//
+// Rows without a class (label < 0) leave the batch first: the counted rows are copied together, so a padded batch costs
+// what its counted rows cost and nothing of a padded row (a NaN, say) reaches a sum over rows.  Then
+//   1  logits, a tile of classes x rows per workgroup; of each tile only (max, sum of exp) per row leave the chip
+//   2  per row: log-sum-exp, loss, and what the gradient needs (four floats a row)
+//   3  per piece of the classes: the logits again, turned into d in the epilogue and written in the operands' type;
+//      dH += d W_piece, dW_piece = d^T H.
+// Recomputing the logits is 2 of the gradient's 8 rows * classes * dim operations; what it saves is rows * classes values.
+//
+// The label's own class stays out of the sum of exponentials: with S = sum over the others of exp(z_v - M), a sure row's
+// nll is log1p(S exp(M - z_l)) and p_l - 1 is expm1(-nll), both without the cancellation that 1 - p_l has.
+// Exponentials are taken to base 2: exp(z_v - M) = 2^(a L - m) with a the product as summed, L = s log2(e) and m the row's
+// largest a L rounded once; m itself is what the rows' kernel adds back, so its rounding cancels.
+// Sums over k stay in float32 accumulators; over tiles and rows of partial results they are added in a fixed order, in
+// float64 for the exponentials.  d is rounded once, to the operands' type, which is what the matrix instructions read.
+#include <math.h>
+
+#include "ssdbox_tile.h"
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLn2 = 0.69314718055994530942;
+constexpr int kScanThreads = 1024;
+constexpr int kRowThreads = 256;
+
+struct HeadScale {                    // what the gradient's rows are multiplied by before d, and the results after
+    float down, up;
+};
+
+struct HeadRow {                      // a counted row: p_v = 2^(a L - m) * c / Z with c = g_n s folded in
+    float m, pz, label, smooth;       // pz = c / Z, label = c (p_l - (1 - eps) - eps / V), smooth = c eps / V
+};
+
+// ------------------------------------------------------------------------------ rows
+struct ScanArgs {
+    const void *labels;
+    int label_bytes, rows;
+    long long classes;
+    const float *grad_loss;
+    float logit_scale;
+    int scaled;                       // 16-bit gradients: bring the largest c to just under 2^15
+    int *place;                       // per row: its place among the counted rows, or -1
+    int *row, *label;                 // per counted row: the row it was, its class
+    int *count;
+    HeadScale *scale;
+    float *loss;
+};
+
+SSD_DEV long long label_at(const void *p, int bytes, int n)
+{
+    return bytes == 8 ? ((const long long *)p)[n] : (long long)((const int *)p)[n];
+}
+
+// One workgroup: the order of the counted rows has to be that of the batch, so that sums over rows are the same every time.
+__global__ __launch_bounds__(kScanThreads) void head_scan_kernel(const ScanArgs p)
+{
+    __shared__ int s_wave[kScanThreads / 64];
+    __shared__ float s_max[kScanThreads / 64];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    int before = 0;
+    float gmax = 0.0f;
+    for (int base = 0; base < p.rows; base += kScanThreads) {
+        const int n = base + t;
+        const long long lab = n < p.rows ? label_at(p.labels, p.label_bytes, n) : -1;
+        const bool counted = lab >= 0 && lab < p.classes;
+        const unsigned long long bal = __ballot(counted);
+        if (lane == 0) s_wave[wave] = __popcll(bal);
+        __syncthreads();
+        int at = before + __popcll(bal & ((1ull << lane) - 1ull)), all = 0;
+#pragma unroll
+        for (int w = 0; w < kScanThreads / 64; ++w) {
+            const int c = s_wave[w];
+            if (w < wave) at += c;
+            all += c;
+        }
+        before += all;
+        if (n < p.rows) {
+            p.place[n] = counted ? at : -1;
+            if (counted) {
+                p.row[at] = n;
+                p.label[at] = (int)lab;
+                if (p.grad_loss) gmax = fmaxf(gmax, fabsf(p.grad_loss[n]));
+            } else {
+                p.loss[n] = lab < 0 ? 0.0f : u2f(0x7FC00000u);
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) gmax = fmaxf(gmax, __shfl_xor(gmax, o));
+    if (lane == 0) s_max[wave] = gmax;
+    __syncthreads();
+    if (t != 0) return;
+    *p.count = before;
+    HeadScale s = {1.0f, 1.0f};
+    if (p.scaled) {
+        for (int w = 0; w < kScanThreads / 64; ++w) gmax = fmaxf(gmax, s_max[w]);
+        if (!p.grad_loss) gmax = 1.0f / (float)p.rows;
+        // Of float16 this uses the range; and an unsure row's d at its label, -c (1 - p), which weighs most in the
+        // gradients, lies just under a power of two, where the rounding to 8 or 11 bits is finest.
+        const float c = gmax * p.logit_scale;
+        if (c > 1e-30f && c < 1e30f) {
+            s.down = 32768.0f * (1.0f - 1.0f / 128.0f) / c;
+            s.up = 1.0f / s.down;
+        }
+    }
+    *p.scale = s;
+}
+
+// One workgroup a row: a counted row to its place (zeros behind its last value), another one's gradient to zero.
+template <typename T>
+__global__ __launch_bounds__(kRowThreads) void head_gather_kernel(const T *hidden, long long ld, const int *place, int dim,
+                                                                  int pitch, T *rows, T *grad_hidden)
+{
+    const long long n = blockIdx.x;
+    const int at = place[n];
+    if (at >= 0) {
+        for (int d = threadIdx.x; d < pitch; d += kRowThreads)
+            rows[(long long)at * pitch + d] = d < dim ? hidden[n * ld + d] : (T)0.0f;
+    } else if (grad_hidden) {
+        for (int d = threadIdx.x; d < dim; d += kRowThreads) grad_hidden[n * dim + d] = (T)0.0f;
+    }
+}
+
+// Rows of a weight whose rows do not start at 16-byte boundaries, laid out so that they do.
+template <typename T>
+__global__ __launch_bounds__(kRowThreads) void head_pitch_kernel(const T *weight, long long ld, int dim, int pitch, T *out)
+{
+    const long long v = blockIdx.x;
+    for (int d = threadIdx.x; d < pitch; d += kRowThreads) out[v * pitch + d] = d < dim ? weight[v * ld + d] : (T)0.0f;
+}
+
+// --------------------------------------------------------------------------- products
+struct LogitArgs {
+    const void *weight, *rows;        // classes x dim from the piece's first class on; counted rows x dim
+    long long ldw, ldh;
+    int dim, classes, tiles;          // classes and tiles of classes in this piece
+    int first;                        // the piece's first class
+    int row_tiles;
+    float l2;                         // logit_scale * log2(e)
+    const int *count, *label;
+    float2 *stat;                     // [row][slots]: (max, sum of exponentials) of one wave's part of a tile
+    float *sum_z;                     // [row][slots], or NULL without smoothing
+    long long slots;
+    int slot0;
+    float *z_label;                   // [row]: the label's product, before the scale
+    const HeadRow *row;
+    void *delta;                      // [row][ld_delta]
+    long long ld_delta;
+};
+
+// GRAD false: statistics of a tile of logits; true: d of it.
+template <typename T, int BM, int BN, int WM, int WN, bool GRAD>
+__global__ __launch_bounds__(WM * WN * 64) void head_logit_kernel(const LogitArgs p)
+{
+    typedef TileProduct<T, BM, BN, WM, WN, false, false> P;
+    __shared__ __align__(1024) char smem[P::kLds];
+    const int count = uniform(*p.count);
+    const int tn = (count + BN - 1) / BN;
+    if ((int)blockIdx.x >= p.tiles * tn) return;
+    int tm_i, tn_i;
+    tile_of(blockIdx.x, p.tiles, tn, 8, tm_i, tn_i);
+    const int m0 = tm_i * BM, n0 = tn_i * BN;
+    typename P::OpA a;
+    typename P::OpB b;
+    a.init(p.weight, p.ldw, m0, p.classes - m0, 0, smem);
+    b.init(p.rows, p.ldh, n0, count - n0, 0, smem + BM * kRowBytes);
+    f32x4 acc[P::MF][P::NF];
+    P::run(a, b, p.dim, smem, acc);
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const int wm = wave / WN, wn = wave % WN;
+    const int v0 = m0 + wm * (BM / WM) + 4 * g;                  // within the piece
+#pragma unroll
+    for (int nj = 0; nj < P::NF; ++nj) {
+        const int n = n0 + wn * (BN / WN) + nj * 16 + (lane & 15);
+        const bool in = n < count;
+        const int lab = in ? p.label[n] - p.first : -1;
+        if constexpr (!GRAD) {
+            float mx = -INFINITY, sz = 0.0f;
+#pragma unroll
+            for (int mi = 0; mi < P::MF; ++mi)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int v = v0 + mi * 16 + i;
+                    const float z = acc[mi][nj][i];
+                    if (v < p.classes) {
+                        sz += z;
+                        if (v != lab) mx = fmaxf(mx, z);
+                        else p.z_label[n] = z;
+                    }
+                }
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const float m = mx * p.l2;
+            const float ref = mx == -INFINITY ? 0.0f : m;
+            float s = 0.0f;
+#pragma unroll
+            for (int mi = 0; mi < P::MF; ++mi)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int v = v0 + mi * 16 + i;
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mi][nj][i], p.l2, -ref));
+                    if (v < p.classes && v != lab) s += e;
+                }
+            s += __shfl_xor(s, 16);
+            s += __shfl_xor(s, 32);
+            if (in && g == 0) p.stat[(long long)n * p.slots + p.slot0 + tm_i * WM + wm] = make_float2(m, s);
+            if (p.sum_z) {
+                sz += __shfl_xor(sz, 16);
+                sz += __shfl_xor(sz, 32);
+                if (in && g == 0) p.sum_z[(long long)n * p.slots + p.slot0 + tm_i * WM + wm] = sz;
+            }
+        } else {
+            const HeadRow r = in ? p.row[n] : HeadRow{0.0f, 0.0f, 0.0f, 0.0f};
+            T *out = (T *)p.delta + (long long)n * p.ld_delta + v0;
+#pragma unroll
+            for (int mi = 0; mi < P::MF; ++mi) {
+                struct __align__(4 * sizeof(T)) Four { T v[4]; } o;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int v = v0 + mi * 16 + i;
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mi][nj][i], p.l2, -r.m));
+                    float d = __builtin_fmaf(e, r.pz, -r.smooth);
+                    d = v == lab ? r.label : d;
+                    o.v[i] = (T)(v < p.classes ? d : 0.0f);
+                }
+                if (in) *(Four *)(out + mi * 16) = o;
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------ row statistics
+struct RowArgs {
+    const int *count, *row, *label;
+    const float2 *stat;
+    const float *sum_z;
+    long long slots;
+    const float *z_label;
+    float l2, logit_scale, smoothing;
+    long long classes;
+    int rows;
+    const float *grad_loss;
+    const HeadScale *scale;
+    float *loss;
+    HeadRow *out;
+};
+
+// One wave of the workgroup a quarter of the row's slots, then wave 0 the row.
+__global__ __launch_bounds__(kRowThreads) void head_row_kernel(const RowArgs p)
+{
+    __shared__ float s_m[kRowThreads / 64];
+    __shared__ double s_s[kRowThreads / 64], s_z[kRowThreads / 64];
+    const int n = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    if (n >= *p.count) return;
+    const float2 *st = p.stat + (long long)n * p.slots;
+    float m = -INFINITY;
+    double s = 0.0, sz = 0.0;
+    for (long long i = t; i < p.slots; i += kRowThreads) {
+        const float2 x = st[i];
+        const float nm = fmaxf(m, x.x);
+        if (nm != -INFINITY) {
+            s = s * (double)__builtin_amdgcn_exp2f(m - nm) + (double)x.y * (double)__builtin_amdgcn_exp2f(x.x - nm);
+        } else {
+            s += (double)x.y;                   // nothing finite so far: zero, or a NaN
+        }
+        m = nm;
+        if (p.sum_z) sz += (double)p.sum_z[(long long)n * p.slots + i];
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const float om = __shfl_xor(m, o);
+        const double os = __shfl_xor(s, o);
+        const float nm = fmaxf(m, om);
+        if (nm != -INFINITY)
+            s = s * (double)__builtin_amdgcn_exp2f(m - nm) + os * (double)__builtin_amdgcn_exp2f(om - nm);
+        else
+            s += os;
+        m = nm;
+        sz += __shfl_xor(sz, o);
+    }
+    if (lane == 0) {
+        s_m[wave] = m;
+        s_s[wave] = s;
+        s_z[wave] = sz;
+    }
+    __syncthreads();
+    if (t != 0) return;
+    m = -INFINITY;
+    for (int w = 0; w < kRowThreads / 64; ++w) m = fmaxf(m, s_m[w]);
+    s = 0.0;
+    sz = 0.0;
+    for (int w = 0; w < kRowThreads / 64; ++w) {
+        s += m != -INFINITY ? s_s[w] * (double)__builtin_amdgcn_exp2f(s_m[w] - m) : s_s[w];
+        sz += s_z[w];
+    }
+    // to base 2: the others' sum is s * 2^m, the label's term 2^zl
+    const double zl = (double)p.z_label[n] * (double)p.l2;
+    double nll = 0.0;
+    if (s != 0.0) {
+        const double d = (double)m - zl;
+        nll = d > 500.0 ? d * kLn2 + log(s) : log1p(s * exp2(d));
+    }
+    const double z_label = (double)p.z_label[n] * (double)p.logit_scale;
+    double loss = nll;
+    if (p.smoothing != 0.0f) {
+        const double mean = sz * (double)p.logit_scale / (double)p.classes;
+        loss = (1.0 - (double)p.smoothing) * nll + (double)p.smoothing * (nll + z_label - mean);
+    }
+    const int n_in = p.row[n];
+    p.loss[n_in] = (float)loss;
+    if (!p.out) return;
+    const double g = p.grad_loss ? (double)p.grad_loss[n_in] : 1.0 / (double)p.rows;
+    const double c = g * (double)p.logit_scale * (double)p.scale->down;
+    const float top = fmaxf(m, (float)zl);
+    const double whole = s * exp2((double)m - (double)top) + exp2(zl - (double)top);
+    HeadRow r;
+    r.m = top;
+    r.pz = (float)(c / (s != 0.0 ? whole : exp2(zl - (double)top)));
+    const double share = (double)p.smoothing / (double)p.classes;
+    r.label = (float)(c * (expm1(-nll) + (double)p.smoothing - share));
+    r.smooth = (float)(c * share);
+    p.out[n] = r;
+}
+
+// ----------------------------------------------------------------------- gradient products
+struct GradArgs {
+    const void *a, *b;                // A: [k][m], m contiguous.  B: dH [n][k], dW [k][n]
+    long long lda, ldb;
+    int m, a_extent, n, k;            // a_extent: columns of A that may be read
+    const int *n_count, *k_count;     // device-side n or k, or NULL
+    int tm;
+    int steps;                        // K tiles per part
+    const HeadScale *scale;
+    void *out;                        // [n][ldo], through row_of when given
+    long long ldo;
+    const int *row_of;
+    float *part;                      // [part][n][ld_part] instead of out, or NULL
+    long long ld_part, part_stride;
+    int add;                          // to what part holds
+};
+
+template <typename T>
+SSD_DEV void store4(T *p, f32x4 v, float up, int left, bool wide)
+{
+    struct __align__(4 * sizeof(T)) Four { T v[4]; } o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o.v[i] = (T)(v[i] * up);
+    if (wide) {
+        if (left > 0) *(Four *)p = o;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i < left) p[i] = o.v[i];
+}
+
+template <typename T, int BM, int BN, int WM, int WN, bool B_KROWS>
+__global__ __launch_bounds__(WM * WN * 64) void head_grad_kernel(const GradArgs p)
+{
+    typedef TileProduct<T, BM, BN, WM, WN, true, B_KROWS> P;
+    __shared__ __align__(1024) char smem[P::kLds];
+    const int nn = uniform(p.n_count ? *p.n_count : p.n);
+    const int kk = uniform(p.k_count ? *p.k_count : p.k);
+    const int tn = (nn + BN - 1) / BN;
+    if ((int)blockIdx.x >= p.tm * tn) return;
+    int tm_i, tn_i;
+    tile_of(blockIdx.x, p.tm, tn, 8, tm_i, tn_i);
+    const int m0 = tm_i * BM, n0 = tn_i * BN;
+    const int k0 = blockIdx.y * p.steps * P::kBK;
+    const int kn = kk - k0 < p.steps * P::kBK ? kk - k0 : p.steps * P::kBK;
+    typename P::OpA a;
+    typename P::OpB b;
+    a.init(p.a, p.lda, m0, p.a_extent - m0, k0, smem);
+    b.init(p.b, p.ldb, n0, nn - n0, k0, smem + BM * kRowBytes);
+    f32x4 acc[P::MF][P::NF];
+    P::run(a, b, kn, smem, acc);
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const int em = m0 + (wave / WN) * (BM / WM) + 4 * g;
+    const int en = n0 + (wave % WN) * (BN / WN) + (lane & 15);
+    const float up = p.scale->up;
+    const bool wide = p.m % 4 == 0 && p.ldo % 4 == 0;
+#pragma unroll
+    for (int nj = 0; nj < P::NF; ++nj) {
+        const int n = en + nj * 16;
+        if (n >= nn) continue;
+        if (p.part) {
+            float *o = p.part + (long long)blockIdx.y * p.part_stride + (long long)n * p.ld_part + em;
+#pragma unroll
+            for (int mi = 0; mi < P::MF; ++mi)
+                if (em + mi * 16 < p.m) {       // ld_part is a multiple of 4: the last group may pass m, not the row
+                    f32x4 v = acc[mi][nj];
+                    if (p.add) v += *(const f32x4 *)(o + mi * 16);
+                    *(f32x4 *)(o + mi * 16) = v;
+                }
+        } else {
+            T *o = (T *)p.out + (p.row_of ? p.row_of[n] : n) * p.ldo + em;
+#pragma unroll
+            for (int mi = 0; mi < P::MF; ++mi) store4<T>(o + mi * 16, acc[mi][nj], up, p.m - em - mi * 16, wide);
+        }
+    }
+}
+
+struct JoinArgs {
+    const float *part;
+    long long ld_part, part_stride;
+    int parts, m, n;
+    const int *n_count;
+    const HeadScale *scale;
+    void *out;
+    long long ldo;
+    const int *row_of;
+};
+
+// The parts of a product over a long k, added in their order.
+template <typename T>
+__global__ __launch_bounds__(kRowThreads) void head_join_kernel(const JoinArgs p)
+{
+    const int n = blockIdx.x;
+    if (n >= (p.n_count ? *p.n_count : p.n)) return;
+    const float up = p.scale->up;
+    T *o = (T *)p.out + (p.row_of ? p.row_of[n] : n) * p.ldo;
+    for (int m = blockIdx.y * kRowThreads + threadIdx.x; m < p.m; m += kRowThreads * gridDim.y) {
+        const float *x = p.part + (long long)n * p.ld_part + m;
+        float s = 0.0f;
+        for (int i = 0; i < p.parts; ++i) s += x[i * p.part_stride];
+        o[m] = (T)(s * up);
+    }
+}
+
+// -------------------------------------------------------------------------------- plan
+// Everything that follows from sizes: which tile, how many parts, and the workspace.
+struct HeadPlan {
+    int es, vec, tile;                // bytes and 16-byte values of a type, tile configuration
+    int bm, bn, wm;
+    int pitch;                        // dim rounded up to 16 bytes
+    bool copy_weight;
+    long long class_tiles, slots;
+    long long piece;                  // classes a piece
+    int pieces;
+    int dh_parts, dh_steps, dw_parts, dw_steps;
+    size_t o_rows, o_weight, o_place, o_row, o_label, o_count, o_scale, o_stat, o_sumz, o_zl, o_out, o_delta, o_dh, o_dw;
+    size_t bytes;
+};
+
+constexpr size_t kDeltaBytes = (size_t)1 << 30;    // of one piece's d
+
+size_t put(size_t &at, size_t bytes)
+{
+    const size_t o = at;
+    at = (at + bytes + 255) / 256 * 256;
+    return o;
+}
+
+// Parts of k so that the tiles fill the chip, at least four K tiles each.
+void split(long long tiles, long long k_tiles, int &parts, int &steps)
+{
+    long long s = tiles > 0 ? 512 / tiles : 1;
+    if (s > k_tiles / 4) s = k_tiles / 4;
+    if (s > 64) s = 64;
+    if (s < 1) s = 1;
+    steps = (int)((k_tiles + s - 1) / s);
+    if (steps < 1) steps = 1;
+    parts = (int)((k_tiles + steps - 1) / steps);
+    if (parts < 1) parts = 1;
+}
+
+HeadPlan make_plan(long long rows, long long classes, long long dim, long long weight_ld, int dtype, float smoothing,
+                   bool grad_hidden, bool grad_weight)
+{
+    HeadPlan q = {};
+    q.es = dtype == SSDBOX_DTYPE_F32 ? 4 : 2;
+    q.vec = 16 / q.es;
+    q.pitch = (int)((dim + q.vec - 1) / q.vec * q.vec);
+    q.copy_weight = dim % q.vec != 0 || weight_ld % q.vec != 0;
+    // float32 keeps two sums a value (ssdbox_tile.h): the large tile's would not fit the registers
+    q.tile = rows <= 32 ? 0 : (rows <= 512 || dtype == SSDBOX_DTYPE_F32 ? 1 : 2);
+    q.bm = q.tile == 2 ? 256 : 128;
+    q.bn = q.tile == 2 ? 256 : (q.tile == 1 ? 128 : 32);
+    q.wm = q.tile == 0 ? 4 : 2;
+    q.class_tiles = (classes + q.bm - 1) / q.bm;
+    q.slots = q.class_tiles * q.wm;
+    const bool grad = grad_hidden || grad_weight;
+    if (grad) {
+        const long long row_bytes = rows * q.es > 0 ? rows * q.es : 1;
+        long long most = (long long)kDeltaBytes / row_bytes / 256 * 256;
+        if (most < 256) most = 256;
+        if (most > (1 << 21)) most = 1 << 21;
+        const long long whole = (classes + 255) / 256 * 256;
+        q.pieces = (int)((whole + most - 1) / most);
+        q.piece = ((whole + q.pieces - 1) / q.pieces + 255) / 256 * 256;
+        q.pieces = (int)((whole + q.piece - 1) / q.piece);
+    }
+    size_t at = 0;
+    q.o_count = put(at, 256);
+    q.o_scale = put(at, 256);
+    q.o_place = put(at, rows * 4);
+    q.o_row = put(at, rows * 4);
+    q.o_label = put(at, rows * 4);
+    q.o_zl = put(at, rows * 4);
+    q.o_out = put(at, rows * sizeof(HeadRow));
+    q.o_rows = put(at, (size_t)rows * q.pitch * q.es);
+    q.o_stat = put(at, (size_t)rows * q.slots * sizeof(float2));
+    q.o_sumz = put(at, smoothing != 0.0f ? (size_t)rows * q.slots * 4 : 0);
+    q.o_weight = put(at, q.copy_weight ? (size_t)classes * q.pitch * q.es : 0);
+    q.o_delta = put(at, grad ? (size_t)rows * q.piece * q.es : 0);
+    const int bk = kRowBytes / q.es;
+    const long long dim_tiles = (dim + q.bm - 1) / q.bm;
+    const long long wide = (dim + 3) / 4 * 4;
+    if (grad_hidden) {
+        split(dim_tiles * ((rows + q.bn - 1) / q.bn), (q.piece + bk - 1) / bk, q.dh_parts, q.dh_steps);
+        q.o_dh = put(at, q.dh_parts > 1 || q.pieces > 1 ? (size_t)q.dh_parts * rows * wide * 4 : 0);
+    }
+    if (grad_weight) {
+        const int bn = q.tile == 2 ? 256 : 128;
+        split(dim_tiles * ((q.piece + bn - 1) / bn), (rows + bk - 1) / bk, q.dw_parts, q.dw_steps);
+        q.o_dw = put(at, q.dw_parts > 1 ? (size_t)q.dw_parts * q.piece * wide * 4 : 0);
+    }
+    q.bytes = at;
+    return q;
+}
+
+struct HeadCall {
+    ssdbox_ctx *ctx;
+    const void *hidden, *weight, *labels;
+    long long hidden_ld, weight_ld;
+    int label_bytes;
+    long long rows, classes, dim;
+    float logit_scale, smoothing;
+    const float *grad_loss;
+    float *loss;
+    void *grad_hidden, *grad_weight;
+    char *ws;
+};
+
+template <typename T, int BM, int BN, int WM, int WN>
+void launch_logits(const HeadCall &c, const LogitArgs &a, bool grad)
+{
+    const dim3 grid((unsigned)((long long)a.tiles * ((c.rows + BN - 1) / BN))), block(WM * WN * 64);
+    if (grad)
+        launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_logit_kernel<T, BM, BN, WM, WN, true>, grid, block, a);
+    else
+        launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_logit_kernel<T, BM, BN, WM, WN, false>, grid, block, a);
+}
+
+template <typename T>
+void launch_logits(const HeadCall &c, int tile, const LogitArgs &a, bool grad)
+{
+    if (tile == 0) launch_logits<T, 128, 32, 4, 1>(c, a, grad);
+    else if (tile == 1) launch_logits<T, 128, 128, 2, 2>(c, a, grad);
+    else if constexpr (sizeof(T) == 2) launch_logits<T, 256, 256, 2, 4>(c, a, grad);
+}
+
+template <typename T, int BM, int BN, int WM, int WN, bool B_KROWS>
+void launch_grad(const HeadCall &c, GradArgs a, int parts)
+{
+    a.tm = (a.m + BM - 1) / BM;
+    const dim3 grid((unsigned)((long long)a.tm * ((a.n + BN - 1) / BN)), (unsigned)parts), block(WM * WN * 64);
+    launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_grad_kernel<T, BM, BN, WM, WN, B_KROWS>, grid, block, a);
+}
+
+template <typename T>
+void launch_join(const HeadCall &c, const GradArgs &a, int parts)
+{
+    JoinArgs j = {};
+    j.part = a.part;
+    j.ld_part = a.ld_part;
+    j.part_stride = a.part_stride;
+    j.parts = parts;
+    j.m = a.m;
+    j.n = a.n;
+    j.n_count = a.n_count;
+    j.scale = a.scale;
+    j.out = a.out;
+    j.ldo = a.ldo;
+    j.row_of = a.row_of;
+    const unsigned across = (unsigned)((a.m + kRowThreads - 1) / kRowThreads);
+    launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_join_kernel<T>, dim3((unsigned)a.n, across), dim3(kRowThreads), j);
+}
+
+template <typename T>
+int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
+{
+    ssdbox_ctx *ctx = c.ctx;
+    const bool grad = c.grad_hidden || c.grad_weight;
+    int *count = (int *)(c.ws + q.o_count), *place = (int *)(c.ws + q.o_place), *row = (int *)(c.ws + q.o_row);
+    int *label = (int *)(c.ws + q.o_label);
+    HeadScale *scale = (HeadScale *)(c.ws + q.o_scale);
+    T *rows = (T *)(c.ws + q.o_rows);
+
+    ScanArgs s = {};
+    s.labels = c.labels;
+    s.label_bytes = c.label_bytes;
+    s.rows = (int)c.rows;
+    s.classes = c.classes;
+    s.grad_loss = grad ? c.grad_loss : nullptr;
+    s.logit_scale = c.logit_scale;
+    s.scaled = dtype != SSDBOX_DTYPE_F32;
+    s.place = place;
+    s.row = row;
+    s.label = label;
+    s.count = count;
+    s.scale = scale;
+    s.loss = c.loss;
+    launch_stage(ctx, SSDBOX_STAGE_LOSS, head_scan_kernel, dim3(1), dim3(kScanThreads), s);
+    if (c.rows > 0)
+        launch_stage(ctx, SSDBOX_STAGE_LOSS, head_gather_kernel<T>, dim3((unsigned)c.rows), dim3(kRowThreads),
+                     (const T *)c.hidden, c.hidden_ld, place, (int)c.dim, q.pitch, rows, (T *)c.grad_hidden);
+    const T *weight = (const T *)c.weight;
+    long long ldw = c.weight_ld;
+    if (q.copy_weight && c.rows > 0) {
+        T *w = (T *)(c.ws + q.o_weight);
+        launch_stage(ctx, SSDBOX_STAGE_LOSS, head_pitch_kernel<T>, dim3((unsigned)c.classes), dim3(kRowThreads), weight,
+                     ldw, (int)c.dim, q.pitch, w);
+        weight = w;
+        ldw = q.pitch;
+    }
+
+    LogitArgs l = {};
+    l.weight = weight;
+    l.rows = rows;
+    l.ldw = ldw;
+    l.ldh = q.pitch;
+    l.dim = q.pitch;
+    l.classes = (int)c.classes;
+    l.tiles = (int)q.class_tiles;
+    l.l2 = c.logit_scale * kLog2e;
+    l.count = count;
+    l.label = label;
+    l.stat = (float2 *)(c.ws + q.o_stat);
+    l.sum_z = c.smoothing != 0.0f ? (float *)(c.ws + q.o_sumz) : nullptr;
+    l.slots = q.slots;
+    l.z_label = (float *)(c.ws + q.o_zl);
+    l.row = (const HeadRow *)(c.ws + q.o_out);
+    if (c.rows > 0) {
+        launch_logits<T>(c, q.tile, l, false);
+        RowArgs r = {};
+        r.count = count;
+        r.row = row;
+        r.label = label;
+        r.stat = l.stat;
+        r.sum_z = l.sum_z;
+        r.slots = q.slots;
+        r.z_label = l.z_label;
+        r.l2 = l.l2;
+        r.logit_scale = c.logit_scale;
+        r.smoothing = c.smoothing;
+        r.classes = c.classes;
+        r.rows = (int)c.rows;
+        r.grad_loss = c.grad_loss;
+        r.scale = scale;
+        r.loss = c.loss;
+        r.out = grad ? (HeadRow *)(c.ws + q.o_out) : nullptr;
+        launch_stage(ctx, SSDBOX_STAGE_LOSS, head_row_kernel, dim3((unsigned)c.rows), dim3(kRowThreads), r);
+    }
+    if (!grad) return SSDBOX_OK;
+
+    const long long wide = (c.dim + 3) / 4 * 4;
+    for (int i = 0; i < q.pieces; ++i) {
+        const long long first = i * q.piece;
+        const int n_class = (int)(c.classes - first < q.piece ? c.classes - first : q.piece);
+        T *delta = (T *)(c.ws + q.o_delta);
+        if (c.rows > 0) {
+            LogitArgs d = l;
+            d.weight = weight + first * ldw;
+            d.classes = n_class;
+            d.first = (int)first;
+            d.tiles = (n_class + q.bm - 1) / q.bm;
+            d.delta = delta;
+            d.ld_delta = q.piece;
+            launch_logits<T>(c, q.tile, d, true);
+        }
+        GradArgs g = {};
+        g.m = (int)c.dim;
+        g.a_extent = q.pitch;
+        g.scale = scale;
+        g.ldo = c.dim;
+        if (c.grad_hidden && c.rows > 0) {
+            GradArgs h = g;
+            h.a = weight + first * ldw;
+            h.lda = ldw;
+            h.b = delta;
+            h.ldb = q.piece;
+            h.n = (int)c.rows;
+            h.n_count = count;
+            h.k = n_class;
+            h.steps = q.dh_steps;
+            h.out = c.grad_hidden;
+            h.row_of = row;
+            const bool join = q.dh_parts > 1 || q.pieces > 1;
+            if (join) {
+                h.part = (float *)(c.ws + q.o_dh);
+                h.ld_part = wide;
+                h.part_stride = c.rows * wide;
+                h.add = i > 0;
+            }
+            if (q.tile == 0) launch_grad<T, 128, 32, 4, 1, false>(c, h, q.dh_parts);
+            else if (q.tile == 1) launch_grad<T, 128, 128, 2, 2, false>(c, h, q.dh_parts);
+            else if constexpr (sizeof(T) == 2) launch_grad<T, 256, 256, 2, 4, false>(c, h, q.dh_parts);
+            if (join && i == q.pieces - 1) launch_join<T>(c, h, q.dh_parts);
+        }
+        if (c.grad_weight) {
+            GradArgs w = g;
+            w.a = rows;
+            w.lda = q.pitch;
+            w.b = delta;
+            w.ldb = q.piece;
+            w.n = n_class;
+            w.k = (int)c.rows;
+            w.k_count = count;
+            w.steps = q.dw_steps;
+            w.out = (T *)c.grad_weight + first * c.dim;
+            if (q.dw_parts > 1) {
+                w.part = (float *)(c.ws + q.o_dw);
+                w.ld_part = wide;
+                w.part_stride = q.piece * wide;
+            }
+            if (q.tile != 2) launch_grad<T, 128, 128, 2, 2, true>(c, w, q.dw_parts);
+            else if constexpr (sizeof(T) == 2) launch_grad<T, 256, 256, 2, 4, true>(c, w, q.dw_parts);
+            if (q.dw_parts > 1) launch_join<T>(c, w, q.dw_parts);
+        }
+    }
+    return SSDBOX_OK;
+}
+
+int check_sizes(int64_t rows, int64_t classes, int64_t dim, int64_t weight_ld, int dtype, float smoothing)
+{
+    SSD_REQUIRE(dtype == SSDBOX_DTYPE_F32 || dtype == SSDBOX_DTYPE_F16 || dtype == SSDBOX_DTYPE_BF16,
+                "linear_cross_entropy: dtype %d", dtype);
+    SSD_REQUIRE(rows >= 0 && rows <= (1 << 24), "linear_cross_entropy: %lld rows outside [0, 2^24]", (long long)rows);
+    SSD_REQUIRE(classes >= 1 && classes <= (1 << 28), "linear_cross_entropy: %lld classes outside [1, 2^28]",
+                (long long)classes);
+    SSD_REQUIRE(dim >= 1 && dim <= (1 << 20), "linear_cross_entropy: dim %lld outside [1, 2^20]", (long long)dim);
+    SSD_REQUIRE(weight_ld >= dim && weight_ld <= (1 << 21), "linear_cross_entropy: weight row stride %lld outside [%lld, 2^21]",
+                (long long)weight_ld, (long long)dim);
+    SSD_REQUIRE(smoothing >= 0.0f && smoothing < 1.0f, "linear_cross_entropy: label_smoothing %g outside [0, 1)", smoothing);
+    return SSDBOX_OK;
+}
+
+}  // namespace
+
+extern "C" int ssdbox_linear_cross_entropy_workspace(int64_t rows, int64_t classes, int64_t dim, int64_t weight_ld,
+                                                     int dtype, float label_smoothing, int grad_hidden, int grad_weight,
+                                                     size_t *bytes)
+{
+    SSD_REQUIRE(bytes != nullptr, "linear_cross_entropy_workspace: bytes is NULL");
+    int rc = check_sizes(rows, classes, dim, weight_ld, dtype, label_smoothing);
+    if (rc != SSDBOX_OK) return rc;
+    *bytes = make_plan(rows, classes, dim, weight_ld, dtype, label_smoothing, grad_hidden != 0, grad_weight != 0).bytes;
+    return SSDBOX_OK;
+}
+
+extern "C" int ssdbox_linear_cross_entropy(ssdbox_ctx *ctx, const void *d_hidden, int64_t hidden_ld, const void *d_weight,
+                                           int64_t weight_ld, const void *d_labels, int label_bytes, int64_t rows,
+                                           int64_t classes, int64_t dim, int dtype, float logit_scale,
+                                           float label_smoothing, const float *d_grad_loss, float *d_loss,
+                                           void *d_grad_hidden, void *d_grad_weight, void *d_workspace,
+                                           size_t workspace_bytes)
+{
+    SSD_REQUIRE(ctx != nullptr, "linear_cross_entropy: ctx is NULL");
+    int rc = check_sizes(rows, classes, dim, weight_ld, dtype, label_smoothing);
+    if (rc != SSDBOX_OK) return rc;
+    SSD_REQUIRE(label_bytes == 4 || label_bytes == 8, "linear_cross_entropy: labels of %d bytes", label_bytes);
+    SSD_REQUIRE(hidden_ld >= dim, "linear_cross_entropy: hidden row stride %lld below dim %lld", (long long)hidden_ld,
+                (long long)dim);
+    SSD_REQUIRE(logit_scale > 0.0f && logit_scale <= 1e6f, "linear_cross_entropy: logit_scale %g outside (0, 1e6]",
+                logit_scale);
+    SSD_REQUIRE(d_weight && d_workspace && (rows == 0 || (d_hidden && d_labels && d_loss)),
+                "linear_cross_entropy: NULL buffer");
+    const HeadPlan q = make_plan(rows, classes, dim, weight_ld, dtype, label_smoothing, d_grad_hidden != nullptr,
+                                 d_grad_weight != nullptr);
+    SSD_REQUIRE(workspace_bytes >= q.bytes, "linear_cross_entropy: workspace of %zu bytes, %zu needed", workspace_bytes,
+                q.bytes);
+    SSD_REQUIRE(((uintptr_t)d_workspace % 256) == 0 && ((uintptr_t)d_weight % 16) == 0 &&
+                    ((uintptr_t)d_grad_hidden % 16) == 0 && ((uintptr_t)d_grad_weight % 16) == 0,
+                "linear_cross_entropy: weight and gradients have to start at 16 bytes, the workspace at 256");
+    SSD_REQUIRE(q.class_tiles * ((rows + q.bn - 1) / q.bn) < (1ll << 31) &&
+                    (q.pieces == 0 || (dim + q.bm - 1) / q.bm * ((rows + q.bn - 1) / q.bn) < (1ll << 31)),
+                "linear_cross_entropy: %lld rows x %lld classes", (long long)rows, (long long)classes);
+
+    DeviceGuard guard(ctx->device);
+    HeadCall c = {ctx, d_hidden, d_weight, d_labels, hidden_ld, weight_ld, label_bytes, rows, classes, dim, logit_scale,
+                  label_smoothing, d_grad_loss, d_loss, d_grad_hidden, d_grad_weight, (char *)d_workspace};
+    if (dtype == SSDBOX_DTYPE_F32) rc = run_head<float>(c, q, dtype);
+    else if (dtype == SSDBOX_DTYPE_F16) rc = run_head<f16_t>(c, q, dtype);
+    else rc = run_head<bf16_t>(c, q, dtype);
+    if (rc != SSDBOX_OK) return rc;
+    SSD_CHECK_HIP(hipGetLastError());
+    return SSDBOX_OK;
+}

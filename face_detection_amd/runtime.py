@@ -640,8 +640,9 @@ class Session:
     def empty(self, shape, dtype=np.float32):
         if self.use_torch:
             torch = _torch()
-            tdtype = {np.dtype(np.float32): torch.float32, np.dtype(np.int32): torch.int32,
-                      np.dtype(np.uint8): torch.uint8}[np.dtype(dtype)]
+            tdtype = dtype if isinstance(dtype, torch.dtype) else {
+                np.dtype(np.float32): torch.float32, np.dtype(np.int32): torch.int32,
+                np.dtype(np.uint8): torch.uint8, np.dtype(np.float16): torch.float16}[np.dtype(dtype)]
             return torch.empty(tuple(int(s) for s in shape), dtype=tdtype, device="cuda:%d" % self.device)
         return DevArray.empty(self.ctx, shape, dtype)
 

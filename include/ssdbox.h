@@ -35,6 +35,10 @@ extern "C" {
 #define SSDBOX_MAX_BOXES_PER_CELL 16   /* boxes per feature-map cell                        */
 #define SSDBOX_MAX_NMS_LIMIT    4096   /* ranks one top-k + NMS launch pair of the general path takes */
 #define SSDBOX_MAX_GT           4096   /* largest ground-truth count per image              */
+#define SSDBOX_DTYPE_F32           0   /* types of the classifier losses' operands           */
+#define SSDBOX_DTYPE_F16           1
+#define SSDBOX_DTYPE_BF16          2
+#define SSDBOX_MAX_TOP          1024   /* teacher's entries a row of ssdbox_distill_topk     */
 #define SSDBOX_STATIC_SCRATCH_BYTES (4u << 20) /* fixed per-GPU scratch of ssdbox_match_encode_static */
 
 typedef struct ssdbox_ctx ssdbox_ctx;
@@ -280,6 +284,51 @@ int ssdbox_widerface_rows(ssdbox_ctx *ctx, const float *d_dets, const int32_t *d
 int ssdbox_ssd_loss(ssdbox_ctx *ctx, const float *d_y_true, const float *d_y_pred, int batch,
                     int64_t num_anchors, int neg_pos_ratio, int n_neg_min, float alpha,
                     float *d_total, uint8_t *d_keep, float *d_grad);
+
+/* ---- losses of large classifiers (no counterpart in the reference) ------------------------- */
+/* They allocate nothing: the caller brings a workspace (256-byte aligned, of the bytes that the
+ * _workspace call says for the same sizes) which belongs to the call until the work it enqueued is
+ * done, so that calls on several streams, or in several captured graphs, each have their own. */
+
+/* Softmax cross entropy of a linear head, logits = logit_scale * hidden weight^T, without the
+ * (rows, classes) logits ever being stored whole.  d_hidden (rows, dim) and d_weight (classes, dim)
+ * of `dtype`, rows hidden_ld / weight_ld values apart; d_labels (rows) int32 or int64 (label_bytes
+ * 4 or 8).  A row with a negative label is left out: loss 0, no gradient, and its hidden values
+ * are not used.  A label >= classes gives loss NaN and no gradient.
+ *   d_loss (rows): (1 - label_smoothing) nll + label_smoothing * mean over the classes of -log p.
+ *   d_grad_hidden (rows, dim), d_grad_weight (classes, dim), dense, of `dtype`, either or both NULL:
+ *   gradients of sum_n d_grad_loss[n] loss[n], with d_grad_loss NULL of the mean over all rows.
+ * Results do not depend on timing: every sum is taken in a fixed order.  d_weight and the gradients
+ * have to be 16-byte aligned. */
+int ssdbox_linear_cross_entropy_workspace(int64_t rows, int64_t classes, int64_t dim, int64_t weight_ld,
+                                          int dtype, float label_smoothing, int grad_hidden,
+                                          int grad_weight, size_t *bytes);
+int ssdbox_linear_cross_entropy(ssdbox_ctx *ctx, const void *d_hidden, int64_t hidden_ld,
+                                const void *d_weight, int64_t weight_ld, const void *d_labels,
+                                int label_bytes, int64_t rows, int64_t classes, int64_t dim, int dtype,
+                                float logit_scale, float label_smoothing, const float *d_grad_loss,
+                                float *d_loss, void *d_grad_hidden, void *d_grad_weight,
+                                void *d_workspace, size_t workspace_bytes);
+
+/* Distillation from a teacher's top logits.  d_logits (rows, classes) of `dtype`, rows logits_ld
+ * values apart; d_values (rows, top) the teacher's logits and d_index (rows, top) their classes
+ * (int32 or int64: index_bytes 4 or 8), top <= SSDBOX_MAX_TOP.  An index outside [0, classes) or a
+ * value of -infinity is no entry (padding); a class given twice counts with both its shares; a row
+ * without an entry has loss 0 and no gradient.  p = softmax(logits / temperature);
+ * d_teacher_lse NULL: q = softmax of the entries' values / temperature;
+ * d_teacher_lse (rows), the log-sum-exp of ALL the teacher's logits / temperature: q =
+ *   exp(value / temperature - lse), and the classes without an entry form one bucket, which holds
+ *   1 - sum q of the teacher and the sum of p there of the student.
+ *   d_loss (rows): temperature^2 * KL(q || p) over the entries (and the bucket).
+ *   d_grad (rows, classes), dense, of `dtype`, or NULL: gradient of sum_n d_grad_loss[n] loss[n], with
+ *   d_grad_loss NULL of the mean over the rows.
+ * The same inputs give the same bits. */
+int ssdbox_distill_topk_workspace(int64_t rows, int64_t classes, int dtype, size_t *bytes);
+int ssdbox_distill_topk(ssdbox_ctx *ctx, const void *d_logits, int64_t logits_ld, int64_t rows,
+                        int64_t classes, int dtype, const float *d_values, const void *d_index,
+                        int index_bytes, int top, const float *d_teacher_lse, float temperature,
+                        const float *d_grad_loss, float *d_loss, void *d_grad, void *d_workspace,
+                        size_t workspace_bytes);
 
 /* Device self-checks of the building blocks (wave reductions, exp/log against the values
  * in expect_log/expect_exp for the host inputs x_log/x_exp, n each).  Blocks the host.
