@@ -30,7 +30,7 @@ struct DistArgs {
     const void *logits;
     long long ld;
     int rows, classes;
-    int row0;                         // the launch's first row
+    int row0, row_count;              // the launch's rows
     const float *values;
     const void *index;
     int index_bytes, top;
@@ -81,19 +81,27 @@ struct Piece {
     }
 };
 
-// log2 of a positive finite float64 to a float32's relative error of the mantissa's part alone
-SSD_DEV double log2_of(double x)
-{
-    const unsigned long long u = __builtin_bit_cast(unsigned long long, x);
-    const int e = (int)(u >> 52) - 1023;
-    const float m = (float)__builtin_bit_cast(double, (u & 0x000FFFFFFFFFFFFFull) | 0x3FF0000000000000ull);
-    return (double)e + (double)__builtin_amdgcn_logf(m);
-}
-
+// The logarithm of a positive float64 of ordinary size, to about 1e-11 of max(1, |ln x|): x = 2^e m with m in [0.707, 1.414],
+// ln m = 2 artanh((m - 1) / (m + 1)) by its series.  (The library's would hold its many constants in registers over the rows.)
 SSD_DEV double ln_of(double x)
 {
-    if (!(x > 0.0) || x > 1e300) return log(x);
-    return log2_of(x) * kLn2;
+    const unsigned long long u = __builtin_bit_cast(unsigned long long, x);
+    if (!(x >= 0x1p-1000 && x <= 0x1p1000)) return x == 0.0 ? -INFINITY : (x > 0.0 ? INFINITY : x - x + NAN);
+    int e = (int)(u >> 52) - 1023;
+    double m = __builtin_bit_cast(double, (u & 0x000FFFFFFFFFFFFFull) | 0x3FF0000000000000ull);
+    if (m > 1.41421356) {
+        m *= 0.5;
+        e += 1;
+    }
+    const double z = (m - 1.0) / (m + 1.0), w = z * z;
+    double c = 1.0 / 13.0;
+    c = __builtin_fma(c, w, 1.0 / 11.0);
+    c = __builtin_fma(c, w, 1.0 / 9.0);
+    c = __builtin_fma(c, w, 1.0 / 7.0);
+    c = __builtin_fma(c, w, 0.2);
+    c = __builtin_fma(c, w, 1.0 / 3.0);
+    c = __builtin_fma(c, w, 1.0);
+    return __builtin_fma((double)e, kLn2, 2.0 * z * c);
 }
 
 struct Entry {
@@ -110,94 +118,147 @@ SSD_DEV Entry entry_of(const DistArgs &p, long long row, int k)
     return e;
 }
 
-// ---- reductions over THREADS lanes that work on one row
+// ---- reductions.  Within a wave by DPP: rows of 16 shift by 1, 2, 4, 8, two broadcasts join the rows, lane 63 has it all.
+template <int CTRL, int ROWS>
+SSD_DEV float dpp(float x, float none)
+{
+    return u2f((uint32_t)__builtin_amdgcn_update_dpp((int)f2u(none), (int)f2u(x), CTRL, ROWS, 0xf, false));
+}
+template <int CTRL, int ROWS>
+SSD_DEV double dpp(double x)
+{
+    const unsigned long long u = __builtin_bit_cast(unsigned long long, x);
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)u, CTRL, ROWS, 0xf, false);
+    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(u >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+SSD_DEV float wave_max(float x)
+{
+    const float none = -INFINITY;
+    x = fmaxf(x, dpp<0x111, 0xf>(x, none));
+    x = fmaxf(x, dpp<0x112, 0xf>(x, none));
+    x = fmaxf(x, dpp<0x114, 0xf>(x, none));
+    x = fmaxf(x, dpp<0x118, 0xf>(x, none));
+    x = fmaxf(x, dpp<0x142, 0xa>(x, none));
+    x = fmaxf(x, dpp<0x143, 0xc>(x, none));
+    return u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(x), 63));
+}
+SSD_DEV double wave_sum(double x)
+{
+    x += dpp<0x111, 0xf>(x);
+    x += dpp<0x112, 0xf>(x);
+    x += dpp<0x114, 0xf>(x);
+    x += dpp<0x118, 0xf>(x);
+    x += dpp<0x142, 0xa>(x);
+    x += dpp<0x143, 0xc>(x);
+    const unsigned long long u = __builtin_bit_cast(unsigned long long, x);
+    const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)u, 63);
+    const unsigned hi = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)(u >> 32), 63);
+    return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+
+// The waves' values, one in each lane of every eight (or four), joined in all of them.
+template <int WAVES>
+SSD_DEV float waves_max(float x)
+{
+    x = fmaxf(x, dpp<0xB1, 0xf>(x, x));
+    x = fmaxf(x, dpp<0x4E, 0xf>(x, x));
+    if constexpr (WAVES == 8) x = fmaxf(x, dpp<0x141, 0xf>(x, x));
+    return u2f((uint32_t)__builtin_amdgcn_readfirstlane((int)f2u(x)));
+}
+template <int WAVES>
+SSD_DEV double waves_sum(double x)
+{
+    x += dpp<0xB1, 0xf>(x);
+    x += dpp<0x4E, 0xf>(x);
+    if constexpr (WAVES == 8) x += dpp<0x141, 0xf>(x);
+    const unsigned long long u = __builtin_bit_cast(unsigned long long, x);
+    const unsigned lo = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)u);
+    const unsigned hi = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(u >> 32));
+    return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+
+// THREADS lanes (whole waves) that work on one row.  Each reduction of a row has a place of its own in LDS, so that one
+// barrier each is enough.
 template <int THREADS>
 struct Team {
-    static constexpr int kWaves = THREADS / 64 > 0 ? THREADS / 64 : 1;
-    static constexpr int kWidth = THREADS < 64 ? THREADS : 64;
-    double *lds;                      // kWaves * 4, unused by one wave
+    static constexpr int kWaves = THREADS / 64;    // 1, 4 or 8
+    static constexpr int kPlace = kWaves * 4;      // float64 of one reduction
+    double *lds;
 
-    SSD_DEV void sync() const
+    static SSD_DEV void sync()
     {
         if constexpr (THREADS > 64) __syncthreads();
         else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");    // one wave's LDS accesses run in order
     }
-    template <typename F>
-    SSD_DEV void reduce(double (&x)[4], F f) const
+    template <int N>
+    SSD_DEV void maxima(int place, float (&x)[N]) const
     {
 #pragma unroll
-        for (int o = kWidth / 2; o > 0; o >>= 1) {
-            double y[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = __shfl_xor(x[i], o);
-            f(x, y);
-        }
+        for (int i = 0; i < N; ++i) x[i] = wave_max(x[i]);
         if constexpr (THREADS > 64) {
-            const int wave = threadIdx.x >> 6;
-            __syncthreads();
+            float *p = (float *)(lds + place * kPlace);
             if ((threadIdx.x & 63) == 0)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) lds[wave * 4 + i] = x[i];
+                for (int i = 0; i < N; ++i) p[(threadIdx.x >> 6) * N + i] = x[i];
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = lds[i];
-            for (int w = 1; w < kWaves; ++w) {
-                double y[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) y[i] = lds[w * 4 + i];
-                f(x, y);
-            }
+            for (int i = 0; i < N; ++i) x[i] = waves_max<kWaves>(p[(threadIdx.x & (kWaves - 1)) * N + i]);
         }
     }
-    SSD_DEV void maxima(float &a, float &b, float &c) const
+    template <int N>
+    SSD_DEV void sums(int place, double (&x)[N]) const
     {
-        double x[4] = {(double)a, (double)b, (double)c, 0.0};
-        reduce(x, [](double (&l)[4], const double (&r)[4]) {
-            l[0] = fmax(l[0], r[0]);
-            l[1] = fmax(l[1], r[1]);
-            l[2] = fmax(l[2], r[2]);
-        });
-        a = (float)x[0];
-        b = (float)x[1];
-        c = (float)x[2];
-    }
-    SSD_DEV void sums(double (&x)[4]) const
-    {
-        reduce(x, [](double (&l)[4], const double (&r)[4]) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) l[i] += r[i];
-        });
+        for (int i = 0; i < N; ++i) x[i] = wave_sum(x[i]);
+        if constexpr (THREADS > 64) {
+            double *p = lds + place * kPlace;
+            if ((threadIdx.x & 63) == 0)
+#pragma unroll
+                for (int i = 0; i < N; ++i) p[(threadIdx.x >> 6) * N + i] = x[i];
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] = waves_sum<kWaves>(p[(threadIdx.x & (kWaves - 1)) * N + i]);
+        }
     }
 };
 
-// What a row's statistics make of an entry and of the classes outside.
+// What a row's statistics make of an entry and of the classes outside.  All exponentials of a row are 2^((z - sub) l2 - off)
+// with the same float32 l2, and its logarithms take that l2 too: what l2 and off lack in their last place then cancels,
+// however far from 0 the logits lie.
 struct RowTerms {
-    float m, l2;                      // exp(u - max) = exp2((z - m) l2)
+    float sub, off, l2;
     double ln_s, inv_s;
     double t_top, ln_t;               // log q = (t - t_top) / tau - ln_t
     double inv_tau;
     double whole;                     // Q + q_r
-    float ref, out;                   // outside: grad = exp2((z - ref) l2) * out
+    float osub, out;                  // outside: grad = 2^((z - osub) l2 - off) out
     float c;                          // g tau
 
     SSD_DEV double log_q(float t) const { return ((double)t - t_top) * inv_tau - ln_t; }
-    SSD_DEV double log_p(float z) const { return ((double)z - (double)m) * inv_tau - ln_s; }
+    SSD_DEV double log_p(float z) const { return (((double)z - (double)sub) * (double)l2 - (double)off) * kLn2 - ln_s; }
     SSD_DEV float q(float t) const { return __builtin_amdgcn_exp2f((float)(log_q(t) * kLog2eD)); }
-    SSD_DEV float share(float z) const { return (float)((double)__builtin_amdgcn_exp2f((z - m) * l2) * inv_s); }
+    SSD_DEV float power(float z) const { return __builtin_amdgcn_exp2f(__builtin_fmaf(z - sub, l2, -off)); }
+    SSD_DEV float share(float z) const { return (float)((double)power(z) * inv_s); }
 };
 
-// The k-th entry's terms: (q, loss, p where it is the class's first).  dup: some class is given twice in this row.
-SSD_DEV void add_entry(double (&sum)[4], const RowTerms &r, const DistArgs &p, long long row, int k, const Entry &e, float z,
+// Whether the k-th entry is its class's first.  dup: some class is given twice in this row.
+SSD_DEV bool first_of(const DistArgs &p, long long row, int k, const Entry &e, bool dup)
+{
+    if (dup)
+        for (int j = 0; j < k; ++j)
+            if (entry_of(p, row, j).at == e.at) return false;
+    return true;
+}
+
+// The k-th entry's terms: (q, loss, p where it is the class's first).
+SSD_DEV void add_entry(double (&sum)[3], const RowTerms &r, const DistArgs &p, long long row, int k, const Entry &e, float z,
                        bool dup)
 {
     const float q = r.q(e.t);
     sum[0] += (double)q;
     if (q != 0.0f) sum[1] += (double)q * (r.log_q(e.t) - r.log_p(z));
-    if (!p.teacher_lse) return;
-    if (dup)
-        for (int j = 0; j < k; ++j)
-            if (entry_of(p, row, j).at == e.at) return;
-    sum[2] += (double)r.share(z);
+    if (p.teacher_lse && first_of(p, row, k, e, dup)) sum[2] += (double)r.share(z);
 }
 
 // What the teacher gives a class: of all its entries, in their order.
@@ -225,11 +286,11 @@ SSD_DEV void terms_teacher(RowTerms &r, const DistArgs &p, long long row, float 
 }
 
 // The row's loss from the sums over its entries (sum_p: of p over the classes they name), and the outside's factor.
+// so: of the classes outside, relative to osub.
 SSD_DEV double terms_finish(RowTerms &r, const DistArgs &p, long long row, double sum_q, double sum_loss, double sum_p,
-                            float m, double s, float mo, double so, bool outside)
+                            float osub, double so, bool outside)
 {
-    r.m = m;
-    r.ref = m;
+    r.osub = r.sub;
     const double g = p.grad_loss ? (double)p.grad_loss[row] : 1.0 / (double)p.rows;
     r.c = (float)(g * (double)p.tau);
     r.whole = sum_q;
@@ -238,15 +299,15 @@ SSD_DEV double terms_finish(RowTerms &r, const DistArgs &p, long long row, doubl
         double q_r = 1.0 - sum_q;
         if (q_r < 0.0) q_r = 0.0;
         if (outside && so > 0.0) {
-            r.ref = mo;
+            r.osub = osub;
             r.whole = sum_q + q_r;
             if (q_r > 0.0) {
-                // near 1 a bucket's logarithm is what the entries leave of it, to their own relative error
-                const double ln_pr = sum_p < 0.5 ? log1p(-sum_p)
-                                                 : ((double)mo - (double)m) * r.inv_tau + log(so) - log(s);
-                loss += q_r * ((sum_q < 0.5 ? log1p(-sum_q) : log(q_r)) - ln_pr);
+                // near 1 a bucket is what the entries leave of it, to their own relative error
+                const double ln_pr = sum_p < 0.5 ? ln_of(1.0 - sum_p)
+                                                 : ((double)osub - (double)r.sub) * (double)r.l2 * kLn2 + ln_of(so) - r.ln_s;
+                loss += q_r * (ln_of(q_r) - ln_pr);
             }
-            const double down = (double)__builtin_amdgcn_exp2f((mo - m) * r.l2);
+            const double down = (double)__builtin_amdgcn_exp2f((osub - r.sub) * r.l2);
             out = r.whole * r.inv_s * down - q_r / so;
         }
     }
@@ -255,136 +316,256 @@ SSD_DEV double terms_finish(RowTerms &r, const DistArgs &p, long long row, doubl
 }
 
 // ------------------------------------------------------------------- a team of lanes a row
-// TEAM lanes a row, R pieces of 16 bytes a lane.
+// TEAM lanes a row: R pieces of 16 bytes a lane, TEAM apart, and of what is left beyond the last whole piece a value a lane.
+// Each team takes rows a grid apart and asks for the next row's pieces as the gradient of this one leaves their registers (the
+// longest rows fill the registers: one row a workgroup).
+//
+// Any reference near the row's maximum serves its exponentials: float32 holds 2^126 both ways.  The largest of the
+// teacher's classes' logits is at hand before the row has arrived, so the row's maximum is taken, from memory again, only where
+// the sum says that the reference was far off (or a mask's lowest value overflowed the product).
+//
+// The registers are only ever loaded and read: a piece that holds one of the teacher's classes is summed without them where
+// they are not part of the outside bucket, and their gradients are written after the others'.
+template <typename T, int TEAM, int R>
+struct RowPieces {
+    static constexpr int N = 16 / (int)sizeof(T);
+    struct __attribute__((packed, aligned(sizeof(T)))) Raw { unsigned w[4]; };
+    struct X { unsigned w[4]; };
+    X x[R];
+    float rest;
+    int whole, more, t;               // whole pieces, values beyond them, this lane
+
+    // limit: pieces to be read; the lanes beyond read the first piece (a load without a branch leaves the registers in place)
+    SSD_DEV void load(int r, const T *z, int limit)
+    {
+        const int i = r * TEAM + t;
+        const Raw q = *(const Raw *)((const char *)z + (unsigned)(i < limit ? i : 0) * 16u);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[r].w[j] = q.w[j];
+    }
+    SSD_DEV void load_rest(const T *z) { rest = t < more ? (float)z[whole * N + t] : -INFINITY; }
+    SSD_DEV float value(int r, int i) const
+    {
+        if constexpr (sizeof(T) == 4) return u2f(x[r].w[i]);
+        const unsigned w = x[r].w[i >> 1];
+        if constexpr (__is_same(T, bf16_t)) return u2f(i & 1 ? w & 0xFFFF0000u : w << 16);
+        return (float)__builtin_bit_cast(f16_t, (unsigned short)(i & 1 ? w >> 16 : w & 0xFFFFu));
+    }
+    // Before each use of a piece: keeps the compiler from holding the float32 values of one pass for the next (twice the
+    // registers of 16-bit rows) and from working on many pieces at once.
+    SSD_DEV void forget(int r)
+    {
+        asm volatile("" : "+v"(x[r].w[0]), "+v"(x[r].w[1]), "+v"(x[r].w[2]), "+v"(x[r].w[3]), "+v"(t));
+        __builtin_amdgcn_sched_barrier(0);
+    }
+};
+
 template <typename T, int TEAM, int R>
 __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void distill_row_kernel(const DistArgs p)
 {
-    typedef Piece<T> P;
+    typedef RowPieces<T, TEAM, R> V;
+    constexpr int N = V::N;
     constexpr int kBlockThreads = TEAM < 256 ? 256 : TEAM;
     constexpr int kRows = kBlockThreads / TEAM;
-    constexpr int kWords = TEAM * R * P::N / 32;
+    constexpr int kWords = (TEAM * R + 1) * N / 32 + 1;
     __shared__ unsigned s_bits[kRows * kWords];
-    __shared__ double s_red[kBlockThreads / 64 * 4];
+    __shared__ double s_red[4 * Team<TEAM>::kPlace];
     const int t = threadIdx.x % TEAM;
-    const long long row = p.row0 + (long long)blockIdx.x * kRows + threadIdx.x / TEAM;
-    if (row >= p.rows) return;                            // whole waves: a team is a wave or the workgroup
-    unsigned *bits = s_bits + threadIdx.x / TEAM * kWords;
+    const int mine = TEAM < 256 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TEAM) : 0;
+    long long row = p.row0 + (long long)blockIdx.x * kRows + mine;
+    const long long end = p.row0 + p.row_count, step = (long long)gridDim.x * kRows;
+    if (row >= end) return;                               // whole waves: a team is a wave or the workgroup
+    unsigned *bits = s_bits + mine * kWords;
     const Team<TEAM> team = {s_red};
+    const bool tail = p.teacher_lse != nullptr;
+    constexpr bool kLoop = R == 32;
+    V v;
+    v.t = t;
+    v.whole = p.classes / N;
+    v.more = p.classes - v.whole * N;
     const T *z = (const T *)p.logits + row * p.ld;
 
-    P x[R];
+    // a lane's first entry stays in registers; further ones (more than TEAM) are read again each time
+    Entry e0 = {-1, -INFINITY};
+    if (t < p.top) e0 = entry_of(p, row, t);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int at = (r * TEAM + t) * P::N;
-        x[r].load(z + at, p.classes - at);
-    }
-    for (int i = t; i < (p.classes + 31) / 32; i += TEAM) bits[i] = 0u;
-    team.sync();
-    float m = -INFINITY, mo = -INFINITY, t_top = -INFINITY;
-    int twice = 0, inside = 0;
-    for (int k = t; k < p.top; k += TEAM) {
-        const Entry e = entry_of(p, row, k);
-        if (e.at < 0) continue;
-        t_top = fmaxf(t_top, e.t);
-        const unsigned bit = 1u << (e.at & 31);
-        if (atomicOr(&bits[e.at >> 5], bit) & bit) twice = 1;
-        else ++inside;
-    }
-    team.sync();
-    const bool tail = p.teacher_lse != nullptr;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int at = (r * TEAM + t) * P::N;
-        const unsigned in = tail && at < p.classes ? bits[at >> 5] >> (at & 31) : 0u;
-#pragma unroll
-        for (int i = 0; i < P::N; ++i) {
-            const float v = (float)x[r].v[i];
-            m = fmaxf(m, v);
-            if (tail && !(in >> i & 1u)) mo = fmaxf(mo, v);
-        }
-    }
-    team.maxima(m, mo, t_top);
+    for (int r = 0; r < R; ++r) v.load(r, z, v.whole);
+    v.load_rest(z);
+    for (int i = t; i < kWords; i += TEAM) bits[i] = 0u;
+    Team<TEAM>::sync();
     RowTerms f;
     f.l2 = (float)(kLog2eD / (double)p.tau);
-    const float mref = m == -INFINITY ? 0.0f : m, oref = mo == -INFINITY ? 0.0f : mo;
-    float s = 0.0f, so = 0.0f, st = 0.0f;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int at = (r * TEAM + t) * P::N;
-        const unsigned in = tail && at < p.classes ? bits[at >> 5] >> (at & 31) : 0u;
-#pragma unroll
-        for (int i = 0; i < P::N; ++i) {
-            const float v = (float)x[r].v[i];
-            s += __builtin_amdgcn_exp2f((v - mref) * f.l2);
-            if (tail && !(in >> i & 1u)) so += __builtin_amdgcn_exp2f((v - oref) * f.l2);
-        }
-    }
-    if (!tail)
+
+    for (;;) {
+        const float z0 = e0.at >= 0 ? (float)z[e0.at] : -INFINITY;
+        const auto entry = [&](int k) { return k == t ? e0 : entry_of(p, row, k); };
+        const auto logit = [&](int k, const Entry &e) { return k == t ? z0 : (float)z[e.at]; };
+        float top[2] = {-INFINITY, -INFINITY};             // of the entries' logits, of the teacher's
+        int entries = 0, inside = 0;
+        bool first0 = false;
         for (int k = t; k < p.top; k += TEAM) {
-            const Entry e = entry_of(p, row, k);
-            if (e.at >= 0) st += __builtin_amdgcn_exp2f((e.t - t_top) * f.l2);
-        }
-    double sum[4] = {(double)s, (double)so, (double)st, (double)inside + 65536.0 * (double)twice};
-    team.sums(sum);
-    const int n_inside = (int)sum[3] % 65536;
-    const bool dup = sum[3] >= 65536.0;
-    if (n_inside == 0) {                                   // a row without an entry teaches nothing
-        if (t == 0) p.loss[row] = 0.0f;
-        if (p.grad) {
-            P zero;
-#pragma unroll
-            for (int i = 0; i < P::N; ++i) zero.v[i] = (T)0.0f;
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const int at = (r * TEAM + t) * P::N;
-                zero.store((T *)p.grad + row * p.classes + at, p.classes - at);
+            const Entry e = entry(k);
+            if (e.at < 0) continue;
+            top[0] = fmaxf(top[0], logit(k, e));
+            top[1] = fmaxf(top[1], e.t);
+            const unsigned bit = 1u << (e.at & 31);
+            ++entries;
+            if (!(atomicOr(&bits[e.at >> 5], bit) & bit)) {
+                ++inside;
+                if (k == t) first0 = true;
             }
         }
-        return;
-    }
-    f.m = m;
-    f.inv_s = 1.0 / sum[0];
-    f.ln_s = ln_of(sum[0]);
-    terms_teacher(f, p, row, t_top, sum[2]);
-    double of_entries[4] = {0.0, 0.0, 0.0, 0.0};
-    for (int k = t; k < p.top; k += TEAM) {
-        const Entry e = entry_of(p, row, k);
-        if (e.at < 0) continue;
-        add_entry(of_entries, f, p, row, k, e, (float)z[e.at], dup);
-    }
-    team.sums(of_entries);
-    const double loss = terms_finish(f, p, row, of_entries[0], of_entries[1], of_entries[2], m, sum[0], mo, sum[1],
-                                     n_inside < p.classes);
-    if (t == 0) p.loss[row] = (float)loss;
-    if (!p.grad) return;
-    T *g = (T *)p.grad + row * p.classes;
+        team.template maxima<2>(0, top);                   // its barrier shows the bits as well
+        if constexpr (TEAM == 64) Team<TEAM>::sync();
+        f.sub = 0.0f;
+        f.off = top[0] == -INFINITY ? 0.0f : fmaxf(top[0] * f.l2, -3e38f);
+        const float off = f.off;
+        float osub = 0.0f, so = 0.0f;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int at = (r * TEAM + t) * P::N;
-        P o;
+        for (int r = 0; r < R; ++r) {
+            v.forget(r);
+            const int i = r * TEAM + v.t;
+            if (i < v.whole) {
+                const unsigned in = tail ? bits[i * N >> 5] >> (i * N & 31) & ((1u << N) - 1u) : 0u;
+                float e[N];
 #pragma unroll
-        for (int i = 0; i < P::N; ++i)
-            o.v[i] = (T)(__builtin_amdgcn_exp2f(((float)x[r].v[i] - f.ref) * f.l2) * f.out);
-        o.store(g + at, p.classes - at);
-    }
-    team.sync();                                           // the entries' own values come last
-    for (int k = t; k < p.top; k += TEAM) {
-        const Entry e = entry_of(p, row, k);
-        if (e.at < 0) continue;
-        const double q = teacher_of(f, p, row, e, dup);
-        g[e.at] = (T)(float)((double)f.c * ((double)f.share((float)z[e.at]) * f.whole - q));
+                for (int j = 0; j < N; ++j) e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(v.value(r, j), f.l2, -off));
+                if (in)
+#pragma unroll
+                    for (int j = 0; j < N; ++j) e[j] = in >> j & 1u ? 0.0f : e[j];
+#pragma unroll
+                for (int j = 0; j < N; ++j) so += e[j];
+            }
+        }
+        const int last = v.whole * N + t;
+        if (t < v.more && !(tail && (bits[last >> 5] >> (last & 31) & 1u)))
+            so += __builtin_amdgcn_exp2f(__builtin_fmaf(v.rest, f.l2, -off));
+        double sum[4] = {(double)so, 0.0, (double)inside + 65536.0 * (double)entries, 0.0};
+        if (tail) {
+            if (first0) sum[3] = (double)f.power(z0);
+        } else {
+            for (int k = t; k < p.top; k += TEAM) {
+                const Entry e = entry(k);
+                if (e.at >= 0) sum[1] += (double)__builtin_amdgcn_exp2f((e.t - top[1]) * f.l2);
+            }
+        }
+        team.template sums<4>(1, sum);
+        const int n_entries = (int)(sum[2] / 65536.0), n_inside = (int)(sum[2] - 65536.0 * n_entries);
+        const bool dup = n_entries > n_inside, outside = n_inside < p.classes;
+        // (a bucket without a class needs no reference: its sum of 0 is right)
+        const bool slow = n_inside == 0 || (!(sum[0] > 0x1p-60 && sum[0] < 0x1p120) && (!tail || outside));
+        if (slow && n_inside > 0) {
+            float most[1] = {-INFINITY};
+            for (int i = t; i < p.classes; i += TEAM)
+                if (!tail || !(bits[i >> 5] >> (i & 31) & 1u)) most[0] = fmaxf(most[0], (float)z[i]);
+            team.template maxima<1>(3, most);
+            f.off = 0.0f;
+            f.sub = tail ? fmaxf(most[0], top[0]) : most[0];
+            if (f.sub == -INFINITY) f.sub = 0.0f;
+            osub = most[0] == -INFINITY ? 0.0f : most[0];
+            double again[1] = {0.0};
+            for (int i = t; i < p.classes; i += TEAM)
+                if (!tail || !(bits[i >> 5] >> (i & 31) & 1u))
+                    again[0] += (double)__builtin_amdgcn_exp2f(((float)z[i] - osub) * f.l2);
+            if constexpr (TEAM > 64) __syncthreads();      // place 3's maxima have been read
+            team.template sums<1>(3, again);
+            sum[0] = again[0];
+        }
+        for (int k = t; k < p.top; k += TEAM) {            // the bits are clear again for the next row
+            const Entry e = entry(k);
+            if (e.at >= 0) bits[e.at >> 5] = 0u;
+        }
+        const long long next = row + step;
+        const bool goes_on = kLoop && next < end;
+        const T *zn = goes_on ? z + step * p.ld : z;
+        const int limit = goes_on ? v.whole : 0;
+        Entry en = {-1, -INFINITY};
+        if (goes_on && t < p.top) en = entry_of(p, next, t);
+
+        double s = sum[0];
+        if (tail) {
+            double in[1] = {sum[3]};
+            if (slow || dup || p.top > TEAM) {
+                in[0] = 0.0;
+                for (int k = t; k < p.top; k += TEAM) {
+                    const Entry e = entry(k);
+                    if (e.at >= 0 && first_of(p, row, k, e, dup)) in[0] += (double)f.power(logit(k, e));
+                }
+                team.template sums<1>(0, in);
+            }
+            s = in[0] + s * (double)__builtin_amdgcn_exp2f((osub - f.sub) * f.l2);
+        }
+        f.inv_s = 1.0 / s;
+        f.ln_s = ln_of(s);
+        terms_teacher(f, p, row, top[1], sum[1]);
+        double of_entries[3] = {0.0, 0.0, 0.0};
+        for (int k = t; k < p.top; k += TEAM) {
+            const Entry e = entry(k);
+            if (e.at >= 0) add_entry(of_entries, f, p, row, k, e, logit(k, e), dup);
+        }
+        team.template sums<3>(2, of_entries);
+        const double loss = terms_finish(f, p, row, of_entries[0], of_entries[1], of_entries[2], osub, sum[0], outside);
+        if (t == 0) p.loss[row] = n_inside > 0 ? (float)loss : 0.0f;      // a row without an entry teaches nothing
+        T *g = (T *)p.grad + row * p.classes;
+        if (p.grad && !slow) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                v.forget(r);
+                const int i = r * TEAM + v.t;
+                if (i < v.whole) {
+                    Piece<T> o;
+#pragma unroll
+                    for (int j = 0; j < N; ++j)
+                        o.v[j] = (T)(__builtin_amdgcn_exp2f(__builtin_fmaf(v.value(r, j), f.l2, -off)) * f.out);
+                    o.store((T *)((char *)g + (unsigned)i * 16u), N);
+                }
+                if constexpr (kLoop) v.load(r, zn, limit);
+            }
+            if (t < v.more)
+                g[v.whole * N + t] = (T)(__builtin_amdgcn_exp2f(__builtin_fmaf(v.rest, f.l2, -off)) * f.out);
+        } else {
+            if (p.grad)
+                for (int i = t; i < p.classes; i += TEAM)
+                    g[i] = (T)(n_inside > 0 ? __builtin_amdgcn_exp2f(((float)z[i] - f.osub) * f.l2) * f.out : 0.0f);
+            if constexpr (kLoop)
+#pragma unroll
+                for (int r = 0; r < R; ++r) v.load(r, zn, limit);
+        }
+        if constexpr (kLoop) v.load_rest(zn);
+        if (p.grad) {
+            Team<TEAM>::sync();                            // the entries' own values come last
+            for (int k = t; k < p.top; k += TEAM) {
+                const Entry e = entry(k);
+                if (e.at < 0) continue;
+                const double q = teacher_of(f, p, row, e, dup);
+                g[e.at] = (T)(float)((double)f.c * ((double)f.share(logit(k, e)) * f.whole - q));
+            }
+        }
+        if (!goes_on) return;
+        row = next;
+        z = zn;
+        e0 = en;
     }
 }
 
 // ----------------------------------------------------------------------- few classes a row
 // G lanes a row, up to 4 classes a lane.
+template <int G, typename X, typename F>
+SSD_DEV X group(X x, F f)
+{
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) x = f(x, __shfl_xor(x, o));
+    return x;
+}
+
 template <typename T, int G>
 __global__ __launch_bounds__(256) void distill_small_kernel(const DistArgs p)
 {
     const int l = threadIdx.x % G;
     const long long row = p.row0 + ((long long)blockIdx.x * 256 + threadIdx.x) / G;
     if (row >= p.rows) return;                             // whole teams
-    const Team<G> team = {nullptr};
+    const auto more = [](float a, float b) { return fmaxf(a, b); };
+    const auto plus = [](double a, double b) { return a + b; };
     const T *z = (const T *)p.logits + row * p.ld;
     float x[4];
     float m = -INFINITY, mo = -INFINITY, t_top = -INFINITY;
@@ -408,19 +589,20 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const DistArgs p)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         if (!(in >> i & 1u)) mo = fmaxf(mo, x[i]);
-    float unused = t_top;
-    team.maxima(m, mo, unused);
+    m = group<G>(m, more);
+    mo = group<G>(mo, more);
     RowTerms f;
     f.l2 = (float)(kLog2eD / (double)p.tau);
     const float mref = m == -INFINITY ? 0.0f : m, oref = mo == -INFINITY ? 0.0f : mo;
-    double sum[4] = {0.0, 0.0, 0.0, 0.0};
+    double sum[3] = {0.0, 0.0, 0.0};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         sum[0] += (double)__builtin_amdgcn_exp2f((x[i] - mref) * f.l2);
         if (!(in >> i & 1u)) sum[1] += (double)__builtin_amdgcn_exp2f((x[i] - oref) * f.l2);
         sum[2] += (double)(in >> i & 1u);
     }
-    team.sums(sum);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) sum[i] = group<G>(sum[i], plus);
     T *g = (T *)p.grad + row * p.classes;
     if (entries == 0) {
         if (l == 0) p.loss[row] = 0.0f;
@@ -436,11 +618,12 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const DistArgs p)
             const Entry e = entry_of(p, row, k);
             if (e.at >= 0) st += (double)__builtin_amdgcn_exp2f((e.t - t_top) * f.l2);
         }
-    f.m = m;
+    f.sub = mref;
+    f.off = 0.0f;
     f.inv_s = 1.0 / sum[0];
     f.ln_s = ln_of(sum[0]);
     terms_teacher(f, p, row, t_top, st);
-    double of_entries[4] = {0.0, 0.0, 0.0, 0.0}, q_at[4] = {0.0, 0.0, 0.0, 0.0};
+    double of_entries[3] = {0.0, 0.0, 0.0}, q_at[4] = {0.0, 0.0, 0.0, 0.0};
     const bool dup = entries > (int)sum[2];
     for (int k = 0; k < p.top; ++k) {
         const Entry e = entry_of(p, row, k);
@@ -450,7 +633,7 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const DistArgs p)
         for (int i = 0; i < 4; ++i)
             if (e.at == l + G * i) q_at[i] += (double)f.q(e.t);
     }
-    const double loss = terms_finish(f, p, row, of_entries[0], of_entries[1], of_entries[2], m, sum[0], mo, sum[1],
+    const double loss = terms_finish(f, p, row, of_entries[0], of_entries[1], of_entries[2], oref, sum[1],
                                      (int)sum[2] < p.classes);
     if (l == 0) p.loss[row] = (float)loss;
     if (!p.grad) return;
@@ -459,7 +642,7 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const DistArgs p)
         const int j = l + G * i;
         if (j >= p.classes) continue;
         const float o = (in >> i & 1u) ? (float)((double)f.c * ((double)f.share(x[i]) * f.whole - q_at[i]))
-                                       : __builtin_amdgcn_exp2f((x[i] - f.ref) * f.l2) * f.out;
+                                       : __builtin_amdgcn_exp2f((x[i] - f.osub) * f.l2) * f.out;
         g[j] = (T)o;
     }
 }
@@ -492,7 +675,7 @@ __global__ __launch_bounds__(kSegThreads) void distill_part_kernel(const DistArg
     typedef Piece<T> P;
     constexpr int R = kSegMost / kSegThreads;
     __shared__ unsigned s_bits[kSegMost * P::N / 32];
-    __shared__ double s_red[kSegThreads / 64 * 4];
+    __shared__ double s_red[3 * Team<kSegThreads>::kPlace];
     const int t = threadIdx.x, seg = blockIdx.x % p.segments;
     const long long row = p.row0 + blockIdx.x / p.segments;
     const int first = seg * p.seg_pieces * P::N;
@@ -517,7 +700,7 @@ __global__ __launch_bounds__(kSegThreads) void distill_part_kernel(const DistArg
         if (!(atomicOr(&s_bits[at >> 5], bit) & bit)) ++inside;
     }
     __syncthreads();
-    float m = -INFINITY, mo = -INFINITY, none = 0.0f;
+    float m = -INFINITY, mo = -INFINITY;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const int at = (r * kSegThreads + t) * P::N;
@@ -529,7 +712,10 @@ __global__ __launch_bounds__(kSegThreads) void distill_part_kernel(const DistArg
             if (tail && !(in >> i & 1u)) mo = fmaxf(mo, v);
         }
     }
-    team.maxima(m, mo, none);
+    float top[2] = {m, mo};
+    team.template maxima<2>(0, top);
+    m = top[0];
+    mo = top[1];
     const float l2 = (float)(kLog2eD / (double)p.tau);
     const float mref = m == -INFINITY ? 0.0f : m, oref = mo == -INFINITY ? 0.0f : mo;
     float s = 0.0f, so = 0.0f;
@@ -544,8 +730,8 @@ __global__ __launch_bounds__(kSegThreads) void distill_part_kernel(const DistArg
             if (tail && !(in >> i & 1u)) so += __builtin_amdgcn_exp2f((v - oref) * l2);
         }
     }
-    double sum[4] = {(double)s, (double)so, (double)inside, 0.0};
-    team.sums(sum);
+    double sum[3] = {(double)s, (double)so, (double)inside};
+    team.template sums<3>(1, sum);
     if (t == 0) p.part[row * p.segments + seg] = DistPart{m, mo, sum[0], sum[1], here - (int)sum[2], 0};
 }
 
@@ -555,7 +741,7 @@ __global__ __launch_bounds__(kSegThreads) void distill_segment_kernel(const Dist
 {
     typedef Piece<T> P;
     constexpr int R = kSegMost / kSegThreads;
-    __shared__ double s_red[kSegThreads / 64 * 4];
+    __shared__ double s_red[3 * Team<kSegThreads>::kPlace];
     __shared__ DistPart s_part[kSegThreads];
     const int each = p.grad ? p.segments : 1;
     const int t = threadIdx.x, seg = blockIdx.x % each;
@@ -582,7 +768,7 @@ __global__ __launch_bounds__(kSegThreads) void distill_segment_kernel(const Dist
         __syncthreads();
     }
     const DistPart all = s_part[0];
-    float t_top = -INFINITY, a = 0.0f, b = 0.0f;
+    float t_top = -INFINITY;
     int entries = 0;
     for (int k = t; k < p.top; k += kSegThreads) {
         const Entry e = entry_of(p, row, k);
@@ -590,14 +776,16 @@ __global__ __launch_bounds__(kSegThreads) void distill_segment_kernel(const Dist
         ++entries;
         t_top = fmaxf(t_top, e.t);
     }
-    team.maxima(t_top, a, b);
-    double sum[4] = {(double)entries, 0.0, 0.0, 0.0};
+    float most[1] = {t_top};
+    team.template maxima<1>(0, most);
+    t_top = most[0];
+    double sum[2] = {(double)entries, 0.0};
     if (!p.teacher_lse)
         for (int k = t; k < p.top; k += kSegThreads) {
             const Entry e = entry_of(p, row, k);
             if (e.at >= 0) sum[1] += (double)__builtin_amdgcn_exp2f((e.t - t_top) * f.l2);
         }
-    team.sums(sum);
+    team.template sums<2>(1, sum);
     T *g = (T *)p.grad + row * p.classes + first;
     if (sum[0] == 0.0) {
         if (t == 0 && seg == 0) p.loss[row] = 0.0f;
@@ -613,19 +801,21 @@ __global__ __launch_bounds__(kSegThreads) void distill_segment_kernel(const Dist
         }
         return;
     }
-    f.m = all.m;
+    f.sub = all.m == -INFINITY ? 0.0f : all.m;
+    f.off = 0.0f;
     f.inv_s = 1.0 / all.s;
     f.ln_s = ln_of(all.s);
     terms_teacher(f, p, row, t_top, sum[1]);
     const bool dup = sum[0] > (double)(p.classes - all.outside);
-    double of_entries[4] = {0.0, 0.0, 0.0, 0.0};
+    double of_entries[3] = {0.0, 0.0, 0.0};
     for (int k = t; k < p.top; k += kSegThreads) {
         const Entry e = entry_of(p, row, k);
         if (e.at < 0) continue;
         add_entry(of_entries, f, p, row, k, e, (float)zr[e.at], dup);
     }
-    team.sums(of_entries);
-    const double loss = terms_finish(f, p, row, of_entries[0], of_entries[1], of_entries[2], all.m, all.s, all.mo, all.so,
+    team.template sums<3>(2, of_entries);
+    const double loss = terms_finish(f, p, row, of_entries[0], of_entries[1], of_entries[2],
+                                     all.mo == -INFINITY ? 0.0f : all.mo, all.so,
                                      all.outside > 0);
     if (t == 0 && seg == 0) p.loss[row] = (float)loss;
     if (!p.grad) return;
@@ -635,7 +825,7 @@ __global__ __launch_bounds__(kSegThreads) void distill_segment_kernel(const Dist
         P o;
 #pragma unroll
         for (int i = 0; i < P::N; ++i)
-            o.v[i] = (T)(__builtin_amdgcn_exp2f(((float)x[r].v[i] - f.ref) * f.l2) * f.out);
+            o.v[i] = (T)(__builtin_amdgcn_exp2f(((float)x[r].v[i] - f.osub) * f.l2) * f.out);
         o.store(g + at, here - at);
     }
     __syncthreads();
@@ -661,7 +851,7 @@ DistPlan dist_plan(long long rows, long long classes)
     constexpr int N = 16 / (int)sizeof(T);
     const long long pieces = (classes + N - 1) / N;
     DistPlan q = {};
-    q.cut = pieces > 2048 || (rows < 128 && pieces > 512);
+    q.cut = pieces > 512 * 50;
     if (q.cut) {
         long long segs = (pieces + kSegMost - 1) / kSegMost;
         while (segs * rows < 512 && pieces / (segs * 2) >= kSegThreads) segs *= 2;
@@ -677,7 +867,10 @@ template <typename T, int TEAM, int R>
 void launch_row(ssdbox_ctx *ctx, const DistArgs &a, int rows)
 {
     constexpr int kThreads = TEAM < 256 ? 256 : TEAM;
-    const unsigned grid = (unsigned)((rows + kThreads / TEAM - 1) / (kThreads / TEAM));
+    // as many workgroups as the registers let run at once: each goes on to its next row with the loads in flight
+    constexpr int kEach = TEAM == 512 ? (R <= 8 ? 2 : 1) : 4;
+    const int most = R == 32 ? ctx->num_cus * kEach : rows, need = (rows + kThreads / TEAM - 1) / (kThreads / TEAM);
+    const unsigned grid = (unsigned)(need < most ? need : most);
     launch_stage(ctx, SSDBOX_STAGE_LOSS, distill_row_kernel<T, TEAM, R>, dim3(grid), dim3(kThreads), a);
 }
 
@@ -708,7 +901,11 @@ void launch_distill(ssdbox_ctx *ctx, const DistArgs &a, const DistPlan &q, int r
     else if (pieces <= 256) launch_row<T, 64, 4>(ctx, a, rows);
     else if (pieces <= 512) launch_row<T, 256, 2>(ctx, a, rows);
     else if (pieces <= 1024) launch_row<T, 256, 4>(ctx, a, rows);
-    else launch_row<T, 256, 8>(ctx, a, rows);
+    else if (pieces <= 2048) launch_row<T, 256, 8>(ctx, a, rows);
+    else if (pieces <= 4096) launch_row<T, 512, 8>(ctx, a, rows);
+    else if (pieces <= 8192) launch_row<T, 512, 16>(ctx, a, rows);
+    else if (pieces <= 16384) launch_row<T, 512, 32>(ctx, a, rows);
+    else launch_row<T, 512, 50>(ctx, a, rows);
 }
 
 template <typename T>
@@ -720,7 +917,8 @@ void run_distill(ssdbox_ctx *ctx, DistArgs a, const DistPlan &q)
     a.seg_pieces = q.seg_pieces;
     for (long long r = 0; r < a.rows; r += step) {
         a.row0 = (int)r;
-        launch_distill<T>(ctx, a, q, (int)(a.rows - r < step ? a.rows - r : step));
+        a.row_count = (int)(a.rows - r < step ? a.rows - r : step);
+        launch_distill<T>(ctx, a, q, a.row_count);
     }
 }
 
