@@ -10,11 +10,13 @@ is touched only in the last case (runtime.Session).
 """
 import ctypes
 import functools
+import math
 
 import numpy as np
 
 from . import _lib
-from .runtime import AnchorGrid, Session, _is_tf_tensor, _is_torch_tensor, _ptr, _torch
+from .runtime import (AnchorGrid, Session, _is_tf_tensor, _is_torch_tensor, _ptr, _torch, _torch_device,
+                      _torch_if_loaded)
 
 
 def _on_context_stream(fn):
@@ -250,54 +252,70 @@ def ssd_loss_batch(y_true, y_pred, neg_pos_ratio=3, n_neg_min=0, alpha=1.0, retu
 
 
 # ------------------------------------------------------------------ losses of large classifiers
-def _device_of(*arrays):
-    """The GPU of the first CUDA tensor among the arguments, or None: such a call runs where its data is."""
-    for x in arrays:
-        if _is_torch_tensor(x) and x.is_cuda:
-            return int(x.device.index)
-    return None
-
-
 def _session(context, *arrays):
-    """A session on the device the arrays are on; torch tensors on two GPUs are refused."""
-    device = _device_of(*arrays)
+    """A session on the GPU of the first CUDA tensor among the arrays: such a call runs where its data is.  Torch tensors on
+    two GPUs are refused."""
+    torch, device, use_torch = _torch_if_loaded(), None, False
+    if torch is not None:
+        for x in arrays:
+            if isinstance(x, torch.Tensor):
+                use_torch = True
+                if x.is_cuda:
+                    at = x.get_device()
+                    if device is None:
+                        device = at
+                    elif at != device:
+                        raise ValueError("arrays on GPU %d and GPU %d" % (device, at))
     if context is not None and device is not None and device != context.device:
         raise ValueError("the context runs on GPU %d, the arrays are on GPU %d" % (context.device, device))
-    for x in arrays:
-        if _is_torch_tensor(x) and x.is_cuda and int(x.device.index) != device:
-            raise ValueError("arrays on GPU %d and GPU %d" % (device, int(x.device.index)))
-    return Session(*arrays, context=context, device=device)
+    return Session(context=context, device=device, use_torch=use_torch)
+
+
+def _at(t):
+    """Address of a device array, or None."""
+    return t.data_ptr() if t is not None else None
+
+
+@functools.lru_cache(maxsize=256)
+def _head_bytes(*sizes):
+    need = ctypes.c_size_t()
+    _lib.check(_lib.load().ssdbox_linear_cross_entropy_workspace(*sizes, ctypes.byref(need)))
+    return need.value
+
+
+@functools.lru_cache(maxsize=256)
+def _distill_bytes(*sizes):
+    need = ctypes.c_size_t()
+    _lib.check(_lib.load().ssdbox_distill_topk_workspace(*sizes, ctypes.byref(need)))
+    return need.value
 
 
 def _float_rows(sess, x, name, max_ld=None):
     """A float32 / float16 / bfloat16 array as rows of its last axis: (array, family, rows, row stride,
     SSDBOX_DTYPE code, type).  Rows of a CUDA tensor may lie further apart than they are long."""
     if _is_torch_tensor(x):
-        torch = _torch()
-        code = {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16,
-                torch.bfloat16: _lib.DTYPE_BF16}.get(x.dtype)
+        torch, t = _torch(), x
+        code = (_lib.DTYPE_F32 if t.dtype is torch.float32 else _lib.DTYPE_BF16 if t.dtype is torch.bfloat16
+                else _lib.DTYPE_F16 if t.dtype is torch.float16 else None)
         if code is None:
             raise ValueError("%s must be float32, float16 or bfloat16, got %s" % (name, x.dtype))
-        if x.dim() < 2:
+        if t.dim() < 2:
             raise ValueError("%s must have at least 2 dimensions, got shape %s" % (name, tuple(x.shape)))
-        t = x.detach()
-        if not t.is_cuda or t.device.index != sess.device:
-            t = t.to("cuda:%d" % sess.device)
-        width = int(t.shape[-1])
-        rows = 1
-        for s in t.shape[:-1]:
-            rows *= int(s)
-        if rows and width:
-            try:
-                t = t.view(rows, width)
-            except RuntimeError:
-                t = t.reshape(rows, width)
-            if (t.stride(1) != 1 and width > 1) or (rows > 1 and not width <= t.stride(0) <= (max_ld or 1 << 62)):
-                t = t.contiguous()
-            ld = int(t.stride(0)) if rows > 1 else width
-        else:
-            t, ld = t.reshape(rows, width), width
-        return t, "torch", rows, ld, code, t.dtype
+        if t.requires_grad:
+            t = t.detach()
+        if not t.is_cuda or t.get_device() != sess.device:
+            t = t.to(_torch_device(sess.device))
+        width = t.shape[-1]
+        rows = t.numel() // width if width else math.prod(t.shape[:-1])
+        if t.is_contiguous():
+            return t, "torch", rows, width, code, t.dtype
+        try:
+            t = t.view(rows, width)
+        except RuntimeError:
+            t = t.reshape(rows, width)
+        if (t.stride(1) != 1 and width > 1) or (rows > 1 and not width <= t.stride(0) <= (max_ld or 1 << 62)):
+            t = t.contiguous()
+        return t, "torch", rows, t.stride(0) if rows > 1 else width, code, t.dtype
     dtype = np.dtype(getattr(x, "dtype", np.float32)) if not _is_tf_tensor(x) else np.dtype(x.dtype.as_numpy_dtype)
     if dtype not in (np.dtype(np.float32), np.dtype(np.float16)):
         raise ValueError("%s must be float32 or float16 (or a torch bfloat16 tensor), got %s" % (name, dtype))
@@ -314,16 +332,15 @@ def _float_rows(sess, x, name, max_ld=None):
 def _integers(sess, x, name, shape):
     """An int32 or int64 array of the given shape, dense on the device: (array, bytes a value)."""
     if _is_torch_tensor(x):
-        torch = _torch()
-        t = x.detach()
-        if t.dtype not in (torch.int32, torch.int64):
+        torch, t = _torch(), x
+        if t.dtype is not torch.int64 and t.dtype is not torch.int32:
             if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
                 raise ValueError("%s must be integers, got %s" % (name, t.dtype))
             t = t.to(torch.int64)
-        if not t.is_cuda or t.device.index != sess.device:
-            t = t.to("cuda:%d" % sess.device)
+        if not t.is_cuda or t.get_device() != sess.device:
+            t = t.to(_torch_device(sess.device))
         t = t.contiguous()
-        if tuple(t.shape) != tuple(shape):
+        if t.shape != shape:
             raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
         return t, t.element_size()
     a = x.numpy() if _is_tf_tensor(x) else np.asarray(x)
@@ -342,8 +359,8 @@ def _row_floats(sess, x, name, shape):
     """A float32 array of the given shape on the device, or None."""
     if x is None:
         return None
-    t, _ = sess.put(x.detach() if _is_torch_tensor(x) else x, np.float32)
-    if tuple(t.shape) != tuple(shape):
+    t, _ = sess.put(x.detach() if _is_torch_tensor(x) and x.requires_grad else x, np.float32)
+    if tuple(t.shape) != shape:
         raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
     return t
 
@@ -370,7 +387,7 @@ def linear_cross_entropy_batch(hidden, weight, labels, logit_scale=1.0, label_sm
     """
     sess = _session(context, hidden, weight, labels, grad_loss)
     ctx = sess.ctx
-    lead = tuple(int(s) for s in hidden.shape[:-1])
+    lead = tuple(hidden.shape[:-1])
     h, family, rows, ld_h, code, dtype = _float_rows(sess, hidden, "hidden")
     w, _, classes, ld_w, code_w, _ = _float_rows(sess, weight, "weight", 1 << 21)
     if code != code_w:
@@ -384,17 +401,15 @@ def linear_cross_entropy_batch(hidden, weight, labels, logit_scale=1.0, label_sm
         w, ld_w = _aligned(w, ld_w, dim)
     lab, label_bytes = _integers(sess, labels, "labels", lead)
     g = _row_floats(sess, grad_loss, "grad_loss", lead) if return_grad else None
-    lib, need = ctx.lib, ctypes.c_size_t()
-    _lib.check(lib.ssdbox_linear_cross_entropy_workspace(
-        rows, classes, dim, ld_w, code, float(label_smoothing), int(bool(return_grad)),
-        int(bool(return_grad and weight_grad)), ctypes.byref(need)))
+    need = _head_bytes(rows, classes, dim, ld_w, code, float(label_smoothing), int(bool(return_grad)),
+                       int(bool(return_grad and weight_grad)))
     loss = sess.empty(lead)
     gh = sess.empty(lead + (dim,), dtype) if return_grad else None
     gw = sess.empty((classes, dim), dtype) if return_grad and weight_grad else None
-    work = sess.empty((need.value,), np.uint8)
-    _lib.check(lib.ssdbox_linear_cross_entropy(
-        ctx.handle, _ptr(h), ld_h, _ptr(w), ld_w, _ptr(lab), label_bytes, rows, classes, dim, code,
-        float(logit_scale), float(label_smoothing), _ptr(g), _ptr(loss), _ptr(gh), _ptr(gw), _ptr(work), need.value))
+    work = sess.empty((need,), np.uint8)
+    _lib.check(ctx.lib.ssdbox_linear_cross_entropy(
+        ctx.handle, _at(h), ld_h, _at(w), ld_w, _at(lab), label_bytes, rows, classes, dim, code,
+        float(logit_scale), float(label_smoothing), _at(g), _at(loss), _at(gh), _at(gw), _at(work), need))
     res = (sess.get(loss, family),)
     if return_grad:
         res += (sess.get(gh, family),)
@@ -423,7 +438,7 @@ def distill_topk_batch(logits, teacher_values, teacher_index, temperature=1.0, t
     sess = _session(context, logits, teacher_values, teacher_index, teacher_lse, grad_loss)
     ctx = sess.ctx
     z, family, rows, ld, code, dtype = _float_rows(sess, logits, "logits")
-    lead, classes = tuple(int(s) for s in logits.shape[:-1]), int(z.shape[-1])
+    lead, classes = tuple(logits.shape[:-1]), int(z.shape[-1])
     if classes == 0:
         raise ValueError("logits have no classes: shape %s" % (tuple(logits.shape),))
     if len(teacher_values.shape) != len(lead) + 1:
@@ -433,12 +448,11 @@ def distill_topk_batch(logits, teacher_values, teacher_index, temperature=1.0, t
     index, index_bytes = _integers(sess, teacher_index, "teacher_index", lead + (top,))
     lse = _row_floats(sess, teacher_lse, "teacher_lse", lead)
     g = _row_floats(sess, grad_loss, "grad_loss", lead) if return_grad else None
-    lib, need = ctx.lib, ctypes.c_size_t()
-    _lib.check(lib.ssdbox_distill_topk_workspace(rows, classes, code, ctypes.byref(need)))
+    need = _distill_bytes(rows, classes, code)
     loss = sess.empty(lead)
     grad = sess.empty(lead + (classes,), dtype) if return_grad else None
-    work = sess.empty((need.value,), np.uint8) if need.value else None
-    _lib.check(lib.ssdbox_distill_topk(
-        ctx.handle, _ptr(z), ld, rows, classes, code, _ptr(values), _ptr(index), index_bytes, top, _ptr(lse),
-        float(temperature), _ptr(g), _ptr(loss), _ptr(grad), _ptr(work), need.value))
+    work = sess.empty((need,), np.uint8) if need else None
+    _lib.check(ctx.lib.ssdbox_distill_topk(
+        ctx.handle, _at(z), ld, rows, classes, code, _at(values), _at(index), index_bytes, top, _at(lse),
+        float(temperature), _at(g), _at(loss), _at(grad), _at(work), need))
     return (sess.get(loss, family), sess.get(grad, family)) if return_grad else sess.get(loss, family)

@@ -26,8 +26,11 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.69314718055994530942;
-constexpr int kScanThreads = 1024;
 constexpr int kRowThreads = 256;
+constexpr int kRowsEach = 16;         // rows a workgroup places and copies
+constexpr int kCountRows = 1024;      // rows a workgroup counts, where there are many
+constexpr int kCountFrom = 16384;     // rows from which counting has a launch of its own: below, reading all labels before
+                                      // a workgroup's rows again costs less than the launch
 
 struct HeadScale {                    // what the gradient's rows are multiplied by before d, and the results after
     float down, up;
@@ -38,18 +41,24 @@ struct HeadRow {                      // a counted row: p_v = 2^(a L - m) * c / 
 };
 
 // ------------------------------------------------------------------------------ rows
-struct ScanArgs {
+struct PrepArgs {
     const void *labels;
     int label_bytes, rows;
     long long classes;
     const float *grad_loss;
     float logit_scale;
     int scaled;                       // 16-bit gradients: bring the largest c to just under 2^15
-    int *place;                       // per row: its place among the counted rows, or -1
+    const void *hidden;
+    long long ld;
+    int dim, pitch;
+    int wide;                         // hidden rows start at 16-byte boundaries
+    int *block_count;                 // counted rows and largest |grad_loss| of every kCountRows rows, or NULL
+    float *block_max;
+    int *place_count;                 // the number of counted rows
     int *row, *label;                 // per counted row: the row it was, its class
-    int *count;
     HeadScale *scale;
     float *loss;
+    void *out, *grad_hidden;
 };
 
 SSD_DEV long long label_at(const void *p, int bytes, int n)
@@ -57,75 +66,124 @@ SSD_DEV long long label_at(const void *p, int bytes, int n)
     return bytes == 8 ? ((const long long *)p)[n] : (long long)((const int *)p)[n];
 }
 
-// One workgroup: the order of the counted rows has to be that of the batch, so that sums over rows are the same every time.
-__global__ __launch_bounds__(kScanThreads) void head_scan_kernel(const ScanArgs p)
+SSD_DEV bool counted_at(const PrepArgs &p, int n)
 {
-    __shared__ int s_wave[kScanThreads / 64];
-    __shared__ float s_max[kScanThreads / 64];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const long long lab = label_at(p.labels, p.label_bytes, n);
+    return lab >= 0 && lab < p.classes;
+}
+
+// Sum and maximum over the workgroup's four waves, in all lanes.
+SSD_DEV int block_total(int lane_count, int *lds)
+{
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) lane_count += __shfl_xor(lane_count, o);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = lane_count;
+    __syncthreads();
+    return lds[0] + lds[1] + lds[2] + lds[3];
+}
+SSD_DEV float block_max(float x, float *lds)
+{
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
+    __syncthreads();
+    return fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
+}
+
+__global__ __launch_bounds__(kRowThreads) void head_count_kernel(const PrepArgs p)
+{
+    __shared__ int s_count[4];
+    __shared__ float s_max[4];
+    int c = 0;
+    float g = 0.0f;
+    const int end = min(p.rows, ((int)blockIdx.x + 1) * kCountRows);
+    for (int n = blockIdx.x * kCountRows + threadIdx.x; n < end; n += kRowThreads)
+        if (counted_at(p, n)) {
+            ++c;
+            if (p.grad_loss) g = fmaxf(g, fabsf(p.grad_loss[n]));
+        }
+    c = block_total(c, s_count);
+    g = block_max(g, s_max);
+    if (threadIdx.x == 0) {
+        p.block_count[blockIdx.x] = c;
+        p.block_max[blockIdx.x] = g;
+    }
+}
+
+// Each workgroup takes kRowsEach rows: counts the rows before them (the order of the counted rows is that of the batch, so that
+// sums over rows are the same every time), copies the counted ones to their places, with zeros behind their last value, and
+// settles the others.
+template <typename T>
+__global__ __launch_bounds__(kRowThreads) void head_prep_kernel(const PrepArgs p)
+{
+    __shared__ int s_count[4];
+    __shared__ float s_max[4];
+    __shared__ int s_place[kRowsEach];
+    const int t = threadIdx.x, first = blockIdx.x * kRowsEach;
+    const int blocks = p.block_count ? first / kCountRows : 0;
     int before = 0;
-    float gmax = 0.0f;
-    for (int base = 0; base < p.rows; base += kScanThreads) {
-        const int n = base + t;
-        const long long lab = n < p.rows ? label_at(p.labels, p.label_bytes, n) : -1;
+    for (int i = t; i < blocks; i += kRowThreads) before += p.block_count[i];
+    for (int n = blocks * kCountRows + t; n < first; n += kRowThreads) before += counted_at(p, n) ? 1 : 0;
+    before = block_total(before, s_count);
+    if (t < 64) {
+        const int n = first + t;
+        const bool mine = t < kRowsEach && n < p.rows;
+        const long long lab = mine ? label_at(p.labels, p.label_bytes, n) : -1;
         const bool counted = lab >= 0 && lab < p.classes;
         const unsigned long long bal = __ballot(counted);
-        if (lane == 0) s_wave[wave] = __popcll(bal);
-        __syncthreads();
-        int at = before + __popcll(bal & ((1ull << lane) - 1ull)), all = 0;
-#pragma unroll
-        for (int w = 0; w < kScanThreads / 64; ++w) {
-            const int c = s_wave[w];
-            if (w < wave) at += c;
-            all += c;
+        const int at = before + __popcll(bal & ((1ull << t) - 1ull));
+        if (counted) {
+            p.row[at] = n;
+            p.label[at] = (int)lab;
+        } else if (mine) {
+            p.loss[n] = lab < 0 ? 0.0f : u2f(0x7FC00000u);
         }
-        before += all;
-        if (n < p.rows) {
-            p.place[n] = counted ? at : -1;
-            if (counted) {
-                p.row[at] = n;
-                p.label[at] = (int)lab;
-                if (p.grad_loss) gmax = fmaxf(gmax, fabsf(p.grad_loss[n]));
-            } else {
-                p.loss[n] = lab < 0 ? 0.0f : u2f(0x7FC00000u);
-            }
-        }
-        __syncthreads();
+        if (t < kRowsEach) s_place[t] = counted ? at : -1;
+        if (t == 0 && first + kRowsEach >= p.rows) *p.place_count = before + __popcll(bal);
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) gmax = fmaxf(gmax, __shfl_xor(gmax, o));
-    if (lane == 0) s_max[wave] = gmax;
     __syncthreads();
-    if (t != 0) return;
-    *p.count = before;
+    const T *hidden = (const T *)p.hidden;
+    constexpr int kVec = 16 / (int)sizeof(T);
+    for (int i = t >> 6; i < kRowsEach && first + i < p.rows; i += kRowThreads / 64) {
+        const long long n = first + i, at = s_place[i];
+        const int lane = t & 63;
+        if (at >= 0) {
+            T *o = (T *)p.out + at * p.pitch;
+            if (p.wide) {
+                for (int d = lane * kVec; d < p.pitch; d += 64 * kVec)
+                    *(u32x4 *)(o + d) = *(const u32x4 *)(hidden + n * p.ld + d);
+            } else {
+                for (int d = lane; d < p.pitch; d += 64) o[d] = d < p.dim ? hidden[n * p.ld + d] : (T)0.0f;
+            }
+        } else if (p.grad_hidden) {
+            T *o = (T *)p.grad_hidden + n * p.dim;
+            for (int d = lane; d < p.dim; d += 64) o[d] = (T)0.0f;
+        }
+    }
+    if (blockIdx.x != 0) return;
     HeadScale s = {1.0f, 1.0f};
     if (p.scaled) {
-        for (int w = 0; w < kScanThreads / 64; ++w) gmax = fmaxf(gmax, s_max[w]);
-        if (!p.grad_loss) gmax = 1.0f / (float)p.rows;
+        float g = 0.0f;
+        if (!p.grad_loss) {
+            g = 1.0f / (float)p.rows;
+        } else if (p.block_count) {
+            for (int i = t; i < (p.rows + kCountRows - 1) / kCountRows; i += kRowThreads) g = fmaxf(g, p.block_max[i]);
+        } else {
+            for (int n = t; n < p.rows; n += kRowThreads)
+                if (counted_at(p, n)) g = fmaxf(g, fabsf(p.grad_loss[n]));
+        }
+        g = block_max(g, s_max);
         // Of float16 this uses the range; and an unsure row's d at its label, -c (1 - p), which weighs most in the
         // gradients, lies just under a power of two, where the rounding to 8 or 11 bits is finest.
-        const float c = gmax * p.logit_scale;
+        const float c = g * p.logit_scale;
         if (c > 1e-30f && c < 1e30f) {
             s.down = 32768.0f * (1.0f - 1.0f / 128.0f) / c;
             s.up = 1.0f / s.down;
         }
     }
-    *p.scale = s;
-}
-
-// One workgroup a row: a counted row to its place (zeros behind its last value), another one's gradient to zero.
-template <typename T>
-__global__ __launch_bounds__(kRowThreads) void head_gather_kernel(const T *hidden, long long ld, const int *place, int dim,
-                                                                  int pitch, T *rows, T *grad_hidden)
-{
-    const long long n = blockIdx.x;
-    const int at = place[n];
-    if (at >= 0) {
-        for (int d = threadIdx.x; d < pitch; d += kRowThreads)
-            rows[(long long)at * pitch + d] = d < dim ? hidden[n * ld + d] : (T)0.0f;
-    } else if (grad_hidden) {
-        for (int d = threadIdx.x; d < dim; d += kRowThreads) grad_hidden[n * dim + d] = (T)0.0f;
-    }
+    if (t == 0) *p.scale = s;
 }
 
 // Rows of a weight whose rows do not start at 16-byte boundaries, laid out so that they do.
@@ -142,99 +200,158 @@ struct LogitArgs {
     long long ldw, ldh;
     int dim, classes, tiles;          // classes and tiles of classes in this piece
     int first;                        // the piece's first class
-    int row_tiles;
     float l2;                         // logit_scale * log2(e)
     const int *count, *label;
     float2 *stat;                     // [row][slots]: (max, sum of exponentials) of one wave's part of a tile
     float *sum_z;                     // [row][slots], or NULL without smoothing
     long long slots;
-    int slot0;
     float *z_label;                   // [row]: the label's product, before the scale
     const HeadRow *row;
     void *delta;                      // [row][ld_delta]
     long long ld_delta;
 };
 
-// GRAD false: statistics of a tile of logits; true: d of it.
-template <typename T, int BM, int BN, int WM, int WN, bool GRAD>
-__global__ __launch_bounds__(WM * WN * 64) void head_logit_kernel(const LogitArgs p)
+// Sixteen neighbouring values of one row of the result, half of them in the lane 32 further: lo at m + 4 h .. + 3 and hi
+// at m + 8 + 4 h .. + 3 (h = lane / 32).  16-bit types trade halves, so that each lane stores 16 bytes.
+// Called by both lanes alike; left: values there are from m on.
+template <typename T>
+SSD_DEV void store_pair(T *row, int m, const float (&lo)[4], const float (&hi)[4], int left, bool wide, bool in)
 {
-    typedef TileProduct<T, BM, BN, WM, WN, false, false> P;
-    __shared__ __align__(1024) char smem[P::kLds];
+    const int h = (int)(threadIdx.x >> 5 & 1);
+    if constexpr (sizeof(T) == 4) {
+        if (!in) return;
+        if (wide && left >= 16) {
+            *(f32x4 *)(row + m + 4 * h) = f32x4{lo[0], lo[1], lo[2], lo[3]};
+            *(f32x4 *)(row + m + 8 + 4 * h) = f32x4{hi[0], hi[1], hi[2], hi[3]};
+            return;
+        }
+    } else if (wide && left >= 16) {
+        union { T v[8]; unsigned w[4]; } x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x.v[i] = (T)lo[i];
+            x.v[4 + i] = (T)hi[i];
+        }
+        const auto a = __builtin_amdgcn_permlane32_swap(x.w[0], x.w[2], false, false);
+        const auto b = __builtin_amdgcn_permlane32_swap(x.w[1], x.w[3], false, false);
+        if (in) *(u32x4 *)(row + m + 8 * h) = u32x4{a[0], b[0], a[1], b[1]};
+        return;
+    }
+    if (!in) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (4 * h + i < left) row[m + 4 * h + i] = (T)lo[i];
+        if (8 + 4 * h + i < left) row[m + 8 + 4 * h + i] = (T)hi[i];
+    }
+}
+
+// GRAD false: statistics of a tile of logits; true: d of it.
+template <typename T, int BM, int BN, int WM, int WN, int BLOCKS, bool GRAD>
+__global__ __launch_bounds__(WM * WN * 64, BLOCKS * WM * WN / 4) void head_logit_kernel(const LogitArgs p)
+{
+    typedef TileStream<T, BM, BN, WM, WN, false, false> S;
+    __shared__ __align__(1024) char smem[S::kLds];
     const int count = uniform(*p.count);
     const int tn = (count + BN - 1) / BN;
-    if ((int)blockIdx.x >= p.tiles * tn) return;
-    int tm_i, tn_i;
-    tile_of(blockIdx.x, p.tiles, tn, 8, tm_i, tn_i);
-    const int m0 = tm_i * BM, n0 = tn_i * BN;
-    typename P::OpA a;
-    typename P::OpB b;
-    a.init(p.weight, p.ldw, m0, p.classes - m0, 0, smem);
-    b.init(p.rows, p.ldh, n0, count - n0, 0, smem + BM * kRowBytes);
-    f32x4 acc[P::MF][P::NF];
-    P::run(a, b, p.dim, smem, acc);
-
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
-    const int wm = wave / WN, wn = wave % WN;
-    const int v0 = m0 + wm * (BM / WM) + 4 * g;                  // within the piece
+    const auto unit = [&](int i, TileUnit &u) {
+        int m, n;
+        tile_of(i, p.tiles, tn, 8, m, n);
+        u = TileUnit{m * BM, n * BN, 0, p.dim, 0};
+    };
+    const auto set = [&](typename S::OpA &a, typename S::OpB &b, const TileUnit &u) {
+        a.init(p.weight, p.ldw, u.m0, p.classes - u.m0, 0);
+        b.init(p.rows, p.ldh, u.n0, count - u.n0, 0);
+    };
+    const auto use = [&](f32x16 (&acc)[S::MF][S::NF], const TileUnit &u, int em, int en) {
+        const int lane = threadIdx.x & 63, h = lane >> 5;
+        const int v0 = u.m0 + em + 4 * h;                        // within the piece
+        const bool edge = u.m0 + em + 32 * S::MF > p.classes;    // the wave's part has classes that do not exist
 #pragma unroll
-    for (int nj = 0; nj < P::NF; ++nj) {
-        const int n = n0 + wn * (BN / WN) + nj * 16 + (lane & 15);
-        const bool in = n < count;
-        const int lab = in ? p.label[n] - p.first : -1;
-        if constexpr (!GRAD) {
-            float mx = -INFINITY, sz = 0.0f;
+        for (int nj = 0; nj < S::NF; ++nj) {
+            const int n = u.n0 + en + nj * 32 + (lane & 31);
+            const bool in = n < count;
+            const int lab = in ? p.label[n] - p.first : -1;
+            const int rel = lab - (u.m0 + em);
+            // the tests of single values only where one of the wave's labels lies here, or the last class
+            const bool plain = !edge && !__any(rel >= 0 && rel < 32 * S::MF);
+            if constexpr (!GRAD) {
+                float mx = -INFINITY, sz = 0.0f, s = 0.0f;
+                if (plain) {
 #pragma unroll
-            for (int mi = 0; mi < P::MF; ++mi)
+                    for (int mi = 0; mi < S::MF; ++mi)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int v = v0 + mi * 16 + i;
-                    const float z = acc[mi][nj][i];
-                    if (v < p.classes) {
-                        sz += z;
-                        if (v != lab) mx = fmaxf(mx, z);
-                        else p.z_label[n] = z;
+                        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, acc[mi][nj][e]);
+                    if (p.sum_z)
+#pragma unroll
+                        for (int mi = 0; mi < S::MF; ++mi)
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) sz += acc[mi][nj][e];
+                } else {
+#pragma unroll
+                    for (int mi = 0; mi < S::MF; ++mi)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const int v = v0 + mi * 32 + (e >> 2) * 8 + (e & 3);
+                            const float z = acc[mi][nj][e];
+                            if (v < p.classes) {
+                                sz += z;
+                                if (v != lab) mx = fmaxf(mx, z);
+                                else p.z_label[n] = z;
+                            }
+                        }
+                }
+                mx = fmaxf(mx, __shfl_xor(mx, 32));
+                const float m = mx * p.l2;
+                const float ref = mx == -INFINITY ? 0.0f : m;
+                if (plain) {
+#pragma unroll
+                    for (int mi = 0; mi < S::MF; ++mi)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mi][nj][e], p.l2, -ref));
+                } else {
+#pragma unroll
+                    for (int mi = 0; mi < S::MF; ++mi)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const int v = v0 + mi * 32 + (e >> 2) * 8 + (e & 3);
+                            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mi][nj][e], p.l2, -ref));
+                            if (v < p.classes && v != lab) s += x;
+                        }
+                }
+                s += __shfl_xor(s, 32);
+                const long long slot = (long long)n * p.slots + (u.m0 + em) / (32 * S::MF);
+                if (in && h == 0) p.stat[slot] = make_float2(m, s);
+                if (p.sum_z) {
+                    sz += __shfl_xor(sz, 32);
+                    if (in && h == 0) p.sum_z[slot] = sz;
+                }
+            } else {
+                const HeadRow r = in ? p.row[n] : HeadRow{0.0f, 0.0f, 0.0f, 0.0f};
+                T *out = (T *)p.delta + (long long)n * p.ld_delta;
+#pragma unroll
+                for (int mi = 0; mi < S::MF; ++mi)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 8) {
+                        float d[2][4];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            d[i >> 2][i & 3] = __builtin_fmaf(
+                                __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mi][nj][e + i], p.l2, -r.m)), r.pz, -r.smooth);
+                        const int m = u.m0 + em + mi * 32 + e * 2;
+                        if (!plain)
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const int v = m + 4 * h + (i >> 2) * 8 + (i & 3);
+                                if (v == lab) d[i >> 2][i & 3] = r.label;
+                                if (v >= p.classes) d[i >> 2][i & 3] = 0.0f;
+                            }
+                        store_pair<T>(out, m, d[0], d[1], 16, true, in);
                     }
-                }
-            mx = fmaxf(mx, __shfl_xor(mx, 16));
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            const float m = mx * p.l2;
-            const float ref = mx == -INFINITY ? 0.0f : m;
-            float s = 0.0f;
-#pragma unroll
-            for (int mi = 0; mi < P::MF; ++mi)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int v = v0 + mi * 16 + i;
-                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mi][nj][i], p.l2, -ref));
-                    if (v < p.classes && v != lab) s += e;
-                }
-            s += __shfl_xor(s, 16);
-            s += __shfl_xor(s, 32);
-            if (in && g == 0) p.stat[(long long)n * p.slots + p.slot0 + tm_i * WM + wm] = make_float2(m, s);
-            if (p.sum_z) {
-                sz += __shfl_xor(sz, 16);
-                sz += __shfl_xor(sz, 32);
-                if (in && g == 0) p.sum_z[(long long)n * p.slots + p.slot0 + tm_i * WM + wm] = sz;
-            }
-        } else {
-            const HeadRow r = in ? p.row[n] : HeadRow{0.0f, 0.0f, 0.0f, 0.0f};
-            T *out = (T *)p.delta + (long long)n * p.ld_delta + v0;
-#pragma unroll
-            for (int mi = 0; mi < P::MF; ++mi) {
-                struct __align__(4 * sizeof(T)) Four { T v[4]; } o;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int v = v0 + mi * 16 + i;
-                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mi][nj][i], p.l2, -r.m));
-                    float d = __builtin_fmaf(e, r.pz, -r.smooth);
-                    d = v == lab ? r.label : d;
-                    o.v[i] = (T)(v < p.classes ? d : 0.0f);
-                }
-                if (in) *(Four *)(out + mi * 16) = o;
             }
         }
-    }
+    };
+    S::run(p.tiles * tn, smem, unit, set, use);
 }
 
 // ------------------------------------------------------------------------ row statistics
@@ -337,7 +454,7 @@ struct GradArgs {
     int m, a_extent, n, k;            // a_extent: columns of A that may be read
     const int *n_count, *k_count;     // device-side n or k, or NULL
     int tm;
-    int steps;                        // K tiles per part
+    int parts;                        // k is cut into
     const HeadScale *scale;
     void *out;                        // [n][ldo], through row_of when given
     long long ldo;
@@ -347,66 +464,63 @@ struct GradArgs {
     int add;                          // to what part holds
 };
 
-template <typename T>
-SSD_DEV void store4(T *p, f32x4 v, float up, int left, bool wide)
+template <typename T, int BM, int BN, int WM, int WN, int BLOCKS, bool B_KROWS>
+__global__ __launch_bounds__(WM * WN * 64, BLOCKS * WM * WN / 4) void head_grad_kernel(const GradArgs p)
 {
-    struct __align__(4 * sizeof(T)) Four { T v[4]; } o;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o.v[i] = (T)(v[i] * up);
-    if (wide) {
-        if (left > 0) *(Four *)p = o;
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (i < left) p[i] = o.v[i];
-}
-
-template <typename T, int BM, int BN, int WM, int WN, bool B_KROWS>
-__global__ __launch_bounds__(WM * WN * 64) void head_grad_kernel(const GradArgs p)
-{
-    typedef TileProduct<T, BM, BN, WM, WN, true, B_KROWS> P;
-    __shared__ __align__(1024) char smem[P::kLds];
+    typedef TileStream<T, BM, BN, WM, WN, true, B_KROWS> S;
+    __shared__ __align__(1024) char smem[S::kLds];
     const int nn = uniform(p.n_count ? *p.n_count : p.n);
     const int kk = uniform(p.k_count ? *p.k_count : p.k);
     const int tn = (nn + BN - 1) / BN;
-    if ((int)blockIdx.x >= p.tm * tn) return;
-    int tm_i, tn_i;
-    tile_of(blockIdx.x, p.tm, tn, 8, tm_i, tn_i);
-    const int m0 = tm_i * BM, n0 = tn_i * BN;
-    const int k0 = blockIdx.y * p.steps * P::kBK;
-    const int kn = kk - k0 < p.steps * P::kBK ? kk - k0 : p.steps * P::kBK;
-    typename P::OpA a;
-    typename P::OpB b;
-    a.init(p.a, p.lda, m0, p.a_extent - m0, k0, smem);
-    b.init(p.b, p.ldb, n0, nn - n0, k0, smem + BM * kRowBytes);
-    f32x4 acc[P::MF][P::NF];
-    P::run(a, b, kn, smem, acc);
-
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
-    const int em = m0 + (wave / WN) * (BM / WM) + 4 * g;
-    const int en = n0 + (wave % WN) * (BN / WN) + (lane & 15);
+    const int each = ((kk + S::kBK - 1) / S::kBK + p.parts - 1) / p.parts * S::kBK;   // values of k a part, whole stages
+    const auto unit = [&](int i, TileUnit &u) {
+        const int part = i / (p.tm * tn);
+        int m, n;
+        tile_of(i - part * p.tm * tn, p.tm, tn, 8, m, n);
+        const int k0 = part * each, left = kk - k0;
+        u = TileUnit{m * BM, n * BN, k0, left < each ? left : each, part};
+    };
+    const auto set = [&](typename S::OpA &a, typename S::OpB &b, const TileUnit &u) {
+        a.init(p.a, p.lda, u.m0, p.a_extent - u.m0, u.k0);
+        b.init(p.b, p.ldb, u.n0, nn - u.n0, u.k0);
+    };
     const float up = p.scale->up;
-    const bool wide = p.m % 4 == 0 && p.ldo % 4 == 0;
+    const bool wide = p.m % (16 / (int)sizeof(T)) == 0 && p.ldo % (16 / (int)sizeof(T)) == 0;
+    const auto use = [&](f32x16 (&acc)[S::MF][S::NF], const TileUnit &u, int em, int en) {
+        const int lane = threadIdx.x & 63, h = lane >> 5;
 #pragma unroll
-    for (int nj = 0; nj < P::NF; ++nj) {
-        const int n = en + nj * 16;
-        if (n >= nn) continue;
-        if (p.part) {
-            float *o = p.part + (long long)blockIdx.y * p.part_stride + (long long)n * p.ld_part + em;
+        for (int nj = 0; nj < S::NF; ++nj) {
+            const int n = u.n0 + en + nj * 32 + (lane & 31);
+            const bool in = n < nn;
+            if (p.part) {
+                float *o = p.part + u.part * p.part_stride + (long long)n * p.ld_part;
 #pragma unroll
-            for (int mi = 0; mi < P::MF; ++mi)
-                if (em + mi * 16 < p.m) {       // ld_part is a multiple of 4: the last group may pass m, not the row
-                    f32x4 v = acc[mi][nj];
-                    if (p.add) v += *(const f32x4 *)(o + mi * 16);
-                    *(f32x4 *)(o + mi * 16) = v;
-                }
-        } else {
-            T *o = (T *)p.out + (p.row_of ? p.row_of[n] : n) * p.ldo + em;
+                for (int mi = 0; mi < S::MF; ++mi)
 #pragma unroll
-            for (int mi = 0; mi < P::MF; ++mi) store4<T>(o + mi * 16, acc[mi][nj], up, p.m - em - mi * 16, wide);
+                    for (int e = 0; e < 16; e += 4) {
+                        const int m = u.m0 + em + mi * 32 + e * 2 + 4 * h;
+                        if (in && m < p.m) {      // ld_part is a multiple of 4: the last group may pass m, not the row
+                            f32x4 v = {acc[mi][nj][e], acc[mi][nj][e + 1], acc[mi][nj][e + 2], acc[mi][nj][e + 3]};
+                            if (p.add) v += *(const f32x4 *)(o + m);
+                            *(f32x4 *)(o + m) = v;
+                        }
+                    }
+            } else {
+                T *o = (T *)p.out + (in ? (p.row_of ? (long long)p.row_of[n] : (long long)n) : 0) * p.ldo;
+#pragma unroll
+                for (int mi = 0; mi < S::MF; ++mi)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 8) {
+                        const int m = u.m0 + em + mi * 32 + e * 2;
+                        float d[2][4];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) d[i >> 2][i & 3] = acc[mi][nj][e + i] * up;
+                        store_pair<T>(o, m, d[0], d[1], p.m - m, wide, in);
+                    }
+            }
         }
-    }
+    };
+    S::run(p.parts * p.tm * tn, smem, unit, set, use);
 }
 
 struct JoinArgs {
@@ -440,14 +554,14 @@ __global__ __launch_bounds__(kRowThreads) void head_join_kernel(const JoinArgs p
 // Everything that follows from sizes: which tile, how many parts, and the workspace.
 struct HeadPlan {
     int es, vec, tile;                // bytes and 16-byte values of a type, tile configuration
-    int bm, bn, wm;
+    int bm, bn, each;                 // each: classes of one wave's part of a tile of logits
     int pitch;                        // dim rounded up to 16 bytes
     bool copy_weight;
     long long class_tiles, slots;
     long long piece;                  // classes a piece
     int pieces;
-    int dh_parts, dh_steps, dw_parts, dw_steps;
-    size_t o_rows, o_weight, o_place, o_row, o_label, o_count, o_scale, o_stat, o_sumz, o_zl, o_out, o_delta, o_dh, o_dw;
+    int dh_parts, dw_parts;
+    size_t o_blocks, o_rows, o_weight, o_row, o_label, o_count, o_scale, o_stat, o_sumz, o_zl, o_out, o_delta, o_dh, o_dw;
     size_t bytes;
 };
 
@@ -460,17 +574,13 @@ size_t put(size_t &at, size_t bytes)
     return o;
 }
 
-// Parts of k so that the tiles fill the chip, at least four K tiles each.
-void split(long long tiles, long long k_tiles, int &parts, int &steps)
+// Parts of k so that the tiles fill the chip, at least eight stages each.
+int split(long long tiles, long long k_stages)
 {
     long long s = tiles > 0 ? 512 / tiles : 1;
-    if (s > k_tiles / 4) s = k_tiles / 4;
+    if (s > k_stages / 8) s = k_stages / 8;
     if (s > 64) s = 64;
-    if (s < 1) s = 1;
-    steps = (int)((k_tiles + s - 1) / s);
-    if (steps < 1) steps = 1;
-    parts = (int)((k_tiles + steps - 1) / steps);
-    if (parts < 1) parts = 1;
+    return s < 1 ? 1 : (int)s;
 }
 
 HeadPlan make_plan(long long rows, long long classes, long long dim, long long weight_ld, int dtype, float smoothing,
@@ -482,12 +592,12 @@ HeadPlan make_plan(long long rows, long long classes, long long dim, long long w
     q.pitch = (int)((dim + q.vec - 1) / q.vec * q.vec);
     q.copy_weight = dim % q.vec != 0 || weight_ld % q.vec != 0;
     // float32 keeps two sums a value (ssdbox_tile.h): the large tile's would not fit the registers
-    q.tile = rows <= 32 ? 0 : (rows <= 512 || dtype == SSDBOX_DTYPE_F32 ? 1 : 2);
+    q.tile = rows <= 64 ? 0 : (rows <= 512 || dtype == SSDBOX_DTYPE_F32 ? 1 : 2);
     q.bm = q.tile == 2 ? 256 : 128;
-    q.bn = q.tile == 2 ? 256 : (q.tile == 1 ? 128 : 32);
-    q.wm = q.tile == 0 ? 4 : 2;
+    q.bn = q.tile == 2 ? 256 : (q.tile == 1 ? 128 : 64);
+    q.each = q.tile == 2 ? 128 : (q.tile == 1 ? 64 : 32);
     q.class_tiles = (classes + q.bm - 1) / q.bm;
-    q.slots = q.class_tiles * q.wm;
+    q.slots = q.class_tiles * (q.bm / q.each);
     const bool grad = grad_hidden || grad_weight;
     if (grad) {
         const long long row_bytes = rows * q.es > 0 ? rows * q.es : 1;
@@ -502,7 +612,7 @@ HeadPlan make_plan(long long rows, long long classes, long long dim, long long w
     size_t at = 0;
     q.o_count = put(at, 256);
     q.o_scale = put(at, 256);
-    q.o_place = put(at, rows * 4);
+    q.o_blocks = put(at, rows > kCountFrom ? (rows + kCountRows - 1) / kCountRows * 8 : 0);
     q.o_row = put(at, rows * 4);
     q.o_label = put(at, rows * 4);
     q.o_zl = put(at, rows * 4);
@@ -512,16 +622,16 @@ HeadPlan make_plan(long long rows, long long classes, long long dim, long long w
     q.o_sumz = put(at, smoothing != 0.0f ? (size_t)rows * q.slots * 4 : 0);
     q.o_weight = put(at, q.copy_weight ? (size_t)classes * q.pitch * q.es : 0);
     q.o_delta = put(at, grad ? (size_t)rows * q.piece * q.es : 0);
-    const int bk = kRowBytes / q.es;
+    const int bk = kStageBytes / q.es;
     const long long dim_tiles = (dim + q.bm - 1) / q.bm;
     const long long wide = (dim + 3) / 4 * 4;
     if (grad_hidden) {
-        split(dim_tiles * ((rows + q.bn - 1) / q.bn), (q.piece + bk - 1) / bk, q.dh_parts, q.dh_steps);
+        q.dh_parts = split(dim_tiles * ((rows + q.bn - 1) / q.bn), (q.piece + bk - 1) / bk);
         q.o_dh = put(at, q.dh_parts > 1 || q.pieces > 1 ? (size_t)q.dh_parts * rows * wide * 4 : 0);
     }
     if (grad_weight) {
         const int bn = q.tile == 2 ? 256 : 128;
-        split(dim_tiles * ((q.piece + bn - 1) / bn), (rows + bk - 1) / bk, q.dw_parts, q.dw_steps);
+        q.dw_parts = split(dim_tiles * ((q.piece + bn - 1) / bn), (rows + bk - 1) / bk);
         q.o_dw = put(at, q.dw_parts > 1 ? (size_t)q.dw_parts * q.piece * wide * 4 : 0);
     }
     q.bytes = at;
@@ -541,40 +651,47 @@ struct HeadCall {
     char *ws;
 };
 
-template <typename T, int BM, int BN, int WM, int WN>
+// Workgroups that stay for the whole launch, as many as run at once.
+unsigned stay(const HeadCall &c, long long units, int each)
+{
+    const long long most = (long long)c.ctx->num_cus * each;
+    return (unsigned)(units < most ? (units > 0 ? units : 1) : most);
+}
+
+template <typename T, int BM, int BN, int WM, int WN, int BLOCKS>
 void launch_logits(const HeadCall &c, const LogitArgs &a, bool grad)
 {
-    const dim3 grid((unsigned)((long long)a.tiles * ((c.rows + BN - 1) / BN))), block(WM * WN * 64);
+    const dim3 grid(stay(c, (long long)a.tiles * ((c.rows + BN - 1) / BN), BLOCKS)), block(WM * WN * 64);
     if (grad)
-        launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_logit_kernel<T, BM, BN, WM, WN, true>, grid, block, a);
+        launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_logit_kernel<T, BM, BN, WM, WN, BLOCKS, true>, grid, block, a);
     else
-        launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_logit_kernel<T, BM, BN, WM, WN, false>, grid, block, a);
+        launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_logit_kernel<T, BM, BN, WM, WN, BLOCKS, false>, grid, block, a);
 }
 
 template <typename T>
 void launch_logits(const HeadCall &c, int tile, const LogitArgs &a, bool grad)
 {
-    if (tile == 0) launch_logits<T, 128, 32, 4, 1>(c, a, grad);
-    else if (tile == 1) launch_logits<T, 128, 128, 2, 2>(c, a, grad);
-    else if constexpr (sizeof(T) == 2) launch_logits<T, 256, 256, 2, 4>(c, a, grad);
+    if (tile == 0) launch_logits<T, 128, 64, 4, 1, 3>(c, a, grad);
+    else if (tile == 1) launch_logits<T, 128, 128, 2, 2, 2>(c, a, grad);
+    else if constexpr (sizeof(T) == 2) launch_logits<T, 256, 256, 2, 4, 1>(c, a, grad);
 }
 
-template <typename T, int BM, int BN, int WM, int WN, bool B_KROWS>
-void launch_grad(const HeadCall &c, GradArgs a, int parts)
+template <typename T, int BM, int BN, int WM, int WN, int BLOCKS, bool B_KROWS>
+void launch_grad(const HeadCall &c, GradArgs a)
 {
     a.tm = (a.m + BM - 1) / BM;
-    const dim3 grid((unsigned)((long long)a.tm * ((a.n + BN - 1) / BN)), (unsigned)parts), block(WM * WN * 64);
-    launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_grad_kernel<T, BM, BN, WM, WN, B_KROWS>, grid, block, a);
+    const dim3 grid(stay(c, (long long)a.parts * a.tm * ((a.n + BN - 1) / BN), BLOCKS)), block(WM * WN * 64);
+    launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_grad_kernel<T, BM, BN, WM, WN, BLOCKS, B_KROWS>, grid, block, a);
 }
 
 template <typename T>
-void launch_join(const HeadCall &c, const GradArgs &a, int parts)
+void launch_join(const HeadCall &c, const GradArgs &a)
 {
     JoinArgs j = {};
     j.part = a.part;
     j.ld_part = a.ld_part;
     j.part_stride = a.part_stride;
-    j.parts = parts;
+    j.parts = a.parts;
     j.m = a.m;
     j.n = a.n;
     j.n_count = a.n_count;
@@ -591,12 +708,11 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
 {
     ssdbox_ctx *ctx = c.ctx;
     const bool grad = c.grad_hidden || c.grad_weight;
-    int *count = (int *)(c.ws + q.o_count), *place = (int *)(c.ws + q.o_place), *row = (int *)(c.ws + q.o_row);
-    int *label = (int *)(c.ws + q.o_label);
+    int *count = (int *)(c.ws + q.o_count), *row = (int *)(c.ws + q.o_row), *label = (int *)(c.ws + q.o_label);
     HeadScale *scale = (HeadScale *)(c.ws + q.o_scale);
     T *rows = (T *)(c.ws + q.o_rows);
 
-    ScanArgs s = {};
+    PrepArgs s = {};
     s.labels = c.labels;
     s.label_bytes = c.label_bytes;
     s.rows = (int)c.rows;
@@ -604,16 +720,26 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
     s.grad_loss = grad ? c.grad_loss : nullptr;
     s.logit_scale = c.logit_scale;
     s.scaled = dtype != SSDBOX_DTYPE_F32;
-    s.place = place;
+    s.hidden = c.hidden;
+    s.ld = c.hidden_ld;
+    s.dim = (int)c.dim;
+    s.pitch = q.pitch;
+    s.wide = c.dim % q.vec == 0 && c.hidden_ld % q.vec == 0 && (uintptr_t)c.hidden % 16 == 0;
+    s.place_count = count;
     s.row = row;
     s.label = label;
-    s.count = count;
     s.scale = scale;
     s.loss = c.loss;
-    launch_stage(ctx, SSDBOX_STAGE_LOSS, head_scan_kernel, dim3(1), dim3(kScanThreads), s);
-    if (c.rows > 0)
-        launch_stage(ctx, SSDBOX_STAGE_LOSS, head_gather_kernel<T>, dim3((unsigned)c.rows), dim3(kRowThreads),
-                     (const T *)c.hidden, c.hidden_ld, place, (int)c.dim, q.pitch, rows, (T *)c.grad_hidden);
+    s.out = rows;
+    s.grad_hidden = c.grad_hidden;
+    const int n_blocks = (int)((c.rows + kCountRows - 1) / kCountRows);
+    if (c.rows > kCountFrom) {
+        s.block_count = (int *)(c.ws + q.o_blocks);
+        s.block_max = (float *)(c.ws + q.o_blocks) + n_blocks;
+        launch_stage(ctx, SSDBOX_STAGE_LOSS, head_count_kernel, dim3((unsigned)n_blocks), dim3(kRowThreads), s);
+    }
+    const unsigned n_prep = (unsigned)((c.rows + kRowsEach - 1) / kRowsEach);
+    launch_stage(ctx, SSDBOX_STAGE_LOSS, head_prep_kernel<T>, dim3(n_prep > 0 ? n_prep : 1), dim3(kRowThreads), s);
     const T *weight = (const T *)c.weight;
     long long ldw = c.weight_ld;
     if (q.copy_weight && c.rows > 0) {
@@ -692,7 +818,7 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
             h.n = (int)c.rows;
             h.n_count = count;
             h.k = n_class;
-            h.steps = q.dh_steps;
+            h.parts = q.dh_parts;
             h.out = c.grad_hidden;
             h.row_of = row;
             const bool join = q.dh_parts > 1 || q.pieces > 1;
@@ -702,10 +828,10 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
                 h.part_stride = c.rows * wide;
                 h.add = i > 0;
             }
-            if (q.tile == 0) launch_grad<T, 128, 32, 4, 1, false>(c, h, q.dh_parts);
-            else if (q.tile == 1) launch_grad<T, 128, 128, 2, 2, false>(c, h, q.dh_parts);
-            else if constexpr (sizeof(T) == 2) launch_grad<T, 256, 256, 2, 4, false>(c, h, q.dh_parts);
-            if (join && i == q.pieces - 1) launch_join<T>(c, h, q.dh_parts);
+            if (q.tile == 0) launch_grad<T, 128, 64, 4, 1, 3, false>(c, h);
+            else if (q.tile == 1) launch_grad<T, 128, 128, 2, 2, 2, false>(c, h);
+            else if constexpr (sizeof(T) == 2) launch_grad<T, 256, 256, 2, 4, 1, false>(c, h);
+            if (join && i == q.pieces - 1) launch_join<T>(c, h);
         }
         if (c.grad_weight) {
             GradArgs w = g;
@@ -716,16 +842,16 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
             w.n = n_class;
             w.k = (int)c.rows;
             w.k_count = count;
-            w.steps = q.dw_steps;
+            w.parts = q.dw_parts;
             w.out = (T *)c.grad_weight + first * c.dim;
             if (q.dw_parts > 1) {
                 w.part = (float *)(c.ws + q.o_dw);
                 w.ld_part = wide;
                 w.part_stride = q.piece * wide;
             }
-            if (q.tile != 2) launch_grad<T, 128, 128, 2, 2, true>(c, w, q.dw_parts);
-            else if constexpr (sizeof(T) == 2) launch_grad<T, 256, 256, 2, 4, true>(c, w, q.dw_parts);
-            if (q.dw_parts > 1) launch_join<T>(c, w, q.dw_parts);
+            if (q.tile != 2) launch_grad<T, 128, 128, 2, 2, 2, true>(c, w);
+            else if constexpr (sizeof(T) == 2) launch_grad<T, 256, 256, 2, 4, 1, true>(c, w);
+            if (q.dw_parts > 1) launch_join<T>(c, w);
         }
     }
     return SSDBOX_OK;

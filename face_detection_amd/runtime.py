@@ -8,6 +8,7 @@ inference.py:38-60 -- need no other GPU library.  PyTorch is used only when the 
 torch tensors (or binds a context to a torch stream): their memory and stream are then torch's.
 """
 import ctypes
+import functools
 import sys
 import threading
 
@@ -34,12 +35,18 @@ def device_count():
     return int(_lib.load().ssdbox_device_count())
 
 
+_gpu_seen = False
+
+
 def require_gpu():
     """Raises unless the library is built and an AMD GPU is visible; returns the library."""
+    global _gpu_seen
     lib = _lib.load()
-    if lib.ssdbox_device_count() <= 0:
-        raise RuntimeError("face_detection_amd needs an AMD MI355X (gfx950) GPU; none is visible "
-                           "and there is no CPU fallback")
+    if not _gpu_seen:                       # asked once: the GPUs of a process do not go
+        if lib.ssdbox_device_count() <= 0:
+            raise RuntimeError("face_detection_amd needs an AMD MI355X (gfx950) GPU; none is visible "
+                               "and there is no CPU fallback")
+        _gpu_seen = True
     return lib
 
 
@@ -64,6 +71,17 @@ def current_device():
     if _torch_runs_gpu():
         return int(_torch().cuda.current_device())
     return 0
+
+
+@functools.lru_cache(maxsize=None)
+def _torch_device(index):
+    return _torch().device("cuda", index)
+
+
+@functools.lru_cache(maxsize=None)
+def _torch_type(dtype):
+    torch = _torch()
+    return dtype if isinstance(dtype, torch.dtype) else getattr(torch, np.dtype(dtype).name)
 
 
 def _ptr(t):
@@ -561,9 +579,11 @@ class Session:
     they are DevArrays in library memory on a stream of the library's own, and torch is never
     imported."""
 
-    def __init__(self, *args, context=None, device=None):
+    def __init__(self, *args, context=None, device=None, use_torch=None):
         require_gpu()
-        self.use_torch = any(_is_torch_tensor(a) for a in args) or (context is not None and context.is_torch_stream)
+        if use_torch is None:
+            use_torch = any(_is_torch_tensor(a) for a in args)
+        self.use_torch = use_torch or (context is not None and context.is_torch_stream)
         if context is not None:
             if self.use_torch and not context.is_torch_stream:
                 raise ValueError("torch tensors need a context bound to a torch.cuda.Stream (this one runs on "
@@ -639,11 +659,7 @@ class Session:
     # ---- scratch and outputs
     def empty(self, shape, dtype=np.float32):
         if self.use_torch:
-            torch = _torch()
-            tdtype = dtype if isinstance(dtype, torch.dtype) else {
-                np.dtype(np.float32): torch.float32, np.dtype(np.int32): torch.int32,
-                np.dtype(np.uint8): torch.uint8, np.dtype(np.float16): torch.float16}[np.dtype(dtype)]
-            return torch.empty(tuple(int(s) for s in shape), dtype=tdtype, device="cuda:%d" % self.device)
+            return _torch().empty(tuple(shape), dtype=_torch_type(dtype), device=_torch_device(self.device))
         return DevArray.empty(self.ctx, shape, dtype)
 
     def from_host(self, array):
