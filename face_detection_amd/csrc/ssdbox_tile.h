@@ -222,7 +222,11 @@ struct TileStream {
     static constexpr int kBK = OpA::kBK;
     static constexpr int kLoads = OpA::kPer + OpB::kPer;                 // a stage's, per lane
 
-    // units: unit(i, TileUnit &), set(OpA &, OpB &, unit);  use(acc, unit)
+    // unit(i, TileUnit &): the i-th unit;  set(OpA &, OpB &, unit, slot): its operands, and what its epilogue wants in LDS (one
+    // of kSlots places; loaded with load_to_lds, it has landed, in all waves, when the epilogue runs: it is older than the
+    // unit's first stage);  use(acc, unit, em, en, slot): its epilogue.
+    // An epilogue does better without global loads of its own: their wait would be one for every load in flight.
+    static constexpr int kSlots = kStages + 1;   // as many units may be on their way, of a stage each
     template <typename Unit, typename Set, typename Use>
     static SSD_DEV void run(int total, const char *smem, Unit unit, Set set, Use use)
     {
@@ -237,6 +241,7 @@ struct TileStream {
         OpB b;
         TileTurns ahead = turn;
         int left = 0;                            // values of k of the unit being loaded
+        int slot_put = 0, slot_get = 0;
         const unsigned first = (unsigned)uniform((int)(lds_address(smem) + threadIdx.x / 64 * 1024u));
         unsigned put = first;                    // where the wave's pieces of the next stage go
         const auto next_put = [&]() {
@@ -252,7 +257,10 @@ struct TileStream {
                 unit(ahead.at, u);
                 ahead.at += ahead.step;
                 left = u.k;
-                if (left > 0) set(a, b, u);
+                if (left > 0) {
+                    set(a, b, u, slot_put);
+                    slot_put = slot_put == kSlots - 1 ? 0 : slot_put + 1;
+                }
             }
             a.load(put, left);
             b.load(put + BM * kStageBytes, left);
@@ -333,8 +341,9 @@ struct TileStream {
                             acc[mi][nj] = f32x16{};
                         }
             }
-            if constexpr (kTwice) use(all, u, em, en);
-            else use(acc, u, em, en);
+            if constexpr (kTwice) use(all, u, em, en, slot_get);
+            else use(acc, u, em, en, slot_get);
+            if (u.k > 0) slot_get = slot_get == kSlots - 1 ? 0 : slot_get + 1;
         }
         // LDS may be another workgroup's once this one has ended: no load may be on its way to it
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
