@@ -15,10 +15,12 @@
 // kind is read from LDS as 16 bytes of k per lane; the second is transposed on the way out of LDS (ds_read_b64_tr_b16; plain
 // 4-byte reads for float32).  So the gradients read the weight, the hidden rows and the logits' gradient as they are.
 //
-// LDS holds 16-byte pieces in an order that keeps the lanes that are read together off each other's banks; since a
-// global_load_lds writes its lanes' pieces back to back, the order is made by which piece each lane asks for:
-//   k contiguous:   piece c (of 4) of row r at c ^ (r >> 1 & 3): eight rows' pieces cover 128 bytes
-//   rows of k, 16 bit: 32-byte granule at its index ^ ((k & 3) | (k >> 3 & 1) << 2); float32 rows stay as they are
+// LDS holds 16-byte pieces in an order that keeps the lanes that are read in one clock (256 bytes, 64 banks) off each
+// other's banks; since a global_load_lds writes its lanes' pieces back to back, the order is made by which piece each lane
+// asks for:
+//   k contiguous:   piece c (of 4) of row r at c ^ (r >> 2 & 3): sixteen rows' pieces cover 256 bytes
+//   rows of k, 16 bit: 32-byte granule at its index ^ (k & 3) << 1: of four rows two granules each
+//   rows of k, float32: 128-byte block at its index ^ (k >> 2 & 1): of two rows one block each
 #pragma once
 
 #include "ssdbox_internal.h"
@@ -112,14 +114,14 @@ struct TileOperand {
     unsigned offset[kPer];           // this lane's pieces, bytes from base
     long long step;                  // bytes from one stage to the next
 
-    static SSD_DEV int granule(int k) { return (k & 3) | (k >> 3 & 1) << 2; }
+    static SSD_DEV int granule(int k) { return (k & 3) << 1; }
 
     // row of k (KROWS) or first k (otherwise) that piece i of this lane covers, within the stage
     static SSD_DEV int piece_k(int i)
     {
         const int c = i * THREADS + (int)threadIdx.x;
         const int row = c / kPiecesPerRow, pos = c % kPiecesPerRow;
-        return KROWS ? row : (pos ^ (row >> 1 & 3)) * kVec;
+        return KROWS ? row : (pos ^ (row >> 2 & 3)) * kVec;
     }
 
     // extent: rows of m / n there are from e0 on (at least 1; with KROWS a multiple of a piece); ld in values
@@ -133,12 +135,12 @@ struct TileOperand {
             const int c = i * THREADS + (int)threadIdx.x;
             const int row = c / kPiecesPerRow, pos = c % kPiecesPerRow;
             if (KROWS) {
-                int src = sizeof(T) == 2 ? (((pos >> 1) ^ granule(row)) << 1) | (pos & 1) : pos;
+                int src = sizeof(T) == 2 ? (((pos >> 1) ^ granule(row)) << 1) | (pos & 1) : pos ^ (row >> 2 & 1) << 3;
                 if (src * kVec >= extent) src = 0;       // columns beyond the last are read from the first: never stored
                 offset[i] = (unsigned)((long long)row * ldb) + (unsigned)src * 16u;
             } else {
                 const int r = row < extent ? row : extent - 1;
-                offset[i] = (unsigned)((long long)r * ldb) + (unsigned)((pos ^ (row >> 1 & 3)) * 16);
+                offset[i] = (unsigned)((long long)r * ldb) + (unsigned)((pos ^ (row >> 2 & 3)) * 16);
             }
         }
     }
@@ -162,17 +164,17 @@ struct TileOperand {
         const int lane = threadIdx.x & 63;
         if constexpr (!KROWS) {
             const int row = e + (lane & 31);
-            return *(const u32x4 *)(tile + row * kStageBytes + (((ks * 2 + (lane >> 5)) ^ (row >> 1 & 3)) << 4));
+            return *(const u32x4 *)(tile + row * kStageBytes + (((ks * 2 + (lane >> 5)) ^ (row >> 2 & 3)) << 4));
         } else if constexpr (sizeof(T) == 2) {
             typedef __attribute__((address_space(3))) s16x4 *lds4;
             const int i = lane & 15, g = lane >> 4, r = i >> 2;
             const int k = ks * 16 + 8 * (g >> 1) + r;
-            const char *p = tile + k * (E * 2) + ((((e >> 4) + (g & 1)) ^ (r | (g >> 1) << 2)) << 5) + (i & 3) * 8;
+            const char *p = tile + k * (E * 2) + ((((e >> 4) + (g & 1)) ^ r << 1) << 5) + (i & 3) * 8;
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p);
             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 4 * E * 2));
             return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         } else {
-            const char *p = tile + (ks * 8 + 4 * (lane >> 5)) * (E * 4) + (e + (lane & 31)) * 4;
+            const char *p = tile + (ks * 8 + 4 * (lane >> 5)) * (E * 4) + ((e ^ (lane >> 5) << 5) + (lane & 31)) * 4;
             u32x4 v;
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] = *(const unsigned *)(p + j * E * 4);
