@@ -10,7 +10,9 @@
 //   2  per row: log-sum-exp, loss, and what the gradient needs (four floats a row)
 //   3  per piece of the classes: the logits again, turned into d in the epilogue and written in the operands' type;
 //      dH += d W_piece, dW_piece = d^T H.
-// Recomputing the logits is 2 of the gradient's 8 rows * classes * dim operations; what it saves is rows * classes values.
+// Recomputing the logits is 2 of the gradient's 8 rows * classes * dim operations.  The last piece need not be: its place is
+// free while step 1 runs, so its exponentials wait there in 16 bits, relative to their tile's maximum, for a pass that turns
+// them into d (bfloat16 alone: float16's 11 bits round them finer than d's 8, and where d has 11 too it would be rounded twice).
 //
 // The label's own class stays out of the sum of exponentials: with S = sum over the others of exp(z_v - M), a sure row's
 // nll is log1p(S exp(M - z_l)) and p_l - 1 is expm1(-nll), both without the cancellation that 1 - p_l has.
@@ -46,8 +48,8 @@ struct PrepArgs {
     int label_bytes, rows;
     long long classes;
     const float *grad_loss;
-    float logit_scale;
-    int scaled;                       // 16-bit gradients: bring the largest c to just under 2^15
+    float logit_scale, smoothing;
+    int scaled;                       // 16-bit gradients: bring the largest c (1 - eps) to just under 2^15
     const void *hidden;
     long long ld;
     int dim, pitch;
@@ -175,9 +177,9 @@ __global__ __launch_bounds__(kRowThreads) void head_prep_kernel(const PrepArgs p
                 if (counted_at(p, n)) g = fmaxf(g, fabsf(p.grad_loss[n]));
         }
         g = block_max(g, s_max);
-        // Of float16 this uses the range; and an unsure row's d at its label, -c (1 - p), which weighs most in the
-        // gradients, lies just under a power of two, where the rounding to 8 or 11 bits is finest.
-        const float c = g * p.logit_scale;
+        // Of float16 this uses the range; and an unsure row's d at its label, -c (1 - eps - p), which weighs most in the
+        // gradients, is a value that both types have, just under a power of two, where their rounding is finest.
+        const float c = g * p.logit_scale * (1.0f - fminf(p.smoothing, 0.5f));
         if (c > 1e-30f && c < 1e30f) {
             s.down = 32768.0f * (1.0f - 1.0f / 128.0f) / c;
             s.up = 1.0f / s.down;
@@ -207,9 +209,12 @@ struct LogitArgs {
     long long slots;
     float *z_label;                   // [row]: the label's product, before the scale
     const HeadRow *row;
-    void *delta;                      // [row][ld_delta]
+    void *delta;                      // [row][ld_delta]: d, or from class kept_from on the exponentials times 2^15, float16
     long long ld_delta;
+    int kept_from;
 };
+
+enum { kStat = 0, kDelta = 1, kStatKeep = 2 };        // what a tile of logits leaves: statistics, d, statistics and exponentials
 
 // Sixteen neighbouring values of one row of the result, half of them in the lane 32 further: lo at m + 4 h .. + 3 and hi
 // at m + 8 + 4 h .. + 3 (h = lane / 32).  16-bit types trade halves, so that each lane stores 16 bytes.
@@ -245,13 +250,12 @@ SSD_DEV void store_pair(T *row, int m, const float (&lo)[4], const float (&hi)[4
     }
 }
 
-// GRAD false: statistics of a tile of logits; true: d of it.
-template <typename T, int BM, int BN, int WM, int WN, int BLOCKS, bool GRAD>
+template <typename T, int BM, int BN, int WM, int WN, int BLOCKS, int WHAT>
 __global__ __launch_bounds__(WM * WN * 64, BLOCKS * WM * WN / 4) void head_logit_kernel(const LogitArgs p)
 {
     typedef TileStream<T, BM, BN, WM, WN, false, false> S;
     // what the epilogue wants of its rows: labels (a wave's load of 1024 bytes, of which BN / 256 are wanted), and for d HeadRow
-    constexpr int kSlot = 1024 + (GRAD ? BN * 16 : 0);
+    constexpr int kSlot = 1024 + (WHAT == kDelta ? BN * 16 : 0);
     __shared__ __align__(1024) char smem[S::kLds + S::kSlots * kSlot];
     const int count = uniform(*p.count);
     const int tn = (count + BN - 1) / BN;
@@ -266,7 +270,7 @@ __global__ __launch_bounds__(WM * WN * 64, BLOCKS * WM * WN / 4) void head_logit
         const int wave = uniform(threadIdx.x / 64), lane = threadIdx.x & 63, last = (count - 1 - u.n0);
         const unsigned to = lds_address(smem) + S::kLds + slot * kSlot;
         if (wave == 0) load_to_lds_at(to, (const char *)(p.label + u.n0) + (lane * 4 <= last ? lane : last / 4) * 16);
-        if constexpr (GRAD)
+        if constexpr (WHAT == kDelta)
             for (int i = wave; i < BN / 64; i += WM * WN) {
                 const int n = i * 64 + lane;
                 load_to_lds_at(to + 1024 + i * 1024, (const char *)(p.row + u.n0 + (n <= last ? n : last)));
@@ -285,7 +289,7 @@ __global__ __launch_bounds__(WM * WN * 64, BLOCKS * WM * WN / 4) void head_logit
             const int rel = lab - (u.m0 + em);
             // the tests of single values only where one of the wave's labels lies here, or the last class
             const bool plain = !edge && !__any(rel >= 0 && rel < 32 * S::MF);
-            if constexpr (!GRAD) {
+            if constexpr (WHAT != kDelta) {
                 float mx = -INFINITY, sz = 0.0f, s = 0.0f;
                 if (plain) {
 #pragma unroll
@@ -313,23 +317,34 @@ __global__ __launch_bounds__(WM * WN * 64, BLOCKS * WM * WN / 4) void head_logit
                 }
                 mx = fmaxf(mx, __shfl_xor(mx, 32));
                 const float m = mx * p.l2;
-                const float ref = mx == -INFINITY ? 0.0f : m;
-                if (plain) {
+                // times 2^15, for what is kept in float16; the loss is to the bit the same whether something is kept or not
+                const float ref = (mx == -INFINITY ? 0.0f : m) - 15.0f;
+                const bool keep = WHAT == kStatKeep && u.m0 >= p.kept_from;
+                f16_t *kept_row = (f16_t *)p.delta + (long long)n * p.ld_delta - p.kept_from;
 #pragma unroll
-                    for (int mi = 0; mi < S::MF; ++mi)
+                for (int mi = 0; mi < S::MF; ++mi)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mi][nj][e], p.l2, -ref));
-                } else {
+                    for (int e = 0; e < 16; e += 8) {
+                        float x[2][4];
+                        const int at8 = u.m0 + em + mi * 32 + e * 2;
 #pragma unroll
-                    for (int mi = 0; mi < S::MF; ++mi)
+                        for (int i = 0; i < 8; ++i)
+                            x[i >> 2][i & 3] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mi][nj][e + i], p.l2, -ref));
+                        if (plain) {
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const int v = v0 + mi * 32 + (e >> 2) * 8 + (e & 3);
-                            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mi][nj][e], p.l2, -ref));
-                            if (v < p.classes && v != lab) s += x;
+                            for (int i = 0; i < 8; ++i) s += x[i >> 2][i & 3];
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const int v = at8 + 4 * h + (i >> 2) * 8 + (i & 3);
+                                if (v >= p.classes) x[i >> 2][i & 3] = 0.0f;
+                                if (v != lab) s += x[i >> 2][i & 3];
+                            }
                         }
-                }
+                        if constexpr (WHAT == kStatKeep)
+                            if (keep) store_pair<f16_t>(kept_row, at8, x[0], x[1], 16, true, in);
+                    }
+                s *= 0x1p-15f;
                 s += __shfl_xor(s, 32);
                 const long long slot = (long long)n * p.slots + (u.m0 + em) / (32 * S::MF);
                 if (in && h == 0) p.stat[slot] = make_float2(m, s);
@@ -458,6 +473,42 @@ __global__ __launch_bounds__(kRowThreads) void head_row_kernel(const RowArgs p)
     p.out[n] = r;
 }
 
+struct KeptArgs {
+    const int *count, *label;
+    const HeadRow *row;
+    const float2 *stat;
+    long long slots;
+    int each, first, classes;         // classes a slot; the piece's first class and how many
+    unsigned *delta;
+    long long ld_delta;
+    int blocks;                       // workgroups a row
+};
+
+// Kept exponentials to d, in place: 2^(a L - m_tile + 15) * 2^(m_tile - 15 - m) * c / Z - c eps / V.
+__global__ __launch_bounds__(kRowThreads) void head_kept_kernel(const KeptArgs p)
+{
+    const int n = blockIdx.x / p.blocks;
+    if (n >= *p.count) return;
+    const int v = ((int)(blockIdx.x % p.blocks) * kRowThreads + (int)threadIdx.x) * 8;
+    if (v >= p.ld_delta - 8) return;
+    const HeadRow r = p.row[n];
+    u32x4 *at = (u32x4 *)((char *)p.delta + (n * p.ld_delta + v) * 2);
+    union { u32x4 w; f16_t e[8]; } x;
+    union { u32x4 w; bf16_t d[8]; } o;
+    x.w = *at;
+    const long long slot = (p.first + v) / p.each;
+    const float m = slot < p.slots ? p.stat[n * p.slots + slot].x : -INFINITY;
+    const float f = __builtin_amdgcn_exp2f(m - 15.0f - r.m) * r.pz;
+    const int lab = p.label[n] - p.first;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        float d = __builtin_fmaf((float)x.e[i], f, -r.smooth);
+        if (v + i == lab) d = r.label;
+        o.d[i] = (bf16_t)(v + i < p.classes ? d : 0.0f);
+    }
+    *at = o.w;
+}
+
 // ----------------------------------------------------------------------- gradient products
 struct GradArgs {
     const void *a, *b;                // A: [k][m], m contiguous.  B: dH [n][k], dW [k][n]
@@ -545,20 +596,30 @@ struct JoinArgs {
     const int *row_of;
 };
 
-// The parts of a product over a long k, added in their order.
+// The parts of a product over a long k, added in their order.  Four values a lane, eight parts on their way at a time.
 template <typename T>
 __global__ __launch_bounds__(kRowThreads) void head_join_kernel(const JoinArgs p)
 {
-    const int n = blockIdx.x;
-    if (n >= (p.n_count ? *p.n_count : p.n)) return;
+    const int across = (p.m + 4 * 64 - 1) / (4 * 64);
+    const int id = blockIdx.x * (kRowThreads / 64) + (threadIdx.x >> 6);
+    const int n = id / across, m = (id % across * 64 + (threadIdx.x & 63)) * 4;
+    if (n >= (p.n_count ? *p.n_count : p.n) || m >= p.m) return;
     const float up = p.scale->up;
-    T *o = (T *)p.out + (p.row_of ? p.row_of[n] : n) * p.ldo;
-    for (int m = blockIdx.y * kRowThreads + threadIdx.x; m < p.m; m += kRowThreads * gridDim.y) {
-        const float *x = p.part + (long long)n * p.ld_part + m;
-        float s = 0.0f;
-        for (int i = 0; i < p.parts; ++i) s += x[i * p.part_stride];
-        o[m] = (T)(s * up);
+    const float *x = p.part + (long long)n * p.ld_part + m;
+    f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+    int i = 0;
+    for (; i + 8 <= p.parts; i += 8) {
+        f32x4 v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = *(const f32x4 *)(x + (i + j) * p.part_stride);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += v[j];
     }
+    for (; i < p.parts; ++i) s += *(const f32x4 *)(x + i * p.part_stride);
+    T *o = (T *)p.out + (p.row_of ? p.row_of[n] : n) * p.ldo + m;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (m + j < p.m) o[j] = (T)(s[j] * up);
 }
 
 // -------------------------------------------------------------------------------- plan
@@ -567,7 +628,7 @@ struct HeadPlan {
     int es, vec, tile;                // bytes and 16-byte values of a type, tile configuration
     int bm, bn, each;                 // each: classes of one wave's part of a tile of logits
     int pitch;                        // dim rounded up to 16 bytes
-    bool copy_weight;
+    bool copy_weight, keep;           // keep: the last piece's exponentials
     long long class_tiles, slots;
     long long piece, ld_delta;        // classes a piece, and from one row of its d to the next
     int pieces;
@@ -576,7 +637,10 @@ struct HeadPlan {
     size_t bytes;
 };
 
-constexpr size_t kDeltaBytes = (size_t)1 << 30;    // of one piece's d
+constexpr size_t kDeltaBytes = (size_t)1 << 31;    // of one piece's d
+// Dimensions above which the last piece's exponentials are kept.  Measured (kept, taken again): 8192 x 131072 x 768 5.56,
+// 6.36 ms; 256 x 1000003 x 512 1.54, 1.71; 8192 x 50048 x 256 1.43, 1.43; 8192 x 50048 x 64 1.05, 0.92.
+constexpr int kKeepAbove = 256;
 
 size_t put(size_t &at, size_t bytes)
 {
@@ -590,7 +654,7 @@ int split(long long tiles, long long k_stages)
 {
     long long s = tiles > 0 ? 512 / tiles : 1;
     if (s > k_stages / 8) s = k_stages / 8;
-    if (s > 64) s = 64;
+    if (s > 128) s = 128;
     return s < 1 ? 1 : (int)s;
 }
 
@@ -602,8 +666,9 @@ HeadPlan make_plan(long long rows, long long classes, long long dim, long long w
     q.vec = 16 / q.es;
     q.pitch = (int)((dim + q.vec - 1) / q.vec * q.vec);
     q.copy_weight = dim % q.vec != 0 || weight_ld % q.vec != 0;
-    // float32 keeps two sums a value (ssdbox_tile.h): the large tile's would not fit the registers
-    q.tile = rows <= 64 ? 0 : (rows <= 512 || dtype == SSDBOX_DTYPE_F32 ? 1 : 2);
+    // A tile's rows are what a weight's tile is read for: one of 256 from 129 rows on (256 x 1000003 x 512: 1.68 ms, with
+    // tiles of 128 rows 2.13).  float32 keeps two sums a value (ssdbox_tile.h): the large tile's would not fit the registers.
+    q.tile = rows <= 64 ? 0 : (rows <= 128 || dtype == SSDBOX_DTYPE_F32 ? 1 : 2);
     q.bm = q.tile == 2 ? 256 : 128;
     q.bn = q.tile == 2 ? 256 : (q.tile == 1 ? 128 : 64);
     q.each = q.tile == 2 ? 128 : (q.tile == 1 ? 64 : 32);
@@ -622,6 +687,8 @@ HeadPlan make_plan(long long rows, long long classes, long long dim, long long w
         // 256 bytes more than the piece, often a power of two: the rows that one store or load touches would otherwise all
         // lie in one channel of the L2 (d of 8192 x 65536: 2.2 -> 1.9 ms)
         q.ld_delta = q.piece + 256 / q.es;
+        // the pass over the kept exponentials and their stores move 6 bytes a logit, the products take 2 dim operations
+        q.keep = dtype == SSDBOX_DTYPE_BF16 && q.tile == 2 && dim > kKeepAbove;
     }
     size_t at = 0;
     q.o_count = put(at, 256);
@@ -672,22 +739,22 @@ unsigned stay(const HeadCall &c, long long units, int each)
     return (unsigned)(units < most ? (units > 0 ? units : 1) : most);
 }
 
-template <typename T, int BM, int BN, int WM, int WN, int BLOCKS>
-void launch_logits(const HeadCall &c, const LogitArgs &a, bool grad)
+template <typename T, int BM, int BN, int WM, int WN, int BLOCKS, int WHAT>
+void launch_tiles(const HeadCall &c, const LogitArgs &a)
 {
-    const dim3 grid(stay(c, (long long)a.tiles * ((c.rows + BN - 1) / BN), BLOCKS)), block(WM * WN * 64);
-    if (grad)
-        launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_logit_kernel<T, BM, BN, WM, WN, BLOCKS, true>, grid, block, a);
-    else
-        launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_logit_kernel<T, BM, BN, WM, WN, BLOCKS, false>, grid, block, a);
+    const unsigned grid = stay(c, (long long)a.tiles * ((c.rows + BN - 1) / BN), BLOCKS);
+    launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_logit_kernel<T, BM, BN, WM, WN, BLOCKS, WHAT>, dim3(grid),
+                 dim3(WM * WN * 64), a);
 }
 
-template <typename T>
-void launch_logits(const HeadCall &c, int tile, const LogitArgs &a, bool grad)
+template <typename T, int WHAT>
+void launch_logits(const HeadCall &c, int tile, const LogitArgs &a)
 {
-    if (tile == 0) launch_logits<T, 128, 64, 4, 1, 2>(c, a, grad);
-    else if (tile == 1) launch_logits<T, 128, 128, 2, 2, 2>(c, a, grad);
-    else if constexpr (sizeof(T) == 2) launch_logits<T, 256, 256, 2, 4, 1>(c, a, grad);
+    if constexpr (WHAT != kStatKeep) {
+        if (tile == 0) return launch_tiles<T, 128, 64, 4, 1, 2, WHAT>(c, a);
+        if (tile == 1) return launch_tiles<T, 128, 128, 2, 2, 2, WHAT>(c, a);
+    }
+    if constexpr (sizeof(T) == 2) launch_tiles<T, 256, 256, 2, 4, 1, WHAT>(c, a);
 }
 
 template <typename T, int BM, int BN, int WM, int WN, int BLOCKS, bool B_KROWS>
@@ -713,8 +780,9 @@ void launch_join(const HeadCall &c, const GradArgs &a)
     j.out = a.out;
     j.ldo = a.ldo;
     j.row_of = a.row_of;
-    const unsigned across = (unsigned)((a.m + kRowThreads - 1) / kRowThreads);
-    launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_join_kernel<T>, dim3((unsigned)a.n, across), dim3(kRowThreads), j);
+    const long long waves = (long long)a.n * ((a.m + 255) / 256), each = kRowThreads / 64;
+    launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_join_kernel<T>, dim3((unsigned)((waves + each - 1) / each)),
+                 dim3(kRowThreads), j);
 }
 
 template <typename T>
@@ -733,6 +801,7 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
     s.classes = c.classes;
     s.grad_loss = grad ? c.grad_loss : nullptr;
     s.logit_scale = c.logit_scale;
+    s.smoothing = c.smoothing;
     s.scaled = dtype != SSDBOX_DTYPE_F32;
     s.hidden = c.hidden;
     s.ld = c.hidden_ld;
@@ -781,7 +850,18 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
     l.z_label = (float *)(c.ws + q.o_zl);
     l.row = (const HeadRow *)(c.ws + q.o_out);
     if (c.rows > 0) {
-        launch_logits<T>(c, q.tile, l, false);
+        if constexpr (__is_same(T, bf16_t)) {
+            if (q.keep) {
+                l.kept_from = (int)((q.pieces - 1) * q.piece);
+                l.delta = c.ws + q.o_delta;
+                l.ld_delta = q.ld_delta;
+                launch_logits<T, kStatKeep>(c, q.tile, l);
+            } else {
+                launch_logits<T, kStat>(c, q.tile, l);
+            }
+        } else {
+            launch_logits<T, kStat>(c, q.tile, l);
+        }
         RowArgs r = {};
         r.count = count;
         r.row = row;
@@ -804,11 +884,26 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
     if (!grad) return SSDBOX_OK;
 
     const long long wide = (c.dim + 3) / 4 * 4;
-    for (int i = 0; i < q.pieces; ++i) {
+    for (int turn = 0; turn < q.pieces; ++turn) {
+        const int i = q.keep ? q.pieces - 1 - turn : turn;       // what is kept has to be used before its place is
         const long long first = i * q.piece;
         const int n_class = (int)(c.classes - first < q.piece ? c.classes - first : q.piece);
         T *delta = (T *)(c.ws + q.o_delta);
-        if (c.rows > 0) {
+        if (c.rows > 0 && q.keep && turn == 0) {
+            KeptArgs k = {};
+            k.count = count;
+            k.label = label;
+            k.row = l.row;
+            k.stat = l.stat;
+            k.slots = q.slots;
+            k.each = q.each;
+            k.first = (int)first;
+            k.classes = n_class;
+            k.delta = (unsigned *)delta;
+            k.ld_delta = q.ld_delta;
+            k.blocks = (int)((q.piece + kRowThreads * 8 - 1) / (kRowThreads * 8));
+            launch_stage(ctx, SSDBOX_STAGE_LOSS, head_kept_kernel, dim3((unsigned)(c.rows * k.blocks)), dim3(kRowThreads), k);
+        } else if (c.rows > 0) {
             LogitArgs d = l;
             d.weight = weight + first * ldw;
             d.classes = n_class;
@@ -816,7 +911,7 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
             d.tiles = (n_class + q.bm - 1) / q.bm;
             d.delta = delta;
             d.ld_delta = q.ld_delta;
-            launch_logits<T>(c, q.tile, d, true);
+            launch_logits<T, kDelta>(c, q.tile, d);
         }
         GradArgs g = {};
         g.m = (int)c.dim;
@@ -840,12 +935,12 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
                 h.part = (float *)(c.ws + q.o_dh);
                 h.ld_part = wide;
                 h.part_stride = c.rows * wide;
-                h.add = i > 0;
+                h.add = turn > 0;
             }
             if (q.tile == 0) launch_grad<T, 128, 64, 4, 1, 3, false>(c, h);
             else if (q.tile == 1) launch_grad<T, 128, 128, 2, 2, 2, false>(c, h);
             else if constexpr (sizeof(T) == 2) launch_grad<T, 256, 256, 2, 4, 1, false>(c, h);
-            if (join && i == q.pieces - 1) launch_join<T>(c, h);
+            if (join && turn == q.pieces - 1) launch_join<T>(c, h);
         }
         if (c.grad_weight) {
             GradArgs w = g;
