@@ -188,12 +188,32 @@ __global__ __launch_bounds__(kRowThreads) void head_prep_kernel(const PrepArgs p
     if (t == 0) *p.scale = s;
 }
 
-// Rows of a weight whose rows do not start at 16-byte boundaries, laid out so that they do.
+// Rows of a weight whose rows do not start at 16-byte boundaries, laid out so that they do: 16 bytes a lane, which the
+// loads take from any value's boundary.
 template <typename T>
-__global__ __launch_bounds__(kRowThreads) void head_pitch_kernel(const T *weight, long long ld, int dim, int pitch, T *out)
+__global__ __launch_bounds__(kRowThreads) void head_pitch_kernel(const T *weight, long long ld, long long classes, int dim,
+                                                                 int pitch, T *out)
 {
-    const long long v = blockIdx.x;
-    for (int d = threadIdx.x; d < pitch; d += kRowThreads) out[v * pitch + d] = d < dim ? weight[v * ld + d] : (T)0.0f;
+    constexpr int kVec = 16 / (int)sizeof(T);
+    struct __attribute__((packed, aligned(sizeof(T)))) Raw { unsigned w[4]; };
+    const int pieces = pitch / kVec;
+    const long long all = classes * pieces, step = (long long)gridDim.x * kRowThreads;
+    for (long long i = (long long)blockIdx.x * kRowThreads + threadIdx.x; i < all; i += step) {
+        const long long v = i / pieces;
+        const int d = (int)(i - v * pieces) * kVec;
+        const T *from = weight + v * ld + d;
+        u32x4 x;
+        if (d + kVec <= dim) {
+            const Raw r = *(const Raw *)from;
+            x = u32x4{r.w[0], r.w[1], r.w[2], r.w[3]};
+        } else {
+            union { T v[kVec]; u32x4 w; } y;
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) y.v[j] = d + j < dim ? from[j] : (T)0.0f;
+            x = y.w;
+        }
+        *(u32x4 *)(out + v * pitch + d) = x;
+    }
 }
 
 // --------------------------------------------------------------------------- products
@@ -396,6 +416,37 @@ struct RowArgs {
     HeadRow *out;
 };
 
+// A row's loss and its gradient's terms: the others' exponentials sum to s * 2^m, the label's is 2^(z l2) with its product z.
+SSD_DEV HeadRow row_finish(const RowArgs &p, int n, float m, double s, double sz, float z)
+{
+    const double zl = (double)z * (double)p.l2;
+    double nll = 0.0;
+    if (s != 0.0) {
+        const double d = (double)m - zl;
+        nll = d > 500.0 ? d * kLn2 + log(s) : log1p(s * exp2(d));
+    }
+    double loss = nll;
+    if (p.smoothing != 0.0f) {
+        const double mean = sz * (double)p.logit_scale / (double)p.classes;
+        loss = (1.0 - (double)p.smoothing) * nll + (double)p.smoothing * (nll + (double)z * (double)p.logit_scale - mean);
+    }
+    const int n_in = p.row[n];
+    p.loss[n_in] = (float)loss;
+    HeadRow r = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (!p.out) return r;
+    const double g = p.grad_loss ? (double)p.grad_loss[n_in] : 1.0 / (double)p.rows;
+    const double c = g * (double)p.logit_scale * (double)p.scale->down;
+    const float top = fmaxf(m, (float)zl);
+    const double whole = (s != 0.0 ? s * exp2((double)m - (double)top) : 0.0) + exp2(zl - (double)top);
+    const double share = (double)p.smoothing / (double)p.classes;
+    r.m = top;
+    r.pz = (float)(c / whole);
+    r.label = (float)(c * (expm1(-nll) + (double)p.smoothing - share));
+    r.smooth = (float)(c * share);
+    p.out[n] = r;
+    return r;
+}
+
 // One wave of the workgroup a quarter of the row's slots, then wave 0 the row.
 __global__ __launch_bounds__(kRowThreads) void head_row_kernel(const RowArgs p)
 {
@@ -444,33 +495,76 @@ __global__ __launch_bounds__(kRowThreads) void head_row_kernel(const RowArgs p)
         s += m != -INFINITY ? s_s[w] * (double)__builtin_amdgcn_exp2f(s_m[w] - m) : s_s[w];
         sz += s_z[w];
     }
-    // to base 2: the others' sum is s * 2^m, the label's term 2^zl
-    const double zl = (double)p.z_label[n] * (double)p.l2;
-    double nll = 0.0;
-    if (s != 0.0) {
-        const double d = (double)m - zl;
-        nll = d > 500.0 ? d * kLn2 + log(s) : log1p(s * exp2(d));
+    row_finish(p, n, m, s, sz, p.z_label[n]);
+}
+
+// Few tiles of logits: their products were cut along k, and here are joined (in the parts' order) a row at a time, with the
+// row's statistics and its d.
+template <typename T>
+__global__ __launch_bounds__(kRowThreads) void head_few_kernel(const RowArgs p, float *part, long long ld_part,
+                                                               long long part_stride, int parts, T *delta, long long ld_delta)
+{
+    __shared__ float s_m[kRowThreads / 64], s_label;
+    __shared__ double s_s[kRowThreads / 64], s_z[kRowThreads / 64];
+    __shared__ HeadRow s_row;
+    const int n = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    if (n >= *p.count) return;
+    float *z = part + (long long)n * ld_part;
+    const int classes = (int)p.classes, lab = p.label[n];
+    float mx = -INFINITY;
+    double sz = 0.0;
+    for (int v = t * 4; v < classes; v += kRowThreads * 4) {     // rows are padded to whole fours
+        f32x4 x = *(const f32x4 *)(z + v);
+        for (int i = 1; i < parts; ++i) x += *(const f32x4 *)(z + v + i * part_stride);
+        if (parts > 1) *(f32x4 *)(z + v) = x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (v + j >= classes) continue;
+            sz += (double)x[j];
+            if (v + j == lab) s_label = x[j];
+            else mx = fmaxf(mx, x[j]);
+        }
     }
-    const double z_label = (double)p.z_label[n] * (double)p.logit_scale;
-    double loss = nll;
-    if (p.smoothing != 0.0f) {
-        const double mean = sz * (double)p.logit_scale / (double)p.classes;
-        loss = (1.0 - (double)p.smoothing) * nll + (double)p.smoothing * (nll + z_label - mean);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        mx = fmaxf(mx, __shfl_xor(mx, o));
+        sz += __shfl_xor(sz, o);
     }
-    const int n_in = p.row[n];
-    p.loss[n_in] = (float)loss;
+    if (lane == 0) {
+        s_m[wave] = mx;
+        s_z[wave] = sz;
+    }
+    __syncthreads();
+    mx = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+    const float m = mx * p.l2, ref = mx == -INFINITY ? 0.0f : m;
+    double s = 0.0;
+    for (int v = t * 4; v < classes; v += kRowThreads * 4) {
+        const f32x4 x = *(const f32x4 *)(z + v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (v + j < classes && v + j != lab) s += (double)__builtin_amdgcn_exp2f(__builtin_fmaf(x[j], p.l2, -ref));
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    if (lane == 0) s_s[wave] = s;
+    __syncthreads();
+    if (t == 0)
+        s_row = row_finish(p, n, m, (s_s[0] + s_s[1]) + (s_s[2] + s_s[3]), (s_z[0] + s_z[1]) + (s_z[2] + s_z[3]), s_label);
     if (!p.out) return;
-    const double g = p.grad_loss ? (double)p.grad_loss[n_in] : 1.0 / (double)p.rows;
-    const double c = g * (double)p.logit_scale * (double)p.scale->down;
-    const float top = fmaxf(m, (float)zl);
-    const double whole = s * exp2((double)m - (double)top) + exp2(zl - (double)top);
-    HeadRow r;
-    r.m = top;
-    r.pz = (float)(c / (s != 0.0 ? whole : exp2(zl - (double)top)));
-    const double share = (double)p.smoothing / (double)p.classes;
-    r.label = (float)(c * (expm1(-nll) + (double)p.smoothing - share));
-    r.smooth = (float)(c * share);
-    p.out[n] = r;
+    __syncthreads();
+    const HeadRow r = s_row;
+    T *d = delta + (long long)n * ld_delta;
+    for (int v = t * 4; v < (classes + 63) / 64 * 64; v += kRowThreads * 4) {    // d has zeros behind the last class
+        struct __align__(4 * sizeof(T)) { T v[4]; } o;
+        const f32x4 x = v < classes ? *(const f32x4 *)(z + v) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float y = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(x[j], p.l2, -r.m)), r.pz, -r.smooth);
+            if (v + j == lab) y = r.label;
+            o.v[j] = (T)(v + j < classes ? y : 0.0f);
+        }
+        *(decltype(o) *)(d + v) = o;
+    }
 }
 
 struct KeptArgs {
@@ -511,9 +605,9 @@ __global__ __launch_bounds__(kRowThreads) void head_kept_kernel(const KeptArgs p
 
 // ----------------------------------------------------------------------- gradient products
 struct GradArgs {
-    const void *a, *b;                // A: [k][m], m contiguous.  B: dH [n][k], dW [k][n]
+    const void *a, *b;                // logits: [m][k], [n][k];  dH: [k][m], [n][k];  dW: [k][m], [k][n]
     long long lda, ldb;
-    int m, a_extent, n, k;            // a_extent: columns of A that may be read
+    int m, a_extent, n, k;            // a_extent: rows or columns of A that may be read
     const int *n_count, *k_count;     // device-side n or k, or NULL
     int tm;
     int parts;                        // k is cut into
@@ -526,10 +620,10 @@ struct GradArgs {
     int add;                          // to what part holds
 };
 
-template <typename T, int BM, int BN, int WM, int WN, int BLOCKS, bool B_KROWS>
+template <typename T, int BM, int BN, int WM, int WN, int BLOCKS, bool A_KROWS, bool B_KROWS>
 __global__ __launch_bounds__(WM * WN * 64, BLOCKS * WM * WN / 4) void head_grad_kernel(const GradArgs p)
 {
-    typedef TileStream<T, BM, BN, WM, WN, true, B_KROWS> S;
+    typedef TileStream<T, BM, BN, WM, WN, A_KROWS, B_KROWS> S;
     __shared__ __align__(1024) char smem[S::kLds];
     const int nn = uniform(p.n_count ? *p.n_count : p.n);
     const int kk = uniform(p.k_count ? *p.k_count : p.k);
@@ -625,15 +719,18 @@ __global__ __launch_bounds__(kRowThreads) void head_join_kernel(const JoinArgs p
 // -------------------------------------------------------------------------------- plan
 // Everything that follows from sizes: which tile, how many parts, and the workspace.
 struct HeadPlan {
-    int es, vec, tile;                // bytes and 16-byte values of a type, tile configuration
-    int bm, bn, each;                 // each: classes of one wave's part of a tile of logits
+    int es, vec;                      // bytes and 16-byte values of a type
+    int tile, dh_tile, dw_tile;       // tiles of the three products (kTileM, kTileN)
+    int bm, bn, each;                 // of the logits; each: classes of one wave's part of a tile
+    int few_parts;                    // few tiles of logits: parts of their k, or 0
+    long long few_ld;
     int pitch;                        // dim rounded up to 16 bytes
     bool copy_weight, keep;           // keep: the last piece's exponentials
     long long class_tiles, slots;
     long long piece, ld_delta;        // classes a piece, and from one row of its d to the next
     int pieces;
     int dh_parts, dw_parts;
-    size_t o_blocks, o_rows, o_weight, o_row, o_label, o_count, o_scale, o_stat, o_sumz, o_zl, o_out, o_delta, o_dh, o_dw;
+    size_t o_few, o_blocks, o_rows, o_weight, o_row, o_label, o_count, o_scale, o_stat, o_sumz, o_zl, o_out, o_delta, o_dh, o_dw;
     size_t bytes;
 };
 
@@ -649,13 +746,36 @@ size_t put(size_t &at, size_t bytes)
     return o;
 }
 
-// Parts of k so that the tiles fill the chip, at least eight stages each.
-int split(long long tiles, long long k_stages)
+constexpr int kTileM[3] = {128, 128, 256}, kTileN[3] = {64, 128, 256};
+
+long long tiles(int tile, long long m, long long n)
 {
-    long long s = tiles > 0 ? 512 / tiles : 1;
-    if (s > k_stages / 8) s = k_stages / 8;
-    if (s > 128) s = 128;
-    return s < 1 ? 1 : (int)s;
+    return (m + kTileM[tile] - 1) / kTileM[tile] * ((n + kTileN[tile] - 1) / kTileN[tile]);
+}
+
+// The tile of a product whose k cannot be cut.  The largest does most per value read, but keeps one workgroup a compute
+// unit busy for long; measured (rows x classes x dim, bfloat16, value alone; tiles of 128x64, 128x128, 256x256):
+//   512 x 32768 x 1024 - 61 55 us,  256 x 8192 x 1024 25 26 43,  1024 x 1024 x 1024 24 29 45,  8192 x 4096 x 2048 - 201 170
+// float32, whose instructions take sixteen times as long: 61 x 10007 x 512 34 53,  2048 x 8192 x 512 167 162.
+int whole_tile(long long m, long long n, int es)
+{
+    if (es == 2 && n > 128 && tiles(2, m, n) >= 256) return 2;
+    if (n > 64 && tiles(1, m, n) >= (es == 2 ? 256 : 1024)) return 1;
+    return 0;
+}
+
+// The tile of a product whose k may be cut, and into how many parts: so that the chip is filled, at least eight stages each.
+// (rows_of_k: both operands' rows are of k, which the smallest tile does not take.)
+void cut_tile(long long m, long long n, long long k_stages, int es, bool rows_of_k, int &tile, int &parts)
+{
+    if (es == 2 && n > 128 && tiles(2, m, n) * k_stages >= 256 * 16) tile = 2;
+    else if (rows_of_k || (n > 64 && tiles(1, m, n) * k_stages >= 512 * 12)) tile = 1;
+    else tile = 0;
+    const long long units = n > 0 ? tiles(tile, m, n) : 1, fill = tile == 2 ? 256 : (tile == 1 ? 512 : 768);
+    long long p = fill / units;
+    if (p > k_stages / 8) p = k_stages / 8;
+    if (p > 128) p = 128;
+    parts = p < 1 ? 1 : (int)p;
 }
 
 HeadPlan make_plan(long long rows, long long classes, long long dim, long long weight_ld, int dtype, float smoothing,
@@ -666,12 +786,18 @@ HeadPlan make_plan(long long rows, long long classes, long long dim, long long w
     q.vec = 16 / q.es;
     q.pitch = (int)((dim + q.vec - 1) / q.vec * q.vec);
     q.copy_weight = dim % q.vec != 0 || weight_ld % q.vec != 0;
-    // A tile's rows are what a weight's tile is read for: one of 256 from 129 rows on (256 x 1000003 x 512: 1.68 ms, with
-    // tiles of 128 rows 2.13).  float32 keeps two sums a value (ssdbox_tile.h): the large tile's would not fit the registers.
-    q.tile = rows <= 64 ? 0 : (rows <= 128 || dtype == SSDBOX_DTYPE_F32 ? 1 : 2);
-    q.bm = q.tile == 2 ? 256 : 128;
-    q.bn = q.tile == 2 ? 256 : (q.tile == 1 ? 128 : 64);
+    const int bk = kStageBytes / q.es;
+    q.tile = whole_tile(classes, rows, q.es);
+    q.bm = kTileM[q.tile];
+    q.bn = kTileN[q.tile];
     q.each = q.tile == 2 ? 128 : (q.tile == 1 ? 64 : 32);
+    // Half the chip idle over a long k: the logits are cut along it, and few enough to be written.
+    if (rows > 0 && tiles(q.tile, classes, rows) < 128 && q.pitch >= 16 * bk) {
+        int tile = 0;
+        cut_tile(classes, rows, (q.pitch + bk - 1) / bk, q.es, false, tile, q.few_parts);
+        q.tile = tile;
+        q.few_ld = (classes + 3) / 4 * 4;
+    }
     q.class_tiles = (classes + q.bm - 1) / q.bm;
     q.slots = q.class_tiles * (q.bm / q.each);
     const bool grad = grad_hidden || grad_weight;
@@ -688,9 +814,10 @@ HeadPlan make_plan(long long rows, long long classes, long long dim, long long w
         // lie in one channel of the L2 (d of 8192 x 65536: 2.2 -> 1.9 ms)
         q.ld_delta = q.piece + 256 / q.es;
         // the pass over the kept exponentials and their stores move 6 bytes a logit, the products take 2 dim operations
-        q.keep = dtype == SSDBOX_DTYPE_BF16 && q.tile == 2 && dim > kKeepAbove;
+        q.keep = dtype == SSDBOX_DTYPE_BF16 && q.tile == 2 && !q.few_parts && dim > kKeepAbove;
     }
     size_t at = 0;
+    q.o_few = put(at, (size_t)q.few_parts * rows * q.few_ld * 4);
     q.o_count = put(at, 256);
     q.o_scale = put(at, 256);
     q.o_blocks = put(at, rows > kCountFrom ? (rows + kCountRows - 1) / kCountRows * 8 : 0);
@@ -699,20 +826,17 @@ HeadPlan make_plan(long long rows, long long classes, long long dim, long long w
     q.o_zl = put(at, rows * 4);
     q.o_out = put(at, rows * sizeof(HeadRow));
     q.o_rows = put(at, (size_t)rows * q.pitch * q.es);
-    q.o_stat = put(at, (size_t)rows * q.slots * sizeof(float2));
-    q.o_sumz = put(at, smoothing != 0.0f ? (size_t)rows * q.slots * 4 : 0);
+    q.o_stat = put(at, q.few_parts ? 0 : (size_t)rows * q.slots * sizeof(float2));
+    q.o_sumz = put(at, smoothing != 0.0f && !q.few_parts ? (size_t)rows * q.slots * 4 : 0);
     q.o_weight = put(at, q.copy_weight ? (size_t)classes * q.pitch * q.es : 0);
     q.o_delta = put(at, grad ? (size_t)rows * q.ld_delta * q.es : 0);
-    const int bk = kStageBytes / q.es;
-    const long long dim_tiles = (dim + q.bm - 1) / q.bm;
     const long long wide = (dim + 3) / 4 * 4;
     if (grad_hidden) {
-        q.dh_parts = split(dim_tiles * ((rows + q.bn - 1) / q.bn), (q.piece + bk - 1) / bk);
+        cut_tile(dim, rows, (q.piece + bk - 1) / bk, q.es, false, q.dh_tile, q.dh_parts);
         q.o_dh = put(at, q.dh_parts > 1 || q.pieces > 1 ? (size_t)q.dh_parts * rows * wide * 4 : 0);
     }
     if (grad_weight) {
-        const int bn = q.tile == 2 ? 256 : 128;
-        q.dw_parts = split(dim_tiles * ((q.piece + bn - 1) / bn), (rows + bk - 1) / bk);
+        cut_tile(dim, classes < q.piece ? classes : q.piece, (rows + bk - 1) / bk, q.es, true, q.dw_tile, q.dw_parts);
         q.o_dw = put(at, q.dw_parts > 1 ? (size_t)q.dw_parts * q.piece * wide * 4 : 0);
     }
     q.bytes = at;
@@ -757,12 +881,22 @@ void launch_logits(const HeadCall &c, int tile, const LogitArgs &a)
     if constexpr (sizeof(T) == 2) launch_tiles<T, 256, 256, 2, 4, 1, WHAT>(c, a);
 }
 
-template <typename T, int BM, int BN, int WM, int WN, int BLOCKS, bool B_KROWS>
-void launch_grad(const HeadCall &c, GradArgs a)
+template <typename T, int BM, int BN, int WM, int WN, int BLOCKS, bool A_KROWS, bool B_KROWS>
+void launch_product(const HeadCall &c, GradArgs a)
 {
     a.tm = (a.m + BM - 1) / BM;
     const dim3 grid(stay(c, (long long)a.parts * a.tm * ((a.n + BN - 1) / BN), BLOCKS)), block(WM * WN * 64);
-    launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_grad_kernel<T, BM, BN, WM, WN, BLOCKS, B_KROWS>, grid, block, a);
+    launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_grad_kernel<T, BM, BN, WM, WN, BLOCKS, A_KROWS, B_KROWS>, grid, block, a);
+}
+
+template <typename T, bool A_KROWS, bool B_KROWS>
+void launch_product(const HeadCall &c, int tile, const GradArgs &a)
+{
+    if constexpr (!B_KROWS)
+        if (tile == 0) return launch_product<T, 128, 64, 4, 1, 3, A_KROWS, B_KROWS>(c, a);
+    if constexpr (sizeof(T) == 2)
+        if (tile == 2) return launch_product<T, 256, 256, 2, 4, 1, A_KROWS, B_KROWS>(c, a);
+    launch_product<T, 128, 128, 2, 2, 2, A_KROWS, B_KROWS>(c, a);
 }
 
 template <typename T>
@@ -827,8 +961,9 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
     long long ldw = c.weight_ld;
     if (q.copy_weight && c.rows > 0) {
         T *w = (T *)(c.ws + q.o_weight);
-        launch_stage(ctx, SSDBOX_STAGE_LOSS, head_pitch_kernel<T>, dim3((unsigned)c.classes), dim3(kRowThreads), weight,
-                     ldw, (int)c.dim, q.pitch, w);
+        const long long blocks = (c.classes * (q.pitch / q.vec) + kRowThreads - 1) / kRowThreads;
+        launch_stage(ctx, SSDBOX_STAGE_LOSS, head_pitch_kernel<T>, dim3(stay(c, blocks, 16)), dim3(kRowThreads), weight, ldw,
+                     (long long)c.classes, (int)c.dim, q.pitch, w);
         weight = w;
         ldw = q.pitch;
     }
@@ -850,18 +985,6 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
     l.z_label = (float *)(c.ws + q.o_zl);
     l.row = (const HeadRow *)(c.ws + q.o_out);
     if (c.rows > 0) {
-        if constexpr (__is_same(T, bf16_t)) {
-            if (q.keep) {
-                l.kept_from = (int)((q.pieces - 1) * q.piece);
-                l.delta = c.ws + q.o_delta;
-                l.ld_delta = q.ld_delta;
-                launch_logits<T, kStatKeep>(c, q.tile, l);
-            } else {
-                launch_logits<T, kStat>(c, q.tile, l);
-            }
-        } else {
-            launch_logits<T, kStat>(c, q.tile, l);
-        }
         RowArgs r = {};
         r.count = count;
         r.row = row;
@@ -879,7 +1002,39 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
         r.scale = scale;
         r.loss = c.loss;
         r.out = grad ? (HeadRow *)(c.ws + q.o_out) : nullptr;
-        launch_stage(ctx, SSDBOX_STAGE_LOSS, head_row_kernel, dim3((unsigned)c.rows), dim3(kRowThreads), r);
+        if (q.few_parts) {
+            GradArgs f = {};
+            f.a = weight;
+            f.lda = ldw;
+            f.b = rows;
+            f.ldb = q.pitch;
+            f.m = f.a_extent = (int)c.classes;
+            f.n = (int)c.rows;
+            f.n_count = count;
+            f.k = q.pitch;
+            f.parts = q.few_parts;
+            f.scale = scale;
+            f.part = (float *)(c.ws + q.o_few);
+            f.ld_part = q.few_ld;
+            f.part_stride = c.rows * q.few_ld;
+            launch_product<T, false, false>(c, q.tile, f);
+            launch_stage(ctx, SSDBOX_STAGE_LOSS, head_few_kernel<T>, dim3((unsigned)c.rows), dim3(kRowThreads), r, f.part,
+                         f.ld_part, f.part_stride, f.parts, (T *)(c.ws + q.o_delta), q.ld_delta);
+        } else {
+            if constexpr (__is_same(T, bf16_t)) {
+                if (q.keep) {
+                    l.kept_from = (int)((q.pieces - 1) * q.piece);
+                    l.delta = c.ws + q.o_delta;
+                    l.ld_delta = q.ld_delta;
+                    launch_logits<T, kStatKeep>(c, q.tile, l);
+                } else {
+                    launch_logits<T, kStat>(c, q.tile, l);
+                }
+            } else {
+                launch_logits<T, kStat>(c, q.tile, l);
+            }
+            launch_stage(ctx, SSDBOX_STAGE_LOSS, head_row_kernel, dim3((unsigned)c.rows), dim3(kRowThreads), r);
+        }
     }
     if (!grad) return SSDBOX_OK;
 
@@ -889,7 +1044,9 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
         const long long first = i * q.piece;
         const int n_class = (int)(c.classes - first < q.piece ? c.classes - first : q.piece);
         T *delta = (T *)(c.ws + q.o_delta);
-        if (c.rows > 0 && q.keep && turn == 0) {
+        if (q.few_parts) {
+            // d is there: few tiles are one piece
+        } else if (c.rows > 0 && q.keep && turn == 0) {
             KeptArgs k = {};
             k.count = count;
             k.label = label;
@@ -937,9 +1094,7 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
                 h.part_stride = c.rows * wide;
                 h.add = turn > 0;
             }
-            if (q.tile == 0) launch_grad<T, 128, 64, 4, 1, 3, false>(c, h);
-            else if (q.tile == 1) launch_grad<T, 128, 128, 2, 2, 2, false>(c, h);
-            else if constexpr (sizeof(T) == 2) launch_grad<T, 256, 256, 2, 4, 1, false>(c, h);
+            launch_product<T, true, false>(c, q.dh_tile, h);
             if (join && turn == q.pieces - 1) launch_join<T>(c, h);
         }
         if (c.grad_weight) {
@@ -958,8 +1113,7 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
                 w.ld_part = wide;
                 w.part_stride = q.piece * wide;
             }
-            if (q.tile != 2) launch_grad<T, 128, 128, 2, 2, 2, true>(c, w);
-            else if constexpr (sizeof(T) == 2) launch_grad<T, 256, 256, 2, 4, 1, true>(c, w);
+            launch_product<T, true, true>(c, q.dw_tile, w);
             if (q.dw_parts > 1) launch_join<T>(c, w);
         }
     }

@@ -107,6 +107,7 @@ def test_workspace_refusals_and_sizes():
     def head(rows=8, classes=10, dim=16, ld=16, dtype=0, smoothing=0.0):
         return lib.ssdbox_linear_cross_entropy_workspace(rows, classes, dim, ld, dtype, smoothing, 1, 1, ctypes.byref(need))
     assert head() == _lib.OK and need.value > 0
+    assert head(rows=0) == _lib.OK and head(rows=1, classes=1, dim=1, ld=1) == _lib.OK
     for bad in ({"rows": -1}, {"rows": (1 << 24) + 1}, {"classes": 0}, {"classes": (1 << 28) + 1}, {"dim": 0},
                 {"dim": 17}, {"ld": 15}, {"ld": (1 << 21) + 1}, {"dtype": 3}, {"dtype": -1}, {"smoothing": 1.0},
                 {"smoothing": -0.1}, {"smoothing": float("nan")}):
@@ -128,7 +129,8 @@ def test_workspace_refusals_and_sizes():
 # ------------------------------------------------------------------------------------------------------ head on the GPU
 HEAD_SIZES = [(1, 1, 1), (1, 2, 8), (3, 5, 7), (4, 1000, 128), (31, 257, 72), (32, 128, 64), (33, 129, 40), (65, 300, 33),
               (129, 255, 100), (513, 257, 136), (700, 1030, 65), (2, 30011, 16), (1500, 3, 24),
-              (130, 40, 1032), (300, 1500, 1024), (257, 515, 1030), (140, 700, 264)]
+              (130, 40, 1032), (300, 1500, 1024), (257, 515, 1030), (140, 700, 264), (4, 263, 1975), (2000, 44, 1216),
+              (1, 9000, 600)]
 
 
 @gpu
