@@ -29,9 +29,9 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.69314718055994530942;
 constexpr int kRowThreads = 256;
-constexpr int kRowsEach = 16;         // rows a workgroup places and copies
+constexpr int kRowsEach = 4;          // rows a workgroup places and copies
 constexpr int kCountRows = 1024;      // rows a workgroup counts, where there are many
-constexpr int kCountFrom = 16384;     // rows from which counting has a launch of its own: below, reading all labels before
+constexpr int kCountFrom = 4096;      // rows from which counting has a launch of its own: below, reading all labels before
                                       // a workgroup's rows again costs less than the launch
 
 struct HeadScale {                    // what the gradient's rows are multiplied by before d, and the results after
@@ -53,7 +53,6 @@ struct PrepArgs {
     const void *hidden;
     long long ld;
     int dim, pitch;
-    int wide;                         // hidden rows start at 16-byte boundaries
     int *block_count;                 // counted rows and largest |grad_loss| of every kCountRows rows, or NULL
     float *block_max;
     int *place_count;                 // the number of counted rows
@@ -148,16 +147,21 @@ __global__ __launch_bounds__(kRowThreads) void head_prep_kernel(const PrepArgs p
     __syncthreads();
     const T *hidden = (const T *)p.hidden;
     constexpr int kVec = 16 / (int)sizeof(T);
+    struct __attribute__((packed, aligned(sizeof(T)))) Raw { unsigned w[4]; };
     for (int i = t >> 6; i < kRowsEach && first + i < p.rows; i += kRowThreads / 64) {
         const long long n = first + i, at = s_place[i];
         const int lane = t & 63;
         if (at >= 0) {
+            const T *from = hidden + n * p.ld;
             T *o = (T *)p.out + at * p.pitch;
-            if (p.wide) {
-                for (int d = lane * kVec; d < p.pitch; d += 64 * kVec)
-                    *(u32x4 *)(o + d) = *(const u32x4 *)(hidden + n * p.ld + d);
-            } else {
-                for (int d = lane; d < p.pitch; d += 64) o[d] = d < p.dim ? hidden[n * p.ld + d] : (T)0.0f;
+            for (int d = lane * kVec; d < p.pitch; d += 64 * kVec) {
+                if (d + kVec <= p.dim) {
+                    const Raw r = *(const Raw *)(from + d);
+                    *(u32x4 *)(o + d) = u32x4{r.w[0], r.w[1], r.w[2], r.w[3]};
+                } else {
+#pragma unroll
+                    for (int j = 0; j < kVec; ++j) o[d + j] = d + j < p.dim ? from[d + j] : (T)0.0f;
+                }
             }
         } else if (p.grad_hidden) {
             T *o = (T *)p.grad_hidden + n * p.dim;
@@ -237,29 +241,39 @@ struct LogitArgs {
 enum { kStat = 0, kDelta = 1, kStatKeep = 2 };        // what a tile of logits leaves: statistics, d, statistics and exponentials
 
 // Sixteen neighbouring values of one row of the result, half of them in the lane 32 further: lo at m + 4 h .. + 3 and hi
-// at m + 8 + 4 h .. + 3 (h = lane / 32).  16-bit types trade halves, so that each lane stores 16 bytes.
-// Called by both lanes alike; left: values there are from m on.
+// at m + 8 + 4 h .. + 3 (h = lane / 32).  16-bit types trade halves, so that each lane stores 16 bytes (from any value's
+// boundary: rows of an odd length start there).  Called by both lanes alike; left: values there are from m on.
 template <typename T>
-SSD_DEV void store_pair(T *row, int m, const float (&lo)[4], const float (&hi)[4], int left, bool wide, bool in)
+SSD_DEV void store_pair(T *row, int m, const float (&lo)[4], const float (&hi)[4], int left, bool in)
 {
+    struct __attribute__((packed, aligned(sizeof(T)))) Raw { unsigned w[4]; };
     const int h = (int)(threadIdx.x >> 5 & 1);
-    if constexpr (sizeof(T) == 4) {
-        if (!in) return;
-        if (wide && left >= 16) {
-            *(f32x4 *)(row + m + 4 * h) = f32x4{lo[0], lo[1], lo[2], lo[3]};
-            *(f32x4 *)(row + m + 8 + 4 * h) = f32x4{hi[0], hi[1], hi[2], hi[3]};
-            return;
-        }
-    } else if (wide && left >= 16) {
-        union { T v[8]; unsigned w[4]; } x;
+    if (left >= 16) {
+        Raw a, b;
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x.v[i] = (T)lo[i];
-            x.v[4 + i] = (T)hi[i];
+            for (int i = 0; i < 4; ++i) {
+                a.w[i] = f2u(lo[i]);
+                b.w[i] = f2u(hi[i]);
+            }
+            if (!in) return;
+            *(Raw *)(row + m + 4 * h) = a;
+            *(Raw *)(row + m + 8 + 4 * h) = b;
+        } else {
+            union { T v[8]; unsigned w[4]; } x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x.v[i] = (T)lo[i];
+                x.v[4 + i] = (T)hi[i];
+            }
+            const auto p = __builtin_amdgcn_permlane32_swap(x.w[0], x.w[2], false, false);
+            const auto q = __builtin_amdgcn_permlane32_swap(x.w[1], x.w[3], false, false);
+            a.w[0] = p[0];
+            a.w[1] = q[0];
+            a.w[2] = p[1];
+            a.w[3] = q[1];
+            if (in) *(Raw *)(row + m + 8 * h) = a;
         }
-        const auto a = __builtin_amdgcn_permlane32_swap(x.w[0], x.w[2], false, false);
-        const auto b = __builtin_amdgcn_permlane32_swap(x.w[1], x.w[3], false, false);
-        if (in) *(u32x4 *)(row + m + 8 * h) = u32x4{a[0], b[0], a[1], b[1]};
         return;
     }
     if (!in) return;
@@ -362,7 +376,7 @@ __global__ __launch_bounds__(WM * WN * 64, BLOCKS * WM * WN / 4) void head_logit
                             }
                         }
                         if constexpr (WHAT == kStatKeep)
-                            if (keep) store_pair<f16_t>(kept_row, at8, x[0], x[1], 16, true, in);
+                            if (keep) store_pair<f16_t>(kept_row, at8, x[0], x[1], 16, in);
                     }
                 s *= 0x1p-15f;
                 s += __shfl_xor(s, 32);
@@ -392,7 +406,7 @@ __global__ __launch_bounds__(WM * WN * 64, BLOCKS * WM * WN / 4) void head_logit
                                 if (v == lab) d[i >> 2][i & 3] = r.label;
                                 if (v >= p.classes) d[i >> 2][i & 3] = 0.0f;
                             }
-                        store_pair<T>(out, m, d[0], d[1], 16, true, in);
+                        store_pair<T>(out, m, d[0], d[1], 16, in);
                     }
             }
         }
@@ -448,16 +462,17 @@ SSD_DEV HeadRow row_finish(const RowArgs &p, int n, float m, double s, double sz
 }
 
 // One wave of the workgroup a quarter of the row's slots, then wave 0 the row.
-__global__ __launch_bounds__(kRowThreads) void head_row_kernel(const RowArgs p)
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void head_row_kernel(const RowArgs p)
 {
-    __shared__ float s_m[kRowThreads / 64];
-    __shared__ double s_s[kRowThreads / 64], s_z[kRowThreads / 64];
+    __shared__ float s_m[THREADS / 64];
+    __shared__ double s_s[THREADS / 64], s_z[THREADS / 64];
     const int n = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
     if (n >= *p.count) return;
     const float2 *st = p.stat + (long long)n * p.slots;
     float m = -INFINITY;
     double s = 0.0, sz = 0.0;
-    for (long long i = t; i < p.slots; i += kRowThreads) {
+    for (long long i = t; i < p.slots; i += THREADS) {
         const float2 x = st[i];
         const float nm = fmaxf(m, x.x);
         if (nm != -INFINITY) {
@@ -488,10 +503,10 @@ __global__ __launch_bounds__(kRowThreads) void head_row_kernel(const RowArgs p)
     __syncthreads();
     if (t != 0) return;
     m = -INFINITY;
-    for (int w = 0; w < kRowThreads / 64; ++w) m = fmaxf(m, s_m[w]);
+    for (int w = 0; w < THREADS / 64; ++w) m = fmaxf(m, s_m[w]);
     s = 0.0;
     sz = 0.0;
-    for (int w = 0; w < kRowThreads / 64; ++w) {
+    for (int w = 0; w < THREADS / 64; ++w) {
         s += m != -INFINITY ? s_s[w] * (double)__builtin_amdgcn_exp2f(s_m[w] - m) : s_s[w];
         sz += s_z[w];
     }
@@ -500,12 +515,12 @@ __global__ __launch_bounds__(kRowThreads) void head_row_kernel(const RowArgs p)
 
 // Few tiles of logits: their products were cut along k, and here are joined (in the parts' order) a row at a time, with the
 // row's statistics and its d.
-template <typename T>
-__global__ __launch_bounds__(kRowThreads) void head_few_kernel(const RowArgs p, float *part, long long ld_part,
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void head_few_kernel(const RowArgs p, float *part, long long ld_part,
                                                                long long part_stride, int parts, T *delta, long long ld_delta)
 {
-    __shared__ float s_m[kRowThreads / 64], s_label;
-    __shared__ double s_s[kRowThreads / 64], s_z[kRowThreads / 64];
+    __shared__ float s_m[THREADS / 64], s_label;
+    __shared__ double s_s[THREADS / 64], s_z[THREADS / 64];
     __shared__ HeadRow s_row;
     const int n = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
     if (n >= *p.count) return;
@@ -513,7 +528,7 @@ __global__ __launch_bounds__(kRowThreads) void head_few_kernel(const RowArgs p, 
     const int classes = (int)p.classes, lab = p.label[n];
     float mx = -INFINITY;
     double sz = 0.0;
-    for (int v = t * 4; v < classes; v += kRowThreads * 4) {     // rows are padded to whole fours
+    for (int v = t * 4; v < classes; v += THREADS * 4) {     // rows are padded to whole fours
         f32x4 x = *(const f32x4 *)(z + v);
         for (int i = 1; i < parts; ++i) x += *(const f32x4 *)(z + v + i * part_stride);
         if (parts > 1) *(f32x4 *)(z + v) = x;
@@ -535,10 +550,10 @@ __global__ __launch_bounds__(kRowThreads) void head_few_kernel(const RowArgs p, 
         s_z[wave] = sz;
     }
     __syncthreads();
-    mx = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+    for (int w = 0; w < THREADS / 64; ++w) mx = fmaxf(mx, s_m[w]);
     const float m = mx * p.l2, ref = mx == -INFINITY ? 0.0f : m;
     double s = 0.0;
-    for (int v = t * 4; v < classes; v += kRowThreads * 4) {
+    for (int v = t * 4; v < classes; v += THREADS * 4) {
         const f32x4 x = *(const f32x4 *)(z + v);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -548,13 +563,18 @@ __global__ __launch_bounds__(kRowThreads) void head_few_kernel(const RowArgs p, 
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
     if (lane == 0) s_s[wave] = s;
     __syncthreads();
-    if (t == 0)
-        s_row = row_finish(p, n, m, (s_s[0] + s_s[1]) + (s_s[2] + s_s[3]), (s_z[0] + s_z[1]) + (s_z[2] + s_z[3]), s_label);
+    if (t == 0) {
+        for (int w = 1; w < THREADS / 64; ++w) {
+            s_s[0] += s_s[w];
+            s_z[0] += s_z[w];
+        }
+        s_row = row_finish(p, n, m, s_s[0], s_z[0], s_label);
+    }
     if (!p.out) return;
     __syncthreads();
     const HeadRow r = s_row;
     T *d = delta + (long long)n * ld_delta;
-    for (int v = t * 4; v < (classes + 63) / 64 * 64; v += kRowThreads * 4) {    // d has zeros behind the last class
+    for (int v = t * 4; v < (classes + 63) / 64 * 64; v += THREADS * 4) {    // d has zeros behind the last class
         struct __align__(4 * sizeof(T)) { T v[4]; } o;
         const f32x4 x = v < classes ? *(const f32x4 *)(z + v) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -641,7 +661,6 @@ __global__ __launch_bounds__(WM * WN * 64, BLOCKS * WM * WN / 4) void head_grad_
         b.init(p.b, p.ldb, u.n0, nn - u.n0, u.k0);
     };
     const float up = p.scale->up;
-    const bool wide = p.m % (16 / (int)sizeof(T)) == 0 && p.ldo % (16 / (int)sizeof(T)) == 0;
     const auto use = [&](f32x16 (&acc)[S::MF][S::NF], const TileUnit &u, int em, int en, int) {
         const int lane = threadIdx.x & 63, h = lane >> 5;
 #pragma unroll
@@ -671,7 +690,7 @@ __global__ __launch_bounds__(WM * WN * 64, BLOCKS * WM * WN / 4) void head_grad_
                         float d[2][4];
 #pragma unroll
                         for (int i = 0; i < 8; ++i) d[i >> 2][i & 3] = acc[mi][nj][e + i] * up;
-                        store_pair<T>(o, m, d[0], d[1], p.m - m, wide, in);
+                        store_pair<T>(o, m, d[0], d[1], p.m - m, in);
                     }
             }
         }
@@ -690,26 +709,40 @@ struct JoinArgs {
     const int *row_of;
 };
 
-// The parts of a product over a long k, added in their order.  Four values a lane, eight parts on their way at a time.
-template <typename T>
-__global__ __launch_bounds__(kRowThreads) void head_join_kernel(const JoinArgs p)
+// The parts of a product over a long k, added in a fixed order.  Four values a lane, eight parts on their way at a time;
+// WAVES waves share the parts of one piece of 256 values.
+template <typename T, int WAVES>
+__global__ __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64) void head_join_kernel(const JoinArgs p)
 {
-    const int across = (p.m + 4 * 64 - 1) / (4 * 64);
-    const int id = blockIdx.x * (kRowThreads / 64) + (threadIdx.x >> 6);
-    const int n = id / across, m = (id % across * 64 + (threadIdx.x & 63)) * 4;
-    if (n >= (p.n_count ? *p.n_count : p.n) || m >= p.m) return;
-    const float up = p.scale->up;
-    const float *x = p.part + (long long)n * p.ld_part + m;
+    constexpr int kPieces = WAVES < 4 ? 4 / WAVES : 1;
+    __shared__ f32x4 s_sum[WAVES > 1 ? WAVES : 1][64];
+    const int across = (p.m + 255) / 256, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long long id = (long long)blockIdx.x * kPieces + (WAVES > 1 ? 0 : wave);
+    const int n = (int)(id / across), m = ((int)(id % across) * 64 + lane) * 4;
+    const bool in = n < (p.n_count ? *p.n_count : p.n) && m < p.m;
     f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-    int i = 0;
-    for (; i + 8 <= p.parts; i += 8) {
-        f32x4 v[8];
+    if (in) {
+        const float *x = p.part + (long long)n * p.ld_part + m;
+        const int each = (p.parts + WAVES - 1) / WAVES;
+        int i = WAVES > 1 ? wave * each : 0;
+        const int end = min(p.parts, i + each);
+        for (; i + 8 <= end; i += 8) {
+            f32x4 v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = *(const f32x4 *)(x + (i + j) * p.part_stride);
+            for (int j = 0; j < 8; ++j) v[j] = *(const f32x4 *)(x + (i + j) * p.part_stride);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s += v[j];
+            for (int j = 0; j < 8; ++j) s += v[j];
+        }
+        for (; i < end; ++i) s += *(const f32x4 *)(x + i * p.part_stride);
     }
-    for (; i < p.parts; ++i) s += *(const f32x4 *)(x + i * p.part_stride);
+    if constexpr (WAVES > 1) {
+        s_sum[wave][lane] = s;
+        __syncthreads();
+        if (wave != 0) return;
+        for (int w = 1; w < WAVES; ++w) s += s_sum[w][lane];
+    }
+    if (!in) return;
+    const float up = p.scale->up;
     T *o = (T *)p.out + (p.row_of ? p.row_of[n] : n) * p.ldo + m;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -764,6 +797,8 @@ int whole_tile(long long m, long long n, int es)
     return 0;
 }
 
+constexpr int kPartBytes = 128 << 20;  // of a product's parts together
+
 // The tile of a product whose k may be cut, and into how many parts: so that the chip is filled, at least eight stages each.
 // (rows_of_k: both operands' rows are of k, which the smallest tile does not take.)
 void cut_tile(long long m, long long n, long long k_stages, int es, bool rows_of_k, int &tile, int &parts)
@@ -774,7 +809,8 @@ void cut_tile(long long m, long long n, long long k_stages, int es, bool rows_of
     const long long units = n > 0 ? tiles(tile, m, n) : 1, fill = tile == 2 ? 256 : (tile == 1 ? 512 : 768);
     long long p = fill / units;
     if (p > k_stages / 8) p = k_stages / 8;
-    if (p > 128) p = 128;
+    const long long most = ((long long)kPartBytes / 4) / (m * (n > 0 ? n : 1) + 1);
+    if (p > most) p = most;
     parts = p < 1 ? 1 : (int)p;
 }
 
@@ -791,8 +827,10 @@ HeadPlan make_plan(long long rows, long long classes, long long dim, long long w
     q.bm = kTileM[q.tile];
     q.bn = kTileN[q.tile];
     q.each = q.tile == 2 ? 128 : (q.tile == 1 ? 64 : 32);
-    // Half the chip idle over a long k: the logits are cut along it, and few enough to be written.
-    if (rows > 0 && tiles(q.tile, classes, rows) < 128 && q.pitch >= 16 * bk) {
+    // Much of the chip idle over a long k: the logits are cut along it, and few enough to be written.  Measured (cut, whole;
+    // value and gradients): 25 x 17213 x 1701 float32 233 301 us, 1024 x 2048 x 2048 bfloat16 102 110, 64 x 20000 x 1024 96 72.
+    const long long n_tiles = tiles(q.tile, classes, rows);
+    if (rows > 0 && q.pitch >= 16 * bk && (n_tiles < 128 || (n_tiles < 384 && (q.es == 4 || rows >= 512)))) {
         int tile = 0;
         cut_tile(classes, rows, (q.pitch + bk - 1) / bk, q.es, false, tile, q.few_parts);
         q.tile = tile;
@@ -914,9 +952,13 @@ void launch_join(const HeadCall &c, const GradArgs &a)
     j.out = a.out;
     j.ldo = a.ldo;
     j.row_of = a.row_of;
-    const long long waves = (long long)a.n * ((a.m + 255) / 256), each = kRowThreads / 64;
-    launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_join_kernel<T>, dim3((unsigned)((waves + each - 1) / each)),
-                 dim3(kRowThreads), j);
+    const long long pieces = (long long)a.n * ((a.m + 255) / 256);
+    if (a.parts < 32)
+        launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_join_kernel<T, 1>, dim3((unsigned)((pieces + 3) / 4)), dim3(256), j);
+    else if (a.parts < 256)
+        launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_join_kernel<T, 4>, dim3((unsigned)pieces), dim3(256), j);
+    else
+        launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_join_kernel<T, 16>, dim3((unsigned)pieces), dim3(1024), j);
 }
 
 template <typename T>
@@ -941,7 +983,6 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
     s.ld = c.hidden_ld;
     s.dim = (int)c.dim;
     s.pitch = q.pitch;
-    s.wide = c.dim % q.vec == 0 && c.hidden_ld % q.vec == 0 && (uintptr_t)c.hidden % 16 == 0;
     s.place_count = count;
     s.row = row;
     s.label = label;
@@ -1018,8 +1059,13 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
             f.ld_part = q.few_ld;
             f.part_stride = c.rows * q.few_ld;
             launch_product<T, false, false>(c, q.tile, f);
-            launch_stage(ctx, SSDBOX_STAGE_LOSS, head_few_kernel<T>, dim3((unsigned)c.rows), dim3(kRowThreads), r, f.part,
-                         f.ld_part, f.part_stride, f.parts, (T *)(c.ws + q.o_delta), q.ld_delta);
+            T *d = (T *)(c.ws + q.o_delta);
+            if (c.classes < 4096)
+                launch_stage(ctx, SSDBOX_STAGE_LOSS, head_few_kernel<T, 256>, dim3((unsigned)c.rows), dim3(256), r, f.part,
+                             f.ld_part, f.part_stride, f.parts, d, q.ld_delta);
+            else
+                launch_stage(ctx, SSDBOX_STAGE_LOSS, head_few_kernel<T, 1024>, dim3((unsigned)c.rows), dim3(1024), r, f.part,
+                             f.ld_part, f.part_stride, f.parts, d, q.ld_delta);
         } else {
             if constexpr (__is_same(T, bf16_t)) {
                 if (q.keep) {
@@ -1033,7 +1079,10 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
             } else {
                 launch_logits<T, kStat>(c, q.tile, l);
             }
-            launch_stage(ctx, SSDBOX_STAGE_LOSS, head_row_kernel, dim3((unsigned)c.rows), dim3(kRowThreads), r);
+            if (q.slots < 2048)
+                launch_stage(ctx, SSDBOX_STAGE_LOSS, head_row_kernel<256>, dim3((unsigned)c.rows), dim3(256), r);
+            else
+                launch_stage(ctx, SSDBOX_STAGE_LOSS, head_row_kernel<1024>, dim3((unsigned)c.rows), dim3(1024), r);
         }
     }
     if (!grad) return SSDBOX_OK;
