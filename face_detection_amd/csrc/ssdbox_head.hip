@@ -60,6 +60,10 @@ struct PrepArgs {
     HeadScale *scale;
     float *loss;
     void *out, *grad_hidden;
+    int prep_blocks;                  // workgroups of rows; the launch's others lay out the weight
+    const void *weight;
+    long long weight_ld;
+    void *weight_out;
 };
 
 SSD_DEV long long label_at(const void *p, int bytes, int n)
@@ -113,6 +117,33 @@ __global__ __launch_bounds__(kRowThreads) void head_count_kernel(const PrepArgs 
     }
 }
 
+// Rows of a weight whose rows do not start at 16-byte boundaries, laid out so that they do: 16 bytes a lane, which the
+// loads take from any value's boundary.
+template <typename T>
+SSD_DEV void pitch_weight(const T *weight, long long ld, long long classes, int dim, int pitch, T *out, int block, int blocks)
+{
+    constexpr int kVec = 16 / (int)sizeof(T);
+    struct __attribute__((packed, aligned(sizeof(T)))) Raw { unsigned w[4]; };
+    const int pieces = pitch / kVec;
+    const long long all = classes * pieces, step = (long long)blocks * kRowThreads;
+    for (long long i = (long long)block * kRowThreads + threadIdx.x; i < all; i += step) {
+        const long long v = i / pieces;
+        const int d = (int)(i - v * pieces) * kVec;
+        const T *from = weight + v * ld + d;
+        u32x4 x;
+        if (d + kVec <= dim) {
+            const Raw r = *(const Raw *)from;
+            x = u32x4{r.w[0], r.w[1], r.w[2], r.w[3]};
+        } else {
+            union { T v[kVec]; u32x4 w; } y;
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) y.v[j] = d + j < dim ? from[j] : (T)0.0f;
+            x = y.w;
+        }
+        *(u32x4 *)(out + v * pitch + d) = x;
+    }
+}
+
 // Each workgroup takes kRowsEach rows: counts the rows before them (the order of the counted rows is that of the batch, so that
 // sums over rows are the same every time), copies the counted ones to their places, with zeros behind their last value, and
 // settles the others.
@@ -122,6 +153,11 @@ __global__ __launch_bounds__(kRowThreads) void head_prep_kernel(const PrepArgs p
     __shared__ int s_count[4];
     __shared__ float s_max[4];
     __shared__ int s_place[kRowsEach];
+    if ((int)blockIdx.x >= p.prep_blocks) {
+        pitch_weight<T>((const T *)p.weight, p.weight_ld, p.classes, p.dim, p.pitch, (T *)p.weight_out,
+                        blockIdx.x - p.prep_blocks, gridDim.x - p.prep_blocks);
+        return;
+    }
     const int t = threadIdx.x, first = blockIdx.x * kRowsEach;
     const int blocks = p.block_count ? first / kCountRows : 0;
     int before = 0;
@@ -190,34 +226,6 @@ __global__ __launch_bounds__(kRowThreads) void head_prep_kernel(const PrepArgs p
         }
     }
     if (t == 0) *p.scale = s;
-}
-
-// Rows of a weight whose rows do not start at 16-byte boundaries, laid out so that they do: 16 bytes a lane, which the
-// loads take from any value's boundary.
-template <typename T>
-__global__ __launch_bounds__(kRowThreads) void head_pitch_kernel(const T *weight, long long ld, long long classes, int dim,
-                                                                 int pitch, T *out)
-{
-    constexpr int kVec = 16 / (int)sizeof(T);
-    struct __attribute__((packed, aligned(sizeof(T)))) Raw { unsigned w[4]; };
-    const int pieces = pitch / kVec;
-    const long long all = classes * pieces, step = (long long)gridDim.x * kRowThreads;
-    for (long long i = (long long)blockIdx.x * kRowThreads + threadIdx.x; i < all; i += step) {
-        const long long v = i / pieces;
-        const int d = (int)(i - v * pieces) * kVec;
-        const T *from = weight + v * ld + d;
-        u32x4 x;
-        if (d + kVec <= dim) {
-            const Raw r = *(const Raw *)from;
-            x = u32x4{r.w[0], r.w[1], r.w[2], r.w[3]};
-        } else {
-            union { T v[kVec]; u32x4 w; } y;
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) y.v[j] = d + j < dim ? from[j] : (T)0.0f;
-            x = y.w;
-        }
-        *(u32x4 *)(out + v * pitch + d) = x;
-    }
 }
 
 // --------------------------------------------------------------------------- products
@@ -411,7 +419,7 @@ __global__ __launch_bounds__(WM * WN * 64, BLOCKS * WM * WN / 4) void head_logit
             }
         }
     };
-    S::run(p.tiles * tn, smem, unit, set, use);
+    S::run(p.tiles * tn, blockIdx.x, gridDim.x, smem, unit, set, use);
 }
 
 // ------------------------------------------------------------------------ row statistics
@@ -640,11 +648,10 @@ struct GradArgs {
     int add;                          // to what part holds
 };
 
-template <typename T, int BM, int BN, int WM, int WN, int BLOCKS, bool A_KROWS, bool B_KROWS>
-__global__ __launch_bounds__(WM * WN * 64, BLOCKS * WM * WN / 4) void head_grad_kernel(const GradArgs p)
+template <typename T, int BM, int BN, int WM, int WN, bool A_KROWS, bool B_KROWS>
+SSD_DEV void product(const GradArgs &p, int block, int blocks, char *smem)
 {
     typedef TileStream<T, BM, BN, WM, WN, A_KROWS, B_KROWS> S;
-    __shared__ __align__(1024) char smem[S::kLds];
     const int nn = uniform(p.n_count ? *p.n_count : p.n);
     const int kk = uniform(p.k_count ? *p.k_count : p.k);
     const int tn = (nn + BN - 1) / BN;
@@ -695,7 +702,25 @@ __global__ __launch_bounds__(WM * WN * 64, BLOCKS * WM * WN / 4) void head_grad_
             }
         }
     };
-    S::run(p.parts * p.tm * tn, smem, unit, set, use);
+    S::run(p.parts * p.tm * tn, block, blocks, smem, unit, set, use);
+}
+
+template <typename T, int BM, int BN, int WM, int WN, int BLOCKS, bool A_KROWS, bool B_KROWS>
+__global__ __launch_bounds__(WM * WN * 64, BLOCKS * WM * WN / 4) void head_grad_kernel(const GradArgs p)
+{
+    __shared__ __align__(1024) char smem[TileStream<T, BM, BN, WM, WN, A_KROWS, B_KROWS>::kLds];
+    product<T, BM, BN, WM, WN, A_KROWS, B_KROWS>(p, blockIdx.x, gridDim.x, smem);
+}
+
+// Both gradients of d in one launch, where neither fills the chip with its largest tiles: dH by the first h_blocks workgroups.
+template <typename T, int HN, int HWM, int HWN>
+__global__ __launch_bounds__(256, 2) void head_both_kernel(const GradArgs h, const GradArgs w, int h_blocks)
+{
+    __shared__ __align__(1024) char smem[TileStream<T, 128, 128, 2, 2, true, true>::kLds];
+    if ((int)blockIdx.x < h_blocks)
+        product<T, 128, HN, HWM, HWN, true, false>(h, blockIdx.x, h_blocks, smem);
+    else
+        product<T, 128, 128, 2, 2, true, true>(w, blockIdx.x - h_blocks, gridDim.x - h_blocks, smem);
 }
 
 struct JoinArgs {
@@ -712,12 +737,14 @@ struct JoinArgs {
 // The parts of a product over a long k, added in a fixed order.  Four values a lane, eight parts on their way at a time;
 // WAVES waves share the parts of one piece of 256 values.
 template <typename T, int WAVES>
-__global__ __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64) void head_join_kernel(const JoinArgs p)
+__global__ __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64) void head_join_kernel(const JoinArgs a, const JoinArgs b, int a_blocks)
 {
+    const bool first = (int)blockIdx.x < a_blocks;
+    const JoinArgs &p = first ? a : b;
     constexpr int kPieces = WAVES < 4 ? 4 / WAVES : 1;
     __shared__ f32x4 s_sum[WAVES > 1 ? WAVES : 1][64];
     const int across = (p.m + 255) / 256, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long id = (long long)blockIdx.x * kPieces + (WAVES > 1 ? 0 : wave);
+    const long long id = (long long)(blockIdx.x - (first ? 0 : a_blocks)) * kPieces + (WAVES > 1 ? 0 : wave);
     const int n = (int)(id / across), m = ((int)(id % across) * 64 + lane) * 4;
     const bool in = n < (p.n_count ? *p.n_count : p.n) && m < p.m;
     f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -937,8 +964,7 @@ void launch_product(const HeadCall &c, int tile, const GradArgs &a)
     launch_product<T, 128, 128, 2, 2, 2, A_KROWS, B_KROWS>(c, a);
 }
 
-template <typename T>
-void launch_join(const HeadCall &c, const GradArgs &a)
+JoinArgs join_args(const GradArgs &a)
 {
     JoinArgs j = {};
     j.part = a.part;
@@ -952,13 +978,48 @@ void launch_join(const HeadCall &c, const GradArgs &a)
     j.out = a.out;
     j.ldo = a.ldo;
     j.row_of = a.row_of;
-    const long long pieces = (long long)a.n * ((a.m + 255) / 256);
-    if (a.parts < 32)
-        launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_join_kernel<T, 1>, dim3((unsigned)((pieces + 3) / 4)), dim3(256), j);
-    else if (a.parts < 256)
-        launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_join_kernel<T, 4>, dim3((unsigned)pieces), dim3(256), j);
-    else
-        launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_join_kernel<T, 16>, dim3((unsigned)pieces), dim3(1024), j);
+    return j;
+}
+
+template <typename T, int WAVES>
+void launch_join(const HeadCall &c, const JoinArgs &a, const JoinArgs &b)
+{
+    const auto blocks = [](const JoinArgs &j) {
+        const long long pieces = (long long)j.n * ((j.m + 255) / 256), each = WAVES < 4 ? 4 / WAVES : 1;
+        return (unsigned)((pieces + each - 1) / each);
+    };
+    launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_join_kernel<T, WAVES>, dim3(blocks(a) + blocks(b)),
+                 dim3(WAVES < 4 ? 256 : WAVES * 64), a, b, (int)blocks(a));
+}
+
+// One product's parts, or two's (b NULL: one's).
+template <typename T>
+void launch_join(const HeadCall &c, const GradArgs &a, const GradArgs *b)
+{
+    const JoinArgs x = join_args(a), y = b ? join_args(*b) : JoinArgs{};
+    const int parts = x.parts > y.parts ? x.parts : y.parts;
+    if (parts < 32) launch_join<T, 1>(c, x, y);
+    else if (parts < 256) launch_join<T, 4>(c, x, y);
+    else launch_join<T, 16>(c, x, y);
+}
+
+// dH and dW of one piece: together where the tiles are the smaller ones, each with a launch of its own otherwise.
+template <typename T>
+void launch_gradients(const HeadCall &c, const HeadPlan &q, GradArgs h, GradArgs w, bool want_h, bool want_w)
+{
+    if (want_h && want_w && q.dh_tile < 2 && q.dw_tile < 2) {
+        h.tm = (h.m + 127) / 128;
+        w.tm = (w.m + 127) / 128;
+        const unsigned hb = stay(c, (long long)h.parts * h.tm * ((h.n + kTileN[q.dh_tile] - 1) / kTileN[q.dh_tile]), 2);
+        const unsigned wb = stay(c, (long long)w.parts * w.tm * ((w.n + 127) / 128), 2);
+        if (q.dh_tile == 0)
+            launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_both_kernel<T, 64, 4, 1>, dim3(hb + wb), dim3(256), h, w, (int)hb);
+        else
+            launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_both_kernel<T, 128, 2, 2>, dim3(hb + wb), dim3(256), h, w, (int)hb);
+        return;
+    }
+    if (want_h) launch_product<T, true, false>(c, q.dh_tile, h);
+    if (want_w) launch_product<T, true, true>(c, q.dw_tile, w);
 }
 
 template <typename T>
@@ -996,18 +1057,20 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
         s.block_max = (float *)(c.ws + q.o_blocks) + n_blocks;
         launch_stage(ctx, SSDBOX_STAGE_LOSS, head_count_kernel, dim3((unsigned)n_blocks), dim3(kRowThreads), s);
     }
-    const unsigned n_prep = (unsigned)((c.rows + kRowsEach - 1) / kRowsEach);
-    launch_stage(ctx, SSDBOX_STAGE_LOSS, head_prep_kernel<T>, dim3(n_prep > 0 ? n_prep : 1), dim3(kRowThreads), s);
+    const unsigned n_prep = c.rows > 0 ? (unsigned)((c.rows + kRowsEach - 1) / kRowsEach) : 1;
+    unsigned n_pitch = 0;
     const T *weight = (const T *)c.weight;
     long long ldw = c.weight_ld;
     if (q.copy_weight && c.rows > 0) {
-        T *w = (T *)(c.ws + q.o_weight);
-        const long long blocks = (c.classes * (q.pitch / q.vec) + kRowThreads - 1) / kRowThreads;
-        launch_stage(ctx, SSDBOX_STAGE_LOSS, head_pitch_kernel<T>, dim3(stay(c, blocks, 16)), dim3(kRowThreads), weight, ldw,
-                     (long long)c.classes, (int)c.dim, q.pitch, w);
-        weight = w;
+        n_pitch = stay(c, (c.classes * (q.pitch / q.vec) + kRowThreads - 1) / kRowThreads, 16);
+        s.weight = weight;
+        s.weight_ld = ldw;
+        s.weight_out = c.ws + q.o_weight;
+        weight = (const T *)(c.ws + q.o_weight);
         ldw = q.pitch;
     }
+    s.prep_blocks = (int)n_prep;
+    launch_stage(ctx, SSDBOX_STAGE_LOSS, head_prep_kernel<T>, dim3(n_prep + n_pitch), dim3(kRowThreads), s);
 
     LogitArgs l = {};
     l.weight = weight;
@@ -1119,39 +1182,35 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
             d.ld_delta = q.ld_delta;
             launch_logits<T, kDelta>(c, q.tile, d);
         }
-        GradArgs g = {};
-        g.m = (int)c.dim;
-        g.a_extent = q.pitch;
-        g.scale = scale;
-        g.ldo = c.dim;
-        if (c.grad_hidden && c.rows > 0) {
-            GradArgs h = g;
+        GradArgs h = {}, w = {};
+        h.m = w.m = (int)c.dim;
+        h.a_extent = w.a_extent = q.pitch;
+        h.scale = w.scale = scale;
+        h.ldo = w.ldo = c.dim;
+        h.ldb = w.ldb = q.ld_delta;
+        h.b = w.b = delta;
+        const bool want_h = c.grad_hidden && c.rows > 0;
+        bool join_h = false, join_w = false;
+        if (want_h) {
             h.a = weight + first * ldw;
             h.lda = ldw;
-            h.b = delta;
-            h.ldb = q.ld_delta;
             h.n = (int)c.rows;
             h.n_count = count;
             h.k = n_class;
             h.parts = q.dh_parts;
             h.out = c.grad_hidden;
             h.row_of = row;
-            const bool join = q.dh_parts > 1 || q.pieces > 1;
-            if (join) {
+            if (q.dh_parts > 1 || q.pieces > 1) {
                 h.part = (float *)(c.ws + q.o_dh);
                 h.ld_part = wide;
                 h.part_stride = c.rows * wide;
                 h.add = turn > 0;
+                join_h = turn == q.pieces - 1;
             }
-            launch_product<T, true, false>(c, q.dh_tile, h);
-            if (join && turn == q.pieces - 1) launch_join<T>(c, h);
         }
         if (c.grad_weight) {
-            GradArgs w = g;
             w.a = rows;
             w.lda = q.pitch;
-            w.b = delta;
-            w.ldb = q.ld_delta;
             w.n = n_class;
             w.k = (int)c.rows;
             w.k_count = count;
@@ -1161,10 +1220,12 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
                 w.part = (float *)(c.ws + q.o_dw);
                 w.ld_part = wide;
                 w.part_stride = q.piece * wide;
+                join_w = true;
             }
-            launch_product<T, true, true>(c, q.dw_tile, w);
-            if (q.dw_parts > 1) launch_join<T>(c, w);
         }
+        launch_gradients<T>(c, q, h, w, want_h, c.grad_weight != nullptr);
+        if (join_h) launch_join<T>(c, h, join_w ? &w : nullptr);
+        else if (join_w) launch_join<T>(c, w, nullptr);
     }
     return SSDBOX_OK;
 }

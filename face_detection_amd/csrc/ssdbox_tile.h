@@ -188,17 +188,17 @@ struct TileUnit {                    // a tile (or a part of its k)
     int part;
 };
 
-// Which of `total` units a workgroup takes, in turn.  Consecutive workgroups run on different XCDs, so each XCD is given
+// Which of `total` units a workgroup, the `block`-th of `blocks`, takes, in turn.  Consecutive workgroups run on different XCDs, so each XCD is given
 // one run of the order and its workgroups go through it side by side: they share operands in its L2.
 struct TileTurns {
     int at, end, step;
-    SSD_DEV void init(int total)
+    SSD_DEV void init(int total, int block, int blocks)
     {
-        const int x = blockIdx.x % 8, q = total / 8, r = total % 8;
+        const int x = block % 8, q = total / 8, r = total % 8;
         const int lo = x * q + (x < r ? x : r);
         end = lo + q + (x < r ? 1 : 0);
-        step = ((int)gridDim.x - x + 7) / 8;
-        at = lo + (int)blockIdx.x / 8;
+        step = (blocks - x + 7) / 8;
+        at = lo + block / 8;
     }
 };
 
@@ -230,10 +230,10 @@ struct TileStream {
     // An epilogue does better without global loads of its own: their wait would be one for every load in flight.
     static constexpr int kSlots = kStages + 1;   // as many units may be on their way, of a stage each
     template <typename Unit, typename Set, typename Use>
-    static SSD_DEV void run(int total, const char *smem, Unit unit, Set set, Use use)
+    static SSD_DEV void run(int total, int block, int blocks, const char *smem, Unit unit, Set set, Use use)
     {
         TileTurns turn;
-        turn.init(total);
+        turn.init(total, block, blocks);
         if (turn.at >= turn.end) return;
         const int wave = uniform(threadIdx.x / 64);
         const int em = (wave / WN) * (BM / WM), en = (wave % WN) * (BN / WN);
