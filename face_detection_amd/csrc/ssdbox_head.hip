@@ -22,6 +22,8 @@
 // float64 for the exponentials.  d is rounded once, to the operands' type, which is what the matrix instructions read.
 #include <math.h>
 
+#include <type_traits>
+
 #include "ssdbox_tile.h"
 
 namespace {
@@ -60,6 +62,7 @@ struct PrepArgs {
     HeadScale *scale;
     float *loss;
     void *out, *grad_hidden;
+    bool stay;                        // every row keeps its place, and is copied whatever its label
     int prep_blocks;                  // workgroups of rows; the launch's others lay out the weight
     const void *weight;
     long long weight_ld;
@@ -77,16 +80,21 @@ SSD_DEV bool counted_at(const PrepArgs &p, int n)
     return lab >= 0 && lab < p.classes;
 }
 
-// Sum and maximum over the workgroup's four waves, in all lanes.
-SSD_DEV int block_total(int lane_count, int *lds)
+// Sum and maximum over the workgroup's waves, in all lanes.
+template <int WAVES>
+SSD_DEV int block_total(int x, int *lds)
 {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) lane_count += __shfl_xor(lane_count, o);
+    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = lane_count;
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
     __syncthreads();
-    return lds[0] + lds[1] + lds[2] + lds[3];
+    x = lds[0];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) x += lds[w];
+    return x;
 }
+template <int WAVES>
 SSD_DEV float block_max(float x, float *lds)
 {
 #pragma unroll
@@ -94,7 +102,38 @@ SSD_DEV float block_max(float x, float *lds)
     __syncthreads();
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
     __syncthreads();
-    return fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
+    x = lds[0];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) x = fmaxf(x, lds[w]);
+    return x;
+}
+
+// What d is scaled by: called by the whole workgroup.
+template <int WAVES>
+SSD_DEV HeadScale scale_of(const PrepArgs &p, float *lds)
+{
+    HeadScale s = {1.0f, 1.0f};
+    if (!p.scaled) return s;
+    float g = 0.0f;
+    if (!p.grad_loss) {
+        g = 1.0f / (float)p.rows;
+    } else {
+        if (p.block_count) {
+            for (int i = threadIdx.x; i < (p.rows + kCountRows - 1) / kCountRows; i += WAVES * 64) g = fmaxf(g, p.block_max[i]);
+        } else {
+            for (int n = threadIdx.x; n < p.rows; n += WAVES * 64)
+                if (counted_at(p, n)) g = fmaxf(g, fabsf(p.grad_loss[n]));
+        }
+        g = block_max<WAVES>(g, lds);
+    }
+    // Of float16 this uses the range; and an unsure row's d at its label, -c (1 - eps - p), which weighs most in the
+    // gradients, is a value that both types have, just under a power of two, where their rounding is finest.
+    const float c = g * p.logit_scale * (1.0f - fminf(p.smoothing, 0.5f));
+    if (c > 1e-30f && c < 1e30f) {
+        s.down = 32768.0f * (1.0f - 1.0f / 128.0f) / c;
+        s.up = 1.0f / s.down;
+    }
+    return s;
 }
 
 __global__ __launch_bounds__(kRowThreads) void head_count_kernel(const PrepArgs p)
@@ -109,8 +148,8 @@ __global__ __launch_bounds__(kRowThreads) void head_count_kernel(const PrepArgs 
             ++c;
             if (p.grad_loss) g = fmaxf(g, fabsf(p.grad_loss[n]));
         }
-    c = block_total(c, s_count);
-    g = block_max(g, s_max);
+    c = block_total<kRowThreads / 64>(c, s_count);
+    g = block_max<kRowThreads / 64>(g, s_max);
     if (threadIdx.x == 0) {
         p.block_count[blockIdx.x] = c;
         p.block_max[blockIdx.x] = g;
@@ -159,26 +198,30 @@ __global__ __launch_bounds__(kRowThreads) void head_prep_kernel(const PrepArgs p
         return;
     }
     const int t = threadIdx.x, first = blockIdx.x * kRowsEach;
-    const int blocks = p.block_count ? first / kCountRows : 0;
-    int before = 0;
-    for (int i = t; i < blocks; i += kRowThreads) before += p.block_count[i];
-    for (int n = blocks * kCountRows + t; n < first; n += kRowThreads) before += counted_at(p, n) ? 1 : 0;
-    before = block_total(before, s_count);
-    if (t < 64) {
-        const int n = first + t;
-        const bool mine = t < kRowsEach && n < p.rows;
-        const long long lab = mine ? label_at(p.labels, p.label_bytes, n) : -1;
-        const bool counted = lab >= 0 && lab < p.classes;
-        const unsigned long long bal = __ballot(counted);
-        const int at = before + __popcll(bal & ((1ull << t) - 1ull));
-        if (counted) {
-            p.row[at] = n;
-            p.label[at] = (int)lab;
-        } else if (mine) {
-            p.loss[n] = lab < 0 ? 0.0f : u2f(0x7FC00000u);
+    if (p.stay) {
+        if (t < kRowsEach) s_place[t] = first + t;
+    } else {
+        const int blocks = p.block_count ? first / kCountRows : 0;
+        int before = 0;
+        for (int i = t; i < blocks; i += kRowThreads) before += p.block_count[i];
+        for (int n = blocks * kCountRows + t; n < first; n += kRowThreads) before += counted_at(p, n) ? 1 : 0;
+        before = block_total<kRowThreads / 64>(before, s_count);
+        if (t < 64) {
+            const int n = first + t;
+            const bool mine = t < kRowsEach && n < p.rows;
+            const long long lab = mine ? label_at(p.labels, p.label_bytes, n) : -1;
+            const bool counted = lab >= 0 && lab < p.classes;
+            const unsigned long long bal = __ballot(counted);
+            const int at = before + __popcll(bal & ((1ull << t) - 1ull));
+            if (counted) {
+                p.row[at] = n;
+                p.label[at] = (int)lab;
+            } else if (mine) {
+                p.loss[n] = lab < 0 ? 0.0f : u2f(0x7FC00000u);
+            }
+            if (t < kRowsEach) s_place[t] = counted ? at : -1;
+            if (t == 0 && first + kRowsEach >= p.rows) *p.place_count = before + __popcll(bal);
         }
-        if (t < kRowsEach) s_place[t] = counted ? at : -1;
-        if (t == 0 && first + kRowsEach >= p.rows) *p.place_count = before + __popcll(bal);
     }
     __syncthreads();
     const T *hidden = (const T *)p.hidden;
@@ -204,27 +247,8 @@ __global__ __launch_bounds__(kRowThreads) void head_prep_kernel(const PrepArgs p
             for (int d = lane; d < p.dim; d += 64) o[d] = (T)0.0f;
         }
     }
-    if (blockIdx.x != 0) return;
-    HeadScale s = {1.0f, 1.0f};
-    if (p.scaled) {
-        float g = 0.0f;
-        if (!p.grad_loss) {
-            g = 1.0f / (float)p.rows;
-        } else if (p.block_count) {
-            for (int i = t; i < (p.rows + kCountRows - 1) / kCountRows; i += kRowThreads) g = fmaxf(g, p.block_max[i]);
-        } else {
-            for (int n = t; n < p.rows; n += kRowThreads)
-                if (counted_at(p, n)) g = fmaxf(g, fabsf(p.grad_loss[n]));
-        }
-        g = block_max(g, s_max);
-        // Of float16 this uses the range; and an unsure row's d at its label, -c (1 - eps - p), which weighs most in the
-        // gradients, is a value that both types have, just under a power of two, where their rounding is finest.
-        const float c = g * p.logit_scale * (1.0f - fminf(p.smoothing, 0.5f));
-        if (c > 1e-30f && c < 1e30f) {
-            s.down = 32768.0f * (1.0f - 1.0f / 128.0f) / c;
-            s.up = 1.0f / s.down;
-        }
-    }
+    if (p.stay || blockIdx.x != 0) return;
+    const HeadScale s = scale_of<kRowThreads / 64>(p, s_max);
     if (t == 0) *p.scale = s;
 }
 
@@ -241,12 +265,14 @@ struct LogitArgs {
     long long slots;
     float *z_label;                   // [row]: the label's product, before the scale
     const HeadRow *row;
-    void *delta;                      // [row][ld_delta]: d, or from class kept_from on the exponentials times 2^15, float16
+    void *delta;                      // [row][ld_delta]: d, or from class kept_from on what is kept
     long long ld_delta;
     int kept_from;
 };
 
-enum { kStat = 0, kDelta = 1, kStatKeep = 2 };        // what a tile of logits leaves: statistics, d, statistics and exponentials
+// What a tile of logits leaves: statistics, d, or statistics and what d can be made of later (of 16-bit types exponentials
+// times 2^15 as float16, of float32 the products themselves)
+enum { kStat = 0, kDelta = 1, kStatKeep = 2 };
 
 // Sixteen neighbouring values of one row of the result, half of them in the lane 32 further: lo at m + 4 h .. + 3 and hi
 // at m + 8 + 4 h .. + 3 (h = lane / 32).  16-bit types trade halves, so that each lane stores 16 bytes (from any value's
@@ -362,13 +388,19 @@ __global__ __launch_bounds__(WM * WN * 64, BLOCKS * WM * WN / 4) void head_logit
                 // times 2^15, for what is kept in float16; the loss is to the bit the same whether something is kept or not
                 const float ref = (mx == -INFINITY ? 0.0f : m) - 15.0f;
                 const bool keep = WHAT == kStatKeep && u.m0 >= p.kept_from;
-                f16_t *kept_row = (f16_t *)p.delta + (long long)n * p.ld_delta - p.kept_from;
+                typedef typename std::conditional<sizeof(T) == 4, float, f16_t>::type Kept;
+                Kept *kept_row = (Kept *)p.delta + (long long)n * p.ld_delta - p.kept_from;
 #pragma unroll
                 for (int mi = 0; mi < S::MF; ++mi)
 #pragma unroll
                     for (int e = 0; e < 16; e += 8) {
                         float x[2][4];
                         const int at8 = u.m0 + em + mi * 32 + e * 2;
+                        if constexpr (WHAT == kStatKeep && sizeof(T) == 4) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) x[i >> 2][i & 3] = acc[mi][nj][e + i];
+                            if (keep) store_pair<float>(kept_row, at8, x[0], x[1], 16, in);
+                        }
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
                             x[i >> 2][i & 3] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mi][nj][e + i], p.l2, -ref));
@@ -383,7 +415,7 @@ __global__ __launch_bounds__(WM * WN * 64, BLOCKS * WM * WN / 4) void head_logit
                                 if (v != lab) s += x[i >> 2][i & 3];
                             }
                         }
-                        if constexpr (WHAT == kStatKeep)
+                        if constexpr (WHAT == kStatKeep && sizeof(T) == 2)
                             if (keep) store_pair<f16_t>(kept_row, at8, x[0], x[1], 16, in);
                     }
                 s *= 0x1p-15f;
@@ -439,7 +471,7 @@ struct RowArgs {
 };
 
 // A row's loss and its gradient's terms: the others' exponentials sum to s * 2^m, the label's is 2^(z l2) with its product z.
-SSD_DEV HeadRow row_finish(const RowArgs &p, int n, float m, double s, double sz, float z)
+SSD_DEV HeadRow row_finish(const RowArgs &p, int n_in, float down, float m, double s, double sz, float z)
 {
     const double zl = (double)z * (double)p.l2;
     double nll = 0.0;
@@ -452,12 +484,11 @@ SSD_DEV HeadRow row_finish(const RowArgs &p, int n, float m, double s, double sz
         const double mean = sz * (double)p.logit_scale / (double)p.classes;
         loss = (1.0 - (double)p.smoothing) * nll + (double)p.smoothing * (nll + (double)z * (double)p.logit_scale - mean);
     }
-    const int n_in = p.row[n];
     p.loss[n_in] = (float)loss;
     HeadRow r = {0.0f, 0.0f, 0.0f, 0.0f};
     if (!p.out) return r;
     const double g = p.grad_loss ? (double)p.grad_loss[n_in] : 1.0 / (double)p.rows;
-    const double c = g * (double)p.logit_scale * (double)p.scale->down;
+    const double c = g * (double)p.logit_scale * (double)down;
     const float top = fmaxf(m, (float)zl);
     const double whole = (s != 0.0 ? s * exp2((double)m - (double)top) : 0.0) + exp2(zl - (double)top);
     const double share = (double)p.smoothing / (double)p.classes;
@@ -465,11 +496,10 @@ SSD_DEV HeadRow row_finish(const RowArgs &p, int n, float m, double s, double sz
     r.pz = (float)(c / whole);
     r.label = (float)(c * (expm1(-nll) + (double)p.smoothing - share));
     r.smooth = (float)(c * share);
-    p.out[n] = r;
     return r;
 }
 
-// One wave of the workgroup a quarter of the row's slots, then wave 0 the row.
+// A row a workgroup: its tiles' statistics together, then its loss.
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void head_row_kernel(const RowArgs p)
 {
@@ -518,22 +548,55 @@ __global__ __launch_bounds__(THREADS) void head_row_kernel(const RowArgs p)
         s += m != -INFINITY ? s_s[w] * (double)__builtin_amdgcn_exp2f(s_m[w] - m) : s_s[w];
         sz += s_z[w];
     }
-    row_finish(p, n, m, s, sz, p.z_label[n]);
+    const HeadRow r = row_finish(p, p.row[n], p.out ? p.scale->down : 1.0f, m, s, sz, p.z_label[n]);
+    if (p.out) p.out[n] = r;
 }
 
-// Few tiles of logits: their products were cut along k, and here are joined (in the parts' order) a row at a time, with the
-// row's statistics and its d.
-template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS) void head_few_kernel(const RowArgs p, float *part, long long ld_part,
-                                                               long long part_stride, int parts, T *delta, long long ld_delta)
+// Few logits: their products (in parts, where k was cut) are joined in the parts' order a row at a time, with the row's
+// statistics and its d.  DIRECT: of the batch's own rows, which nothing has placed before; what prep does then happens here,
+// but that the rows without a class stay where they are, with d and values of zero (row_of -1: their gradient is written here).
+template <typename T, int THREADS, bool DIRECT>
+__global__ __launch_bounds__(THREADS) void head_few_kernel(const RowArgs p, const PrepArgs b, float *part, long long ld_part,
+                                                           long long part_stride, int parts, T *delta, long long ld_delta)
 {
-    __shared__ float s_m[THREADS / 64], s_label;
+    __shared__ float s_m[THREADS / 64], s_g[THREADS / 64], s_label;
     __shared__ double s_s[THREADS / 64], s_z[THREADS / 64];
     __shared__ HeadRow s_row;
-    const int n = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    if (n >= *p.count) return;
+    const int n = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6, classes = (int)p.classes;
+    int lab, n_in;
+    float down = 1.0f;
+    if constexpr (DIRECT) {
+        if (p.out) {
+            const HeadScale s = scale_of<THREADS / 64>(b, s_g);
+            down = s.down;
+            if (n == 0 && t == 0) *b.scale = s;
+        }
+        const long long given = label_at(b.labels, b.label_bytes, n);
+        const bool counted = given >= 0 && given < p.classes;
+        lab = (int)given;
+        n_in = n;
+        if (p.out) {
+            if (t == 0) b.row[n] = counted ? n : -1;
+            constexpr int kVec = 16 / (int)sizeof(T);
+            for (int d = t * kVec; d < b.pitch; d += THREADS * kVec)
+                *(u32x4 *)((T *)b.out + (long long)n * b.pitch + d) =
+                    counted ? *(const u32x4 *)((const T *)b.hidden + n * b.ld + d) : u32x4{0u, 0u, 0u, 0u};
+        }
+        if (!counted) {
+            if (t == 0) p.loss[n] = given < 0 ? 0.0f : u2f(0x7FC00000u);
+            if (!p.out) return;
+            for (int v = t; v < (classes + 63) / 64 * 64; v += THREADS) delta[n * ld_delta + v] = (T)0.0f;
+            if (b.grad_hidden)
+                for (int d = t; d < b.dim; d += THREADS) ((T *)b.grad_hidden)[(long long)n * b.dim + d] = (T)0.0f;
+            return;
+        }
+    } else {
+        if (n >= *p.count) return;
+        lab = p.label[n];
+        n_in = p.row[n];
+        if (p.out) down = p.scale->down;
+    }
     float *z = part + (long long)n * ld_part;
-    const int classes = (int)p.classes, lab = p.label[n];
     float mx = -INFINITY;
     double sz = 0.0;
     for (int v = t * 4; v < classes; v += THREADS * 4) {     // rows are padded to whole fours
@@ -576,7 +639,7 @@ __global__ __launch_bounds__(THREADS) void head_few_kernel(const RowArgs p, floa
             s_s[0] += s_s[w];
             s_z[0] += s_z[w];
         }
-        s_row = row_finish(p, n, m, s_s[0], s_z[0], s_label);
+        s_row = row_finish(p, n_in, down, m, s_s[0], s_z[0], s_label);
     }
     if (!p.out) return;
     __syncthreads();
@@ -601,32 +664,42 @@ struct KeptArgs {
     const float2 *stat;
     long long slots;
     int each, first, classes;         // classes a slot; the piece's first class and how many
-    unsigned *delta;
+    float l2;
+    void *delta;
     long long ld_delta;
     int blocks;                       // workgroups a row
 };
 
-// Kept exponentials to d, in place: 2^(a L - m_tile + 15) * 2^(m_tile - 15 - m) * c / Z - c eps / V.
+// What was kept to d, in place, 16 bytes a lane.  bfloat16, of exponentials: 2^(a L - m_tile + 15) * 2^(m_tile - 15 - m) * c / Z
+// - c eps / V.  float32, of products: as the logits' epilogue does it.
+template <typename T>
 __global__ __launch_bounds__(kRowThreads) void head_kept_kernel(const KeptArgs p)
 {
+    constexpr int kVec = 16 / (int)sizeof(T);
+    typedef typename std::conditional<sizeof(T) == 4, float, f16_t>::type Kept;
     const int n = blockIdx.x / p.blocks;
     if (n >= *p.count) return;
-    const int v = ((int)(blockIdx.x % p.blocks) * kRowThreads + (int)threadIdx.x) * 8;
-    if (v >= p.ld_delta - 8) return;
+    const int v = ((int)(blockIdx.x % p.blocks) * kRowThreads + (int)threadIdx.x) * kVec;
+    if (v >= p.ld_delta - kVec) return;
     const HeadRow r = p.row[n];
-    u32x4 *at = (u32x4 *)((char *)p.delta + (n * p.ld_delta + v) * 2);
-    union { u32x4 w; f16_t e[8]; } x;
-    union { u32x4 w; bf16_t d[8]; } o;
+    u32x4 *at = (u32x4 *)((T *)p.delta + n * p.ld_delta + v);
+    union { u32x4 w; Kept e[kVec]; } x;
+    union { u32x4 w; T d[kVec]; } o;
     x.w = *at;
-    const long long slot = (p.first + v) / p.each;
-    const float m = slot < p.slots ? p.stat[n * p.slots + slot].x : -INFINITY;
-    const float f = __builtin_amdgcn_exp2f(m - 15.0f - r.m) * r.pz;
+    float f = 0.0f;
+    if constexpr (sizeof(T) == 2) {
+        const long long slot = (p.first + v) / p.each;
+        const float m = slot < p.slots ? p.stat[n * p.slots + slot].x : -INFINITY;
+        f = __builtin_amdgcn_exp2f(m - 15.0f - r.m) * r.pz;
+    }
     const int lab = p.label[n] - p.first;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        float d = __builtin_fmaf((float)x.e[i], f, -r.smooth);
+    for (int i = 0; i < kVec; ++i) {
+        float d;
+        if constexpr (sizeof(T) == 2) d = __builtin_fmaf((float)x.e[i], f, -r.smooth);
+        else d = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(x.e[i], p.l2, -r.m)), r.pz, -r.smooth);
         if (v + i == lab) d = r.label;
-        o.d[i] = (bf16_t)(v + i < p.classes ? d : 0.0f);
+        o.d[i] = (T)(v + i < p.classes ? d : 0.0f);
     }
     *at = o.w;
 }
@@ -673,7 +746,7 @@ SSD_DEV void product(const GradArgs &p, int block, int blocks, char *smem)
 #pragma unroll
         for (int nj = 0; nj < S::NF; ++nj) {
             const int n = u.n0 + en + nj * 32 + (lane & 31);
-            const bool in = n < nn;
+            bool in = n < nn;
             if (p.part) {
                 float *o = p.part + u.part * p.part_stride + (long long)n * p.ld_part;
 #pragma unroll
@@ -688,7 +761,9 @@ SSD_DEV void product(const GradArgs &p, int block, int blocks, char *smem)
                         }
                     }
             } else {
-                T *o = (T *)p.out + (in ? (p.row_of ? (long long)p.row_of[n] : (long long)n) : 0) * p.ldo;
+                const int to = in ? (p.row_of ? p.row_of[n] : n) : -1;
+                in = to >= 0;
+                T *o = (T *)p.out + (in ? (long long)to : 0) * p.ldo;
 #pragma unroll
                 for (int mi = 0; mi < S::MF; ++mi)
 #pragma unroll
@@ -727,6 +802,7 @@ struct JoinArgs {
     const float *part;
     long long ld_part, part_stride;
     int parts, m, n;
+    int waves;                        // that share a piece's parts: with it goes the order of the sum, which is a product's own
     const int *n_count;
     const HeadScale *scale;
     void *out;
@@ -750,7 +826,7 @@ __global__ __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64) void head_join_kernel
     f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
     if (in) {
         const float *x = p.part + (long long)n * p.ld_part + m;
-        const int each = (p.parts + WAVES - 1) / WAVES;
+        const int each = (p.parts + p.waves - 1) / p.waves;
         int i = WAVES > 1 ? wave * each : 0;
         const int end = min(p.parts, i + each);
         for (; i + 8 <= end; i += 8) {
@@ -766,17 +842,28 @@ __global__ __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64) void head_join_kernel
         s_sum[wave][lane] = s;
         __syncthreads();
         if (wave != 0) return;
-        for (int w = 1; w < WAVES; ++w) s += s_sum[w][lane];
+        for (int w = 1; w < p.waves; ++w) s += s_sum[w][lane];
     }
     if (!in) return;
+    const int to = p.row_of ? p.row_of[n] : n;
+    if (to < 0) return;
     const float up = p.scale->up;
-    T *o = (T *)p.out + (p.row_of ? p.row_of[n] : n) * p.ldo + m;
+    T *o = (T *)p.out + to * p.ldo + m;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
         if (m + j < p.m) o[j] = (T)(s[j] * up);
 }
 
 // -------------------------------------------------------------------------------- plan
+// Few logits are written (float32, they stay in the caches) and joined a row a workgroup, which a row of more than
+// kFewClasses keeps too busy; and where they are little work too, the rows stay where they are: one launch less, while padded
+// rows cost what the others cost.  A call of so little work is as long as its launches are many: a gradient takes three
+// (products, rows, both gradients) instead of six.  Measured (rows x classes x dim, bfloat16, with gradients; before, now):
+//   1000 x 1000 x 256 50 32 us,  4000 x 200 x 256 52 36,  1000 x 4000 x 256 62 51,  250 x 4000 x 1500 71 63,
+//   4000 x 2000 x 64 63 54;  float32: 138 x 882 x 248 67 36,  1000 x 4000 x 128 81 75
+constexpr long long kFewLogits = 1 << 23, kFewClasses = 1 << 14;
+constexpr double kDirectWork = 1ll << 31, kDirectWorkF32 = 1 << 29;   // rows * classes * dim
+
 // Everything that follows from sizes: which tile, how many parts, and the workspace.
 struct HeadPlan {
     int es, vec;                      // bytes and 16-byte values of a type
@@ -785,7 +872,8 @@ struct HeadPlan {
     int few_parts;                    // few tiles of logits: parts of their k, or 0
     long long few_ld;
     int pitch;                        // dim rounded up to 16 bytes
-    bool copy_weight, keep;           // keep: the last piece's exponentials
+    bool copy_weight, keep;           // keep: of the last piece what d can be made of
+    bool direct;                      // few logits and little work: the rows stay where they are
     long long class_tiles, slots;
     long long piece, ld_delta;        // classes a piece, and from one row of its d to the next
     int pieces;
@@ -857,7 +945,10 @@ HeadPlan make_plan(long long rows, long long classes, long long dim, long long w
     // Much of the chip idle over a long k: the logits are cut along it, and few enough to be written.  Measured (cut, whole;
     // value and gradients): 25 x 17213 x 1701 float32 233 301 us, 1024 x 2048 x 2048 bfloat16 102 110, 64 x 20000 x 1024 96 72.
     const long long n_tiles = tiles(q.tile, classes, rows);
-    if (rows > 0 && q.pitch >= 16 * bk && (n_tiles < 128 || (n_tiles < 384 && (q.es == 4 || rows >= 512)))) {
+    const bool few = rows > 0 && rows * classes <= kFewLogits && classes <= kFewClasses;
+    q.direct = few && rows <= kCountFrom &&
+               (double)rows * (double)classes * (double)dim <= (q.es == 4 ? kDirectWorkF32 : kDirectWork);
+    if (few || (rows > 0 && q.pitch >= 16 * bk && (n_tiles < 128 || (n_tiles < 384 && (q.es == 4 || rows >= 512))))) {
         int tile = 0;
         cut_tile(classes, rows, (q.pitch + bk - 1) / bk, q.es, false, tile, q.few_parts);
         q.tile = tile;
@@ -879,7 +970,8 @@ HeadPlan make_plan(long long rows, long long classes, long long dim, long long w
         // lie in one channel of the L2 (d of 8192 x 65536: 2.2 -> 1.9 ms)
         q.ld_delta = q.piece + 256 / q.es;
         // the pass over the kept exponentials and their stores move 6 bytes a logit, the products take 2 dim operations
-        q.keep = dtype == SSDBOX_DTYPE_BF16 && q.tile == 2 && !q.few_parts && dim > kKeepAbove;
+        q.keep = !q.few_parts && (dtype == SSDBOX_DTYPE_F32 ||
+                                 (dtype == SSDBOX_DTYPE_BF16 && q.tile == 2 && dim > kKeepAbove));
     }
     size_t at = 0;
     q.o_few = put(at, (size_t)q.few_parts * rows * q.few_ld * 4);
@@ -939,7 +1031,7 @@ void launch_tiles(const HeadCall &c, const LogitArgs &a)
 template <typename T, int WHAT>
 void launch_logits(const HeadCall &c, int tile, const LogitArgs &a)
 {
-    if constexpr (WHAT != kStatKeep) {
+    if constexpr (WHAT != kStatKeep || sizeof(T) == 4) {
         if (tile == 0) return launch_tiles<T, 128, 64, 4, 1, 2, WHAT>(c, a);
         if (tile == 1) return launch_tiles<T, 128, 128, 2, 2, 2, WHAT>(c, a);
     }
@@ -971,6 +1063,7 @@ JoinArgs join_args(const GradArgs &a)
     j.ld_part = a.ld_part;
     j.part_stride = a.part_stride;
     j.parts = a.parts;
+    j.waves = a.parts < 32 ? 1 : (a.parts < 256 ? 4 : 16);
     j.m = a.m;
     j.n = a.n;
     j.n_count = a.n_count;
@@ -997,9 +1090,9 @@ template <typename T>
 void launch_join(const HeadCall &c, const GradArgs &a, const GradArgs *b)
 {
     const JoinArgs x = join_args(a), y = b ? join_args(*b) : JoinArgs{};
-    const int parts = x.parts > y.parts ? x.parts : y.parts;
-    if (parts < 32) launch_join<T, 1>(c, x, y);
-    else if (parts < 256) launch_join<T, 4>(c, x, y);
+    const int waves = x.waves > y.waves ? x.waves : y.waves;
+    if (waves == 1) launch_join<T, 1>(c, x, y);
+    else if (waves == 4) launch_join<T, 4>(c, x, y);
     else launch_join<T, 16>(c, x, y);
 }
 
@@ -1070,7 +1163,12 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
         ldw = q.pitch;
     }
     s.prep_blocks = (int)n_prep;
-    launch_stage(ctx, SSDBOX_STAGE_LOSS, head_prep_kernel<T>, dim3(n_prep + n_pitch), dim3(kRowThreads), s);
+    s.stay = q.direct;
+    if (!q.direct || q.copy_weight || c.hidden_ld % q.vec != 0 || (uintptr_t)c.hidden % 16 != 0) {
+        launch_stage(ctx, SSDBOX_STAGE_LOSS, head_prep_kernel<T>, dim3(n_prep + n_pitch), dim3(kRowThreads), s);
+        s.hidden = rows;
+        s.ld = q.pitch;
+    }
 
     LogitArgs l = {};
     l.weight = weight;
@@ -1110,11 +1208,11 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
             GradArgs f = {};
             f.a = weight;
             f.lda = ldw;
-            f.b = rows;
-            f.ldb = q.pitch;
+            f.b = q.direct ? s.hidden : rows;
+            f.ldb = q.direct ? s.ld : q.pitch;
             f.m = f.a_extent = (int)c.classes;
             f.n = (int)c.rows;
-            f.n_count = count;
+            f.n_count = q.direct ? nullptr : count;
             f.k = q.pitch;
             f.parts = q.few_parts;
             f.scale = scale;
@@ -1123,14 +1221,14 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
             f.part_stride = c.rows * q.few_ld;
             launch_product<T, false, false>(c, q.tile, f);
             T *d = (T *)(c.ws + q.o_delta);
-            if (c.classes < 4096)
-                launch_stage(ctx, SSDBOX_STAGE_LOSS, head_few_kernel<T, 256>, dim3((unsigned)c.rows), dim3(256), r, f.part,
-                             f.ld_part, f.part_stride, f.parts, d, q.ld_delta);
-            else
-                launch_stage(ctx, SSDBOX_STAGE_LOSS, head_few_kernel<T, 1024>, dim3((unsigned)c.rows), dim3(1024), r, f.part,
-                             f.ld_part, f.part_stride, f.parts, d, q.ld_delta);
+            const auto few = [&](auto kernel, int threads) {
+                launch_stage(ctx, SSDBOX_STAGE_LOSS, kernel, dim3((unsigned)c.rows), dim3(threads), r, s, f.part, f.ld_part,
+                             f.part_stride, f.parts, d, q.ld_delta);
+            };
+            if (c.classes < 4096) few(q.direct ? head_few_kernel<T, 256, true> : head_few_kernel<T, 256, false>, 256);
+            else few(q.direct ? head_few_kernel<T, 1024, true> : head_few_kernel<T, 1024, false>, 1024);
         } else {
-            if constexpr (__is_same(T, bf16_t)) {
+            if constexpr (!__is_same(T, f16_t)) {
                 if (q.keep) {
                     l.kept_from = (int)((q.pieces - 1) * q.piece);
                     l.delta = c.ws + q.o_delta;
@@ -1168,10 +1266,11 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
             k.each = q.each;
             k.first = (int)first;
             k.classes = n_class;
-            k.delta = (unsigned *)delta;
+            k.l2 = l.l2;
+            k.delta = delta;
             k.ld_delta = q.ld_delta;
-            k.blocks = (int)((q.piece + kRowThreads * 8 - 1) / (kRowThreads * 8));
-            launch_stage(ctx, SSDBOX_STAGE_LOSS, head_kept_kernel, dim3((unsigned)(c.rows * k.blocks)), dim3(kRowThreads), k);
+            k.blocks = (int)((q.piece + kRowThreads * q.vec - 1) / (kRowThreads * q.vec));
+            launch_stage(ctx, SSDBOX_STAGE_LOSS, head_kept_kernel<T>, dim3((unsigned)(c.rows * k.blocks)), dim3(kRowThreads), k);
         } else if (c.rows > 0) {
             LogitArgs d = l;
             d.weight = weight + first * ldw;
@@ -1195,7 +1294,7 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
             h.a = weight + first * ldw;
             h.lda = ldw;
             h.n = (int)c.rows;
-            h.n_count = count;
+            h.n_count = q.direct ? nullptr : count;
             h.k = n_class;
             h.parts = q.dh_parts;
             h.out = c.grad_hidden;
@@ -1213,7 +1312,7 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
             w.lda = q.pitch;
             w.n = n_class;
             w.k = (int)c.rows;
-            w.k_count = count;
+            w.k_count = q.direct ? nullptr : count;
             w.parts = q.dw_parts;
             w.out = (T *)c.grad_weight + first * c.dim;
             if (q.dw_parts > 1) {

@@ -130,7 +130,9 @@ def test_workspace_refusals_and_sizes():
 HEAD_SIZES = [(1, 1, 1), (1, 2, 8), (3, 5, 7), (4, 1000, 128), (31, 257, 72), (32, 128, 64), (33, 129, 40), (65, 300, 33),
               (129, 255, 100), (513, 257, 136), (700, 1030, 65), (2, 30011, 16), (1500, 3, 24),
               (130, 40, 1032), (300, 1500, 1024), (257, 515, 1030), (140, 700, 264), (4, 263, 1975), (2000, 44, 1216),
-              (1, 9000, 600)]
+              (1, 9000, 600),
+              # more logits than are written: statistics of tiles of every shape, d taken again or made of what was kept
+              (40, 16500, 24), (513, 16421, 24), (540, 16600, 270), (130, 65600, 40), (1030, 9001, 33), (5000, 2003, 72)]
 
 
 @gpu
@@ -153,11 +155,11 @@ def test_head(n, v, dim, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-@pytest.mark.parametrize("n", [20, 300, 900])
-def test_head_options(n, dtype):
+@pytest.mark.parametrize("n,v", [(20, 777), (300, 777), (900, 777), (33, 20011), (530, 16390), (4500, 2002)])
+def test_head_options(n, v, dtype):
     """Scale, smoothing, rows' weights, labels of both widths, all at once."""
     import face_detection_amd as fda
-    hidden, weight, labels = head_inputs(n, 777, 48, dtype, seed=5, device="cuda", scale=4.0)
+    hidden, weight, labels = head_inputs(n, v, 48, dtype, seed=5, device="cuda", scale=4.0)
     g = torch.rand(n, device="cuda") * 3 - 1
     want, off = O.head(hidden, weight, labels, 4.0, 0.15, g)
     got = fda.linear_cross_entropy_batch(hidden, weight, labels.to(torch.int32), logit_scale=4.0, label_smoothing=0.15,
@@ -167,11 +169,12 @@ def test_head_options(n, dtype):
 
 
 @gpu
-@pytest.mark.parametrize("n", [6, 200])
-def test_head_rows_left_out(n):
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("n,v,dim", [(6, 50, 16), (200, 50, 16), (200, 50, 19), (300, 700, 600), (600, 16390, 16), (4500, 2002, 40)])
+def test_head_rows_left_out(n, v, dim, dtype):
     """Rows without a class cost nothing and spoil nothing, whatever their hidden values hold."""
     import face_detection_amd as fda
-    hidden, weight, labels = head_inputs(n, 50, 16, torch.bfloat16, seed=2, device="cuda", ignored=0.5)
+    hidden, weight, labels = head_inputs(n, v, dim, dtype, seed=2, device="cuda", ignored=0.5)
     labels[0], labels[1] = -1, 3
     clean = fda.linear_cross_entropy_batch(hidden, weight, labels, return_grad=True)
     dirty = torch.where((labels < 0)[:, None], torch.full_like(hidden, float("nan")), hidden)
@@ -181,7 +184,7 @@ def test_head_rows_left_out(n):
     assert (got[0][labels < 0] == 0).all() and (got[1][labels < 0] == 0).all()
     # a class that does not exist: no gradient, and a loss that says so
     far = labels.clone()
-    far[1] = 50
+    far[1] = v
     far[2] = 2 ** 32 + 3                                # 3 in its low 32 bits
     out = fda.linear_cross_entropy_batch(hidden, weight, far, return_grad=True)
     kept = labels.clone()
@@ -206,19 +209,20 @@ def test_head_empty_batch():
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-def test_head_sure_rows(dtype):
+@pytest.mark.parametrize("v,sure", [(40, 30), (17000, 45)])
+def test_head_sure_rows(v, sure, dtype):
     """A row whose label has nearly everything: loss and gradients keep their relative accuracy far below one unit of 1."""
     import face_detection_amd as fda
-    weight = torch.zeros(40, 8, device="cuda", dtype=dtype)
-    weight[:, 0] = torch.arange(40, device="cuda", dtype=torch.float32).div(64).to(dtype)
-    weight[7, 1] = 30
+    weight = torch.zeros(v, 8, device="cuda", dtype=dtype)
+    weight[:40, 0] = torch.arange(40, device="cuda", dtype=torch.float32).div(64).to(dtype)
+    weight[7, 1] = sure
     hidden = torch.zeros(3, 8, device="cuda", dtype=dtype)
     hidden[:, :2] = 1
     labels = torch.tensor([7, 8, 7], device="cuda")
     want, off = O.head(hidden, weight, labels)
     got = fda.linear_cross_entropy_batch(hidden, weight, labels, return_grad=True)
     assert 0 < float(want[0][0]) < 1e-10
-    assert abs(float(got[0][0]) / float(want[0][0]) - 1) < 32 * 2 ** -19   # a few units of float32 in z of about 32
+    assert abs(float(got[0][0]) / float(want[0][0]) - 1) < 32 * 2 ** -19   # a few units of float32 in z, near 32 or above
     for x, w, o, what in zip(got, want, off, ("loss", "grad_hidden", "grad_weight")):
         within(x, w, o, what)
 
@@ -244,27 +248,28 @@ def test_head_slope_of_its_own_loss():
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-def test_head_strides_and_alignment(dtype):
+@pytest.mark.parametrize("n,v", [(70, 90), (530, 16390)])
+def test_head_strides_and_alignment(n, v, dtype):
     import face_detection_amd as fda
-    hidden, weight, labels = head_inputs(70, 90, 40, dtype, seed=4, device="cuda")
+    hidden, weight, labels = head_inputs(n, v, 40, dtype, seed=4, device="cuda")
     want = fda.linear_cross_entropy_batch(hidden, weight, labels, return_grad=True)
 
     def same(h, w, lab=labels):
         got = fda.linear_cross_entropy_batch(h, w, lab, return_grad=True)
         assert all(torch.equal(a.reshape(b.shape), b) for a, b in zip(got, want))
-    wide = torch.full((70, 57), float("nan"), device="cuda", dtype=dtype)
+    wide = torch.full((n, 57), float("nan"), device="cuda", dtype=dtype)
     wide[:, 3:43] = hidden
     same(wide[:, 3:43], weight)                                    # rows further apart, off any boundary
     for pitch, first in ((64, 8), (47, 0), (43, 1)):
-        wide = torch.full((90, pitch), float("nan"), device="cuda", dtype=dtype)
+        wide = torch.full((v, pitch), float("nan"), device="cuda", dtype=dtype)
         wide[:, first:first + 40] = weight
         same(hidden, wide[:, first:first + 40])
     same(hidden.t().contiguous().t(), weight.t().contiguous().t())
-    same(hidden.reshape(7, 10, 40), weight, labels.reshape(7, 10))
-    same(hidden.reshape(7, 10, 40), weight, labels.to(torch.int16).reshape(7, 10))
-    flat = torch.empty(90 * 40 + 1, device="cuda", dtype=dtype)
+    same(hidden.reshape(-1, 10, 40), weight, labels.reshape(-1, 10))
+    same(hidden.reshape(-1, 10, 40), weight, labels.to(torch.int16).reshape(-1, 10))
+    flat = torch.empty(v * 40 + 1, device="cuda", dtype=dtype)
     flat[1:] = weight.reshape(-1)
-    same(hidden, flat[1:].view(90, 40))                            # a base off any boundary
+    same(hidden, flat[1:].view(v, 40))                            # a base off any boundary
 
 
 @gpu
