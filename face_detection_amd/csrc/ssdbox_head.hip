@@ -813,14 +813,11 @@ struct JoinArgs {
 // The parts of a product over a long k, added in a fixed order.  Four values a lane, eight parts on their way at a time;
 // WAVES waves share the parts of one piece of 256 values.
 template <typename T, int WAVES>
-__global__ __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64) void head_join_kernel(const JoinArgs a, const JoinArgs b, int a_blocks)
+SSD_DEV void join(const JoinArgs &p, int block, f32x4 (&s_sum)[WAVES > 1 ? WAVES : 1][64])
 {
-    const bool first = (int)blockIdx.x < a_blocks;
-    const JoinArgs &p = first ? a : b;
     constexpr int kPieces = WAVES < 4 ? 4 / WAVES : 1;
-    __shared__ f32x4 s_sum[WAVES > 1 ? WAVES : 1][64];
     const int across = (p.m + 255) / 256, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long id = (long long)(blockIdx.x - (first ? 0 : a_blocks)) * kPieces + (WAVES > 1 ? 0 : wave);
+    const long long id = (long long)block * kPieces + (WAVES > 1 ? 0 : wave);
     const int n = (int)(id / across), m = ((int)(id % across) * 64 + lane) * 4;
     const bool in = n < (p.n_count ? *p.n_count : p.n) && m < p.m;
     f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -852,6 +849,15 @@ __global__ __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64) void head_join_kernel
 #pragma unroll
     for (int j = 0; j < 4; ++j)
         if (m + j < p.m) o[j] = (T)(s[j] * up);
+}
+
+// One product's parts, or in one launch two products'.
+template <typename T, int WAVES>
+__global__ __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64) void head_join_kernel(const JoinArgs a, const JoinArgs b, int a_blocks)
+{
+    __shared__ f32x4 s_sum[WAVES > 1 ? WAVES : 1][64];
+    if ((int)blockIdx.x < a_blocks) join<T, WAVES>(a, blockIdx.x, s_sum);
+    else join<T, WAVES>(b, blockIdx.x - a_blocks, s_sum);
 }
 
 // -------------------------------------------------------------------------------- plan
@@ -1096,9 +1102,12 @@ void launch_join(const HeadCall &c, const GradArgs &a, const GradArgs *b)
     else launch_join<T, 16>(c, x, y);
 }
 
-// dH and dW of one piece: together where the tiles are the smaller ones, each with a launch of its own otherwise.
+// dH and dW of one piece, each if it is wanted, and their parts joined if they are whole: two launches for both where the
+// tiles are the smaller ones.  Otherwise dH's parts are joined at once, from the caches (256 x 1000003 x 512: 12 us, and 22
+// after dW has gone through them).
 template <typename T>
-void launch_gradients(const HeadCall &c, const HeadPlan &q, GradArgs h, GradArgs w, bool want_h, bool want_w)
+void launch_gradients(const HeadCall &c, const HeadPlan &q, GradArgs h, GradArgs w, bool want_h, bool want_w, bool join_h,
+                      bool join_w)
 {
     if (want_h && want_w && q.dh_tile < 2 && q.dw_tile < 2) {
         h.tm = (h.m + 127) / 128;
@@ -1109,10 +1118,14 @@ void launch_gradients(const HeadCall &c, const HeadPlan &q, GradArgs h, GradArgs
             launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_both_kernel<T, 64, 4, 1>, dim3(hb + wb), dim3(256), h, w, (int)hb);
         else
             launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_both_kernel<T, 128, 2, 2>, dim3(hb + wb), dim3(256), h, w, (int)hb);
+        if (join_h) launch_join<T>(c, h, join_w ? &w : nullptr);
+        else if (join_w) launch_join<T>(c, w, nullptr);
         return;
     }
     if (want_h) launch_product<T, true, false>(c, q.dh_tile, h);
+    if (join_h) launch_join<T>(c, h, nullptr);
     if (want_w) launch_product<T, true, true>(c, q.dw_tile, w);
+    if (join_w) launch_join<T>(c, w, nullptr);
 }
 
 template <typename T>
@@ -1322,9 +1335,7 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
                 join_w = true;
             }
         }
-        launch_gradients<T>(c, q, h, w, want_h, c.grad_weight != nullptr);
-        if (join_h) launch_join<T>(c, h, join_w ? &w : nullptr);
-        else if (join_w) launch_join<T>(c, w, nullptr);
+        launch_gradients<T>(c, q, h, w, want_h, c.grad_weight != nullptr, join_h, join_w);
     }
     return SSDBOX_OK;
 }
