@@ -8,9 +8,9 @@
 //
 // A row is read once, stays in registers for its maximum, its sum and its gradient, and is written once: 2 * V values a row
 // is all the HBM traffic there is, which bounds the kernel.  Rows of up to 64 classes: a few lanes a row, each with its
-// values in registers; up to 256 pieces of 16 bytes: a wave a row; longer: a workgroup a row.  Rows longer than the
-// registers of a workgroup, and too few rows for the chip, are cut into segments with a launch for the sums before the
-// one that writes.
+// values in registers; up to 128 pieces of 16 bytes with few entries: sixteen lanes a row; up to 256 pieces: a wave a row;
+// longer: a workgroup a row.  Rows longer than the registers of a workgroup are cut into segments with a launch for the sums
+// before the one that writes.
 //
 // The outside bucket keeps a maximum and a sum of its own (mo, so), so that p_r and its logarithm hold where the top classes
 // have everything.  Per-row sums are joined in float64 and logarithms taken of mantissa and exponent apart: the loss is a
@@ -157,6 +157,22 @@ SSD_DEV double wave_sum(double x)
     return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
 }
 
+// Within sixteen lanes, by rotations: all of them get the same bits, as both sides of every addition are the same two.
+SSD_DEV float row_max(float x)
+{
+    x = fmaxf(x, dpp<0x128, 0xf>(x, x));
+    x = fmaxf(x, dpp<0x124, 0xf>(x, x));
+    x = fmaxf(x, dpp<0x122, 0xf>(x, x));
+    return fmaxf(x, dpp<0x121, 0xf>(x, x));
+}
+SSD_DEV double row_sum(double x)
+{
+    x += dpp<0x128, 0xf>(x);
+    x += dpp<0x124, 0xf>(x);
+    x += dpp<0x122, 0xf>(x);
+    return x + dpp<0x121, 0xf>(x);
+}
+
 // The waves' values, one in each lane of every eight (or four), joined in all of them.
 template <int WAVES>
 SSD_DEV float waves_max(float x)
@@ -178,11 +194,11 @@ SSD_DEV double waves_sum(double x)
     return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
 }
 
-// THREADS lanes (whole waves) that work on one row.  Each reduction of a row has a place of its own in LDS, so that one
+// THREADS lanes (sixteen, or whole waves) that work on one row.  Each reduction of a row has a place of its own in LDS, so that one
 // barrier each is enough.
 template <int THREADS>
 struct Team {
-    static constexpr int kWaves = THREADS / 64;    // 1, 4 or 8
+    static constexpr int kWaves = THREADS < 64 ? 1 : THREADS / 64;    // 1, 4 or 8
     static constexpr int kPlace = kWaves * 4;      // float64 of one reduction
     double *lds;
 
@@ -195,7 +211,7 @@ struct Team {
     SSD_DEV void maxima(int place, float (&x)[N]) const
     {
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = wave_max(x[i]);
+        for (int i = 0; i < N; ++i) x[i] = THREADS == 16 ? row_max(x[i]) : wave_max(x[i]);
         if constexpr (THREADS > 64) {
             float *p = (float *)(lds + place * kPlace);
             if ((threadIdx.x & 63) == 0)
@@ -210,7 +226,7 @@ struct Team {
     SSD_DEV void sums(int place, double (&x)[N]) const
     {
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = wave_sum(x[i]);
+        for (int i = 0; i < N; ++i) x[i] = THREADS == 16 ? row_sum(x[i]) : wave_sum(x[i]);
         if constexpr (THREADS > 64) {
             double *p = lds + place * kPlace;
             if ((threadIdx.x & 63) == 0)
@@ -360,6 +376,10 @@ struct RowPieces {
     }
 };
 
+// Entries of a lane in registers: 64 entries of sixteen lanes, 256 of the larger teams.
+template <int TEAM>
+constexpr int kEntries = TEAM <= 64 ? 4 : 1;
+
 template <typename T, int TEAM, int R>
 __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void distill_row_kernel(const DistArgs p)
 {
@@ -371,10 +391,10 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void distill_row_kernel(co
     __shared__ unsigned s_bits[kRows * kWords];
     __shared__ double s_red[4 * Team<TEAM>::kPlace];
     const int t = threadIdx.x % TEAM;
-    const int mine = TEAM < 256 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TEAM) : 0;
+    const int mine = TEAM == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TEAM) : TEAM < 64 ? threadIdx.x / TEAM : 0;
     long long row = p.row0 + (long long)blockIdx.x * kRows + mine;
     const long long end = p.row0 + p.row_count, step = (long long)gridDim.x * kRows;
-    if (row >= end) return;                               // whole waves: a team is a wave or the workgroup
+    if (row >= end) return;                               // whole teams, of which only those of several waves have barriers
     unsigned *bits = s_bits + mine * kWords;
     const Team<TEAM> team = {s_red};
     const bool tail = p.teacher_lse != nullptr;
@@ -385,9 +405,17 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void distill_row_kernel(co
     v.more = p.classes - v.whole * N;
     const T *z = (const T *)p.logits + row * p.ld;
 
-    // a lane's first entry stays in registers; further ones (more than TEAM) are read again each time
-    Entry e0 = {-1, -INFINITY};
-    if (t < p.top) e0 = entry_of(p, row, t);
+    // a lane's first entries stay in registers; further ones are read again each time
+    constexpr int E = kEntries<TEAM>;
+    Entry e0[E];
+    const auto take = [&](Entry (&e)[E], long long of, bool any) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            e[j] = Entry{-1, -INFINITY};
+            if (any && t + j * TEAM < p.top) e[j] = entry_of(p, of, t + j * TEAM);
+        }
+    };
+    take(e0, row, true);
 #pragma unroll
     for (int r = 0; r < R; ++r) v.load(r, z, v.whole);
     v.load_rest(z);
@@ -397,26 +425,34 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void distill_row_kernel(co
     f.l2 = (float)(kLog2eD / (double)p.tau);
 
     for (;;) {
-        const float z0 = e0.at >= 0 ? (float)z[e0.at] : -INFINITY;
-        const auto entry = [&](int k) { return k == t ? e0 : entry_of(p, row, k); };
-        const auto logit = [&](int k, const Entry &e) { return k == t ? z0 : (float)z[e.at]; };
+        float z0[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j) z0[j] = e0[j].at >= 0 ? (float)z[e0[j].at] : -INFINITY;
+        // f(place among the registers' or E, k, entry, its logit) for each of the lane's entries
+        const auto entries_of = [&](auto f) {
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+                if (e0[j].at >= 0) f(j, t + j * TEAM, e0[j], z0[j]);
+            for (int k = t + E * TEAM; k < p.top; k += TEAM) {
+                const Entry e = entry_of(p, row, k);
+                if (e.at >= 0) f(E, k, e, (float)z[e.at]);
+            }
+        };
         float top[2] = {-INFINITY, -INFINITY};             // of the entries' logits, of the teacher's
         int entries = 0, inside = 0;
-        bool first0 = false;
-        for (int k = t; k < p.top; k += TEAM) {
-            const Entry e = entry(k);
-            if (e.at < 0) continue;
-            top[0] = fmaxf(top[0], logit(k, e));
+        unsigned first0 = 0u;
+        entries_of([&](int j, int, const Entry &e, float ze) {
+            top[0] = fmaxf(top[0], ze);
             top[1] = fmaxf(top[1], e.t);
             const unsigned bit = 1u << (e.at & 31);
             ++entries;
             if (!(atomicOr(&bits[e.at >> 5], bit) & bit)) {
                 ++inside;
-                if (k == t) first0 = true;
+                first0 |= 1u << j;
             }
-        }
+        });
         team.template maxima<2>(0, top);                   // its barrier shows the bits as well
-        if constexpr (TEAM == 64) Team<TEAM>::sync();
+        if constexpr (TEAM <= 64) Team<TEAM>::sync();
         f.sub = 0.0f;
         f.off = top[0] == -INFINITY ? 0.0f : fmaxf(top[0] * f.l2, -3e38f);
         const float off = f.off;
@@ -442,12 +478,13 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void distill_row_kernel(co
             so += __builtin_amdgcn_exp2f(__builtin_fmaf(v.rest, f.l2, -off));
         double sum[4] = {(double)so, 0.0, (double)inside + 65536.0 * (double)entries, 0.0};
         if (tail) {
-            if (first0) sum[3] = (double)f.power(z0);
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+                if (first0 >> j & 1u) sum[3] += (double)f.power(z0[j]);
         } else {
-            for (int k = t; k < p.top; k += TEAM) {
-                const Entry e = entry(k);
-                if (e.at >= 0) sum[1] += (double)__builtin_amdgcn_exp2f((e.t - top[1]) * f.l2);
-            }
+            entries_of([&](int, int, const Entry &e, float) {
+                sum[1] += (double)__builtin_amdgcn_exp2f((e.t - top[1]) * f.l2);
+            });
         }
         team.template sums<4>(1, sum);
         const int n_entries = (int)(sum[2] / 65536.0), n_inside = (int)(sum[2] - 65536.0 * n_entries);
@@ -471,26 +508,22 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void distill_row_kernel(co
             team.template sums<1>(3, again);
             sum[0] = again[0];
         }
-        for (int k = t; k < p.top; k += TEAM) {            // the bits are clear again for the next row
-            const Entry e = entry(k);
-            if (e.at >= 0) bits[e.at >> 5] = 0u;
-        }
+        if constexpr (kLoop) entries_of([&](int, int, const Entry &e, float) { bits[e.at >> 5] = 0u; });    // for the next row
         const long long next = row + step;
         const bool goes_on = kLoop && next < end;
         const T *zn = goes_on ? z + step * p.ld : z;
         const int limit = goes_on ? v.whole : 0;
-        Entry en = {-1, -INFINITY};
-        if (goes_on && t < p.top) en = entry_of(p, next, t);
+        Entry en[E];
+        take(en, next, goes_on);
 
         double s = sum[0];
         if (tail) {
             double in[1] = {sum[3]};
-            if (slow || dup || p.top > TEAM) {
+            if (slow || dup || p.top > E * TEAM) {
                 in[0] = 0.0;
-                for (int k = t; k < p.top; k += TEAM) {
-                    const Entry e = entry(k);
-                    if (e.at >= 0 && first_of(p, row, k, e, dup)) in[0] += (double)f.power(logit(k, e));
-                }
+                entries_of([&](int, int k, const Entry &e, float ze) {
+                    if (first_of(p, row, k, e, dup)) in[0] += (double)f.power(ze);
+                });
                 team.template sums<1>(0, in);
             }
             s = in[0] + s * (double)__builtin_amdgcn_exp2f((osub - f.sub) * f.l2);
@@ -499,10 +532,7 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void distill_row_kernel(co
         f.ln_s = ln_of(s);
         terms_teacher(f, p, row, top[1], sum[1]);
         double of_entries[3] = {0.0, 0.0, 0.0};
-        for (int k = t; k < p.top; k += TEAM) {
-            const Entry e = entry(k);
-            if (e.at >= 0) add_entry(of_entries, f, p, row, k, e, logit(k, e), dup);
-        }
+        entries_of([&](int, int k, const Entry &e, float ze) { add_entry(of_entries, f, p, row, k, e, ze, dup); });
         team.template sums<3>(2, of_entries);
         const double loss = terms_finish(f, p, row, of_entries[0], of_entries[1], of_entries[2], osub, sum[0], outside);
         if (t == 0) p.loss[row] = n_inside > 0 ? (float)loss : 0.0f;      // a row without an entry teaches nothing
@@ -534,17 +564,16 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void distill_row_kernel(co
         if constexpr (kLoop) v.load_rest(zn);
         if (p.grad) {
             Team<TEAM>::sync();                            // the entries' own values come last
-            for (int k = t; k < p.top; k += TEAM) {
-                const Entry e = entry(k);
-                if (e.at < 0) continue;
+            entries_of([&](int, int, const Entry &e, float ze) {
                 const double q = teacher_of(f, p, row, e, dup);
-                g[e.at] = (T)(float)((double)f.c * ((double)f.share(logit(k, e)) * f.whole - q));
-            }
+                g[e.at] = (T)(float)((double)f.c * ((double)f.share(ze) * f.whole - q));
+            });
         }
         if (!goes_on) return;
         row = next;
         z = zn;
-        e0 = en;
+#pragma unroll
+        for (int j = 0; j < E; ++j) e0[j] = en[j];
     }
 }
 
@@ -896,6 +925,14 @@ void launch_distill(ssdbox_ctx *ctx, const DistArgs &a, const DistPlan &q, int r
     else if (a.classes <= 16) launch_small<T, 4>(ctx, a, rows);
     else if (a.classes <= 32) launch_small<T, 8>(ctx, a, rows);
     else if (a.classes <= 64) launch_small<T, 16>(ctx, a, rows);
+    // short rows: sixteen lanes a row rather than a wave, as long as the registers hold the entries (rows x classes x K, us:
+    // 113154 x 164 x 8 float32 39, a wave 113;  35660 x 74 x 15 float32 18, 40;  50000 x 400 x 64 float32 44, 66;
+    // 20000 x 1000 x 16 bfloat16 20, 31; past the registers' entries 20000 x 500 x 200 float32 133, 37)
+    else if (pieces <= 128 && a.top <= 16 * kEntries<16>) {
+        if (pieces <= 32) launch_row<T, 16, 2>(ctx, a, rows);
+        else if (pieces <= 64) launch_row<T, 16, 4>(ctx, a, rows);
+        else launch_row<T, 16, 8>(ctx, a, rows);
+    }
     else if (pieces <= 64) launch_row<T, 64, 1>(ctx, a, rows);
     else if (pieces <= 128) launch_row<T, 64, 2>(ctx, a, rows);
     else if (pieces <= 256) launch_row<T, 64, 4>(ctx, a, rows);

@@ -349,7 +349,9 @@ def test_head_refusals():
 # --------------------------------------------------------------------------------------------------- distil on the GPU
 DISTIL_SIZES = [(1, 1, 1), (5, 2, 1), (9, 2, 2), (7, 3, 2), (300, 4, 3), (17, 8, 4), (33, 13, 5), (65, 31, 31), (5, 64, 8),
                 (6, 65, 9), (3, 511, 16), (4, 515, 40), (130, 1025, 7), (3, 2048, 64), (130, 4099, 64), (200, 5000, 100),
-                (129, 9001, 17), (2, 4100, 33), (2, 33000, 256), (1, 100003, 16), (131, 20001, 50)]
+                (129, 9001, 17), (2, 4100, 33), (2, 33000, 256), (1, 100003, 16), (131, 20001, 50),
+                # sixteen lanes a row, and a wave where there are more entries
+                (70, 200, 64), (37, 90, 65), (21, 129, 1), (35, 1000, 16), (18, 300, 300), (9, 1024, 64)]
 
 
 @gpu
@@ -373,7 +375,7 @@ def test_distill(n, v, k, tail, dtype):
 
 @gpu
 @pytest.mark.parametrize("tail", [False, True])
-@pytest.mark.parametrize("v", [6, 50, 300, 3000, 40000])
+@pytest.mark.parametrize("v", [6, 50, 300, 1000, 3000, 40000])
 def test_distill_padding_and_twice(v, tail):
     """Padding by index and by value, a class given twice and three times, rows with one entry and with none."""
     import face_detection_amd as fda
@@ -399,7 +401,7 @@ def test_distill_padding_and_twice(v, tail):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-@pytest.mark.parametrize("v", [5, 60, 700, 3001, 30000])
+@pytest.mark.parametrize("v", [5, 60, 200, 700, 3001, 30000])
 def test_distill_masked_classes(v, dtype):
     """Classes the student masks, by -inf and by the type's lowest value, and students that are sure beyond float32."""
     import face_detection_amd as fda
