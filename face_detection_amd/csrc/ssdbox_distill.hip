@@ -342,6 +342,8 @@ SSD_DEV double terms_finish(RowTerms &r, const DistArgs &p, long long row, doubl
 //
 // The registers are only ever loaded and read: a piece that holds one of the teacher's classes is summed without them where
 // they are not part of the outside bucket, and their gradients are written after the others'.
+constexpr int kRegMost = 50;          // pieces a lane that the registers of a workgroup of 512 hold
+
 template <typename T, int TEAM, int R>
 struct RowPieces {
     static constexpr int N = 16 / (int)sizeof(T);
@@ -360,10 +362,11 @@ struct RowPieces {
         for (int j = 0; j < 4; ++j) x[r].w[j] = q.w[j];
     }
     SSD_DEV void load_rest(const T *z) { rest = t < more ? (float)z[whole * N + t] : -INFINITY; }
-    SSD_DEV float value(int r, int i) const
+    SSD_DEV float value(int r, int i) const { return value(x[r].w, i); }
+    static SSD_DEV float value(const unsigned (&of)[4], int i)
     {
-        if constexpr (sizeof(T) == 4) return u2f(x[r].w[i]);
-        const unsigned w = x[r].w[i >> 1];
+        if constexpr (sizeof(T) == 4) return u2f(of[i]);
+        const unsigned w = of[i >> 1];
         if constexpr (__is_same(T, bf16_t)) return u2f(i & 1 ? w & 0xFFFF0000u : w << 16);
         return (float)__builtin_bit_cast(f16_t, (unsigned short)(i & 1 ? w >> 16 : w & 0xFFFFu));
     }
@@ -387,7 +390,8 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void distill_row_kernel(co
     constexpr int N = V::N;
     constexpr int kBlockThreads = TEAM < 256 ? 256 : TEAM;
     constexpr int kRows = kBlockThreads / TEAM;
-    constexpr int kWords = (TEAM * R + 1) * N / 32 + 1;
+    constexpr bool kBeyond = R == kRegMost;               // rows longer than the registers as well
+    constexpr int kWords = (TEAM * R * (kBeyond ? 2 : 1) + 1) * N / 32 + 1;
     __shared__ unsigned s_bits[kRows * kWords];
     __shared__ double s_red[4 * Team<TEAM>::kPlace];
     const int t = threadIdx.x % TEAM;
@@ -473,10 +477,22 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void distill_row_kernel(co
                 for (int j = 0; j < N; ++j) so += e[j];
             }
         }
+        float beyond = 0.0f;
+        if constexpr (kBeyond)
+#pragma unroll 2
+            for (int i = TEAM * R + t; i < v.whole; i += TEAM) {
+                const typename V::Raw q = *(const typename V::Raw *)((const char *)z + (unsigned)i * 16u);
+                const unsigned in = tail ? bits[i * N >> 5] >> (i * N & 31) & ((1u << N) - 1u) : 0u;
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(V::value(q.w, j), f.l2, -off));
+                    beyond += in >> j & 1u ? 0.0f : e;
+                }
+            }
         const int last = v.whole * N + t;
         if (t < v.more && !(tail && (bits[last >> 5] >> (last & 31) & 1u)))
             so += __builtin_amdgcn_exp2f(__builtin_fmaf(v.rest, f.l2, -off));
-        double sum[4] = {(double)so, 0.0, (double)inside + 65536.0 * (double)entries, 0.0};
+        double sum[4] = {(double)so + (double)beyond, 0.0, (double)inside + 65536.0 * (double)entries, 0.0};
         if (tail) {
 #pragma unroll
             for (int j = 0; j < E; ++j)
@@ -551,6 +567,16 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void distill_row_kernel(co
                 }
                 if constexpr (kLoop) v.load(r, zn, limit);
             }
+            if constexpr (kBeyond)
+#pragma unroll 2
+                for (int i = TEAM * R + t; i < v.whole; i += TEAM) {
+                    const typename V::Raw q = *(const typename V::Raw *)((const char *)z + (unsigned)i * 16u);
+                    Piece<T> o;
+#pragma unroll
+                    for (int j = 0; j < N; ++j)
+                        o.v[j] = (T)(__builtin_amdgcn_exp2f(__builtin_fmaf(V::value(q.w, j), f.l2, -off)) * f.out);
+                    o.store((T *)((char *)g + (unsigned)i * 16u), N);
+                }
             if (t < v.more)
                 g[v.whole * N + t] = (T)(__builtin_amdgcn_exp2f(__builtin_fmaf(v.rest, f.l2, -off)) * f.out);
         } else {
@@ -880,7 +906,11 @@ DistPlan dist_plan(long long rows, long long classes)
     constexpr int N = 16 / (int)sizeof(T);
     const long long pieces = (classes + N - 1) / N;
     DistPlan q = {};
-    q.cut = pieces > 512 * 50;
+    // Rows longer than a workgroup's registers: what does not fit is read twice, until that is half of the row; cut rows are
+    // read twice whole (once without a gradient), but by more workgroups.  Measured (rows x classes, cut, not): 2832 x 117899
+    // float32 924 587 us, its value alone 236 303, 1000 x 262144 bfloat16 505 274, 4000 x 262144 its value alone 665 519,
+    // 100 x 117899 float32 50 33, 64 x 204000 float32 52 55, 16 x 250000 bfloat16 25 35.
+    q.cut = pieces > 512 * kRegMost * (rows < 64 ? 1 : 2);
     if (q.cut) {
         long long segs = (pieces + kSegMost - 1) / kSegMost;
         while (segs * rows < 512 && pieces / (segs * 2) >= kSegThreads) segs *= 2;
@@ -942,7 +972,7 @@ void launch_distill(ssdbox_ctx *ctx, const DistArgs &a, const DistPlan &q, int r
     else if (pieces <= 4096) launch_row<T, 512, 8>(ctx, a, rows);
     else if (pieces <= 8192) launch_row<T, 512, 16>(ctx, a, rows);
     else if (pieces <= 16384) launch_row<T, 512, 32>(ctx, a, rows);
-    else launch_row<T, 512, 50>(ctx, a, rows);
+    else launch_row<T, 512, kRegMost>(ctx, a, rows);
 }
 
 template <typename T>

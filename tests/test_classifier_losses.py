@@ -351,7 +351,9 @@ DISTIL_SIZES = [(1, 1, 1), (5, 2, 1), (9, 2, 2), (7, 3, 2), (300, 4, 3), (17, 8,
                 (6, 65, 9), (3, 511, 16), (4, 515, 40), (130, 1025, 7), (3, 2048, 64), (130, 4099, 64), (200, 5000, 100),
                 (129, 9001, 17), (2, 4100, 33), (2, 33000, 256), (1, 100003, 16), (131, 20001, 50),
                 # sixteen lanes a row, and a wave where there are more entries
-                (70, 200, 64), (37, 90, 65), (21, 129, 1), (35, 1000, 16), (18, 300, 300), (9, 1024, 64)]
+                (70, 200, 64), (37, 90, 65), (21, 129, 1), (35, 1000, 16), (18, 300, 300), (9, 1024, 64),
+                # rows longer than the registers, and of those longer than twice the registers
+                (65, 102401, 9), (66, 120003, 20), (64, 205001, 3), (3, 204801, 70)]
 
 
 @gpu
@@ -375,11 +377,11 @@ def test_distill(n, v, k, tail, dtype):
 
 @gpu
 @pytest.mark.parametrize("tail", [False, True])
-@pytest.mark.parametrize("v", [6, 50, 300, 1000, 3000, 40000])
-def test_distill_padding_and_twice(v, tail):
+@pytest.mark.parametrize("n,v", [(8, 6), (8, 50), (8, 300), (8, 1000), (8, 3000), (8, 40000), (8, 103000), (70, 103000)])
+def test_distill_padding_and_twice(n, v, tail):
     """Padding by index and by value, a class given twice and three times, rows with one entry and with none."""
     import face_detection_amd as fda
-    n, k, tau = 8, 5, 2.0
+    k, tau = 5, 2.0
     z, values, index, lse = distill_inputs(n, v, k, torch.float32, seed=1, device="cuda", tau=tau, tail=tail)
     if tail:
         lse = lse + 1.5                                 # room for what is given twice
@@ -401,11 +403,11 @@ def test_distill_padding_and_twice(v, tail):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-@pytest.mark.parametrize("v", [5, 60, 200, 700, 3001, 30000])
-def test_distill_masked_classes(v, dtype):
+@pytest.mark.parametrize("n,v", [(6, 5), (6, 60), (6, 200), (6, 700), (6, 3001), (6, 30000), (64, 103001)])
+def test_distill_masked_classes(n, v, dtype):
     """Classes the student masks, by -inf and by the type's lowest value, and students that are sure beyond float32."""
     import face_detection_amd as fda
-    n, k = 6, 2
+    k = 2
     z, values, index, lse = distill_inputs(n, v, k, dtype, seed=3, device="cuda", tail=True)
     keep = torch.zeros(n, v, dtype=torch.bool, device="cuda").scatter_(1, index, True)
     keep[:, 0] = keep[:, v - 1] = True
