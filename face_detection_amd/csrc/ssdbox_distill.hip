@@ -8,7 +8,7 @@
 //
 // A row is read once, stays in registers for its maximum, its sum and its gradient, and is written once: 2 * V values a row
 // is all the HBM traffic there is, which bounds the kernel.  Rows of up to 64 classes: a few lanes a row, each with its
-// values in registers; up to 128 pieces of 16 bytes with few entries: sixteen lanes a row; up to 256 pieces: a wave a row;
+// values in registers; up to 128 pieces of 16 bytes with few entries: sixteen lanes a row; up to 1024 pieces: a wave a row;
 // longer: a workgroup a row.  Rows longer than the registers of a workgroup are cut into segments with a launch for the sums
 // before the one that writes.
 //
@@ -402,7 +402,7 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void distill_row_kernel(co
     unsigned *bits = s_bits + mine * kWords;
     const Team<TEAM> team = {s_red};
     const bool tail = p.teacher_lse != nullptr;
-    constexpr bool kLoop = R == 32;
+    constexpr bool kLoop = TEAM == 512 && R == 32;
     V v;
     v.t = t;
     v.whole = p.classes / N;
@@ -926,7 +926,8 @@ template <typename T, int TEAM, int R>
 void launch_row(ssdbox_ctx *ctx, const DistArgs &a, int rows)
 {
     constexpr int kThreads = TEAM < 256 ? 256 : TEAM;
-    // as many workgroups as the registers let run at once: each goes on to its next row with the loads in flight
+    // rows that fill half the registers: as many workgroups as run at once, each going on to its next row with its loads in
+    // flight (shorter ones do without: 1021 x 50021 float16 46 us, 62 that way)
     constexpr int kEach = TEAM == 512 ? (R <= 8 ? 2 : 1) : 4;
     const int most = R == 32 ? ctx->num_cus * kEach : rows, need = (rows + kThreads / TEAM - 1) / (kThreads / TEAM);
     const unsigned grid = (unsigned)(need < most ? need : most);
@@ -963,11 +964,15 @@ void launch_distill(ssdbox_ctx *ctx, const DistArgs &a, const DistPlan &q, int r
         else if (pieces <= 64) launch_row<T, 16, 4>(ctx, a, rows);
         else launch_row<T, 16, 8>(ctx, a, rows);
     }
+    // (479494 x 728 x 2 float32 485, a wave 620, its value alone 266, 475;  50000 x 1000 x 60 float32 111, 88)
+    else if (pieces <= 256 && a.top <= 16) launch_row<T, 16, 16>(ctx, a, rows);
     else if (pieces <= 64) launch_row<T, 64, 1>(ctx, a, rows);
     else if (pieces <= 128) launch_row<T, 64, 2>(ctx, a, rows);
     else if (pieces <= 256) launch_row<T, 64, 4>(ctx, a, rows);
-    else if (pieces <= 512) launch_row<T, 256, 2>(ctx, a, rows);
-    else if (pieces <= 1024) launch_row<T, 256, 4>(ctx, a, rows);
+    // (a workgroup of 256 a row instead: 143928 x 2754 x 14 bfloat16 432 us, 852;  30000 x 8000 x 32 196, 224, its value alone
+    // 84, 149;  100 x 2754 x 14 18.0, 17.2;  50000 x 4000 x 14 float32 315, 300)
+    else if (pieces <= 512) launch_row<T, 64, 8>(ctx, a, rows);
+    else if (pieces <= 1024) launch_row<T, 64, 16>(ctx, a, rows);
     else if (pieces <= 2048) launch_row<T, 256, 8>(ctx, a, rows);
     else if (pieces <= 4096) launch_row<T, 512, 8>(ctx, a, rows);
     else if (pieces <= 8192) launch_row<T, 512, 16>(ctx, a, rows);
