@@ -10,9 +10,11 @@
 //   2  per row: log-sum-exp, loss, and what the gradient needs (four floats a row)
 //   3  per piece of the classes: the logits again, turned into d in the epilogue and written in the operands' type;
 //      dH += d W_piece, dW_piece = d^T H.
-// Recomputing the logits is 2 of the gradient's 8 rows * classes * dim operations.  The last piece need not be: its place is
-// free while step 1 runs, so its exponentials wait there in 16 bits, relative to their tile's maximum, for a pass that turns
-// them into d (bfloat16 alone: float16's 11 bits round them finer than d's 8, and where d has 11 too it would be rounded twice).
+// Recomputing the logits is 2 of the gradient's 8 rows * classes * dim operations.  The last piece need not be: while step 1
+// runs, what d can be made of waits for a pass that turns it into d.  float32: the products, in d's own place.  bfloat16: the
+// exponentials in 16 bits, relative to their tile's maximum, there too (float16's 11 bits round them finer than d's 8).
+// float16, whose d has 11 bits too and would be rounded twice: the products, in a place of their own.
+// Few logits are written as products, too, and a row of them goes through statistics and d in one launch.
 //
 // The label's own class stays out of the sum of exponentials: with S = sum over the others of exp(z_v - M), a sure row's
 // nll is log1p(S exp(M - z_l)) and p_l - 1 is expm1(-nll), both without the cancellation that 1 - p_l has.
@@ -270,9 +272,13 @@ struct LogitArgs {
     int kept_from;
 };
 
-// What a tile of logits leaves: statistics, d, or statistics and what d can be made of later (of 16-bit types exponentials
-// times 2^15 as float16, of float32 the products themselves)
+// What a tile of logits leaves: statistics, d, or statistics and what d can be made of later.
 enum { kStat = 0, kDelta = 1, kStatKeep = 2 };
+
+// That is for bfloat16 exponentials times 2^15 as float16, otherwise the products as float32; for float32 and bfloat16 it lies
+// where d will.
+template <typename T>
+using Kept = typename std::conditional<__is_same(T, bf16_t), f16_t, float>::type;
 
 // Sixteen neighbouring values of one row of the result, half of them in the lane 32 further: lo at m + 4 h .. + 3 and hi
 // at m + 8 + 4 h .. + 3 (h = lane / 32).  16-bit types trade halves, so that each lane stores 16 bytes (from any value's
@@ -388,15 +394,14 @@ __global__ __launch_bounds__(WM * WN * 64, BLOCKS * WM * WN / 4) void head_logit
                 // times 2^15, for what is kept in float16; the loss is to the bit the same whether something is kept or not
                 const float ref = (mx == -INFINITY ? 0.0f : m) - 15.0f;
                 const bool keep = WHAT == kStatKeep && u.m0 >= p.kept_from;
-                typedef typename std::conditional<sizeof(T) == 4, float, f16_t>::type Kept;
-                Kept *kept_row = (Kept *)p.delta + (long long)n * p.ld_delta - p.kept_from;
+                Kept<T> *kept_row = (Kept<T> *)p.delta + (long long)n * p.ld_delta - p.kept_from;
 #pragma unroll
                 for (int mi = 0; mi < S::MF; ++mi)
 #pragma unroll
                     for (int e = 0; e < 16; e += 8) {
                         float x[2][4];
                         const int at8 = u.m0 + em + mi * 32 + e * 2;
-                        if constexpr (WHAT == kStatKeep && sizeof(T) == 4) {
+                        if constexpr (WHAT == kStatKeep && __is_same(Kept<T>, float)) {
 #pragma unroll
                             for (int i = 0; i < 8; ++i) x[i >> 2][i & 3] = acc[mi][nj][e + i];
                             if (keep) store_pair<float>(kept_row, at8, x[0], x[1], 16, in);
@@ -415,7 +420,7 @@ __global__ __launch_bounds__(WM * WN * 64, BLOCKS * WM * WN / 4) void head_logit
                                 if (v != lab) s += x[i >> 2][i & 3];
                             }
                         }
-                        if constexpr (WHAT == kStatKeep && sizeof(T) == 2)
+                        if constexpr (WHAT == kStatKeep && !__is_same(Kept<T>, float))
                             if (keep) store_pair<f16_t>(kept_row, at8, x[0], x[1], 16, in);
                     }
                 s *= 0x1p-15f;
@@ -665,29 +670,32 @@ struct KeptArgs {
     long long slots;
     int each, first, classes;         // classes a slot; the piece's first class and how many
     float l2;
+    const void *kept;                 // kept and delta may be one
+    long long ld_kept;
     void *delta;
-    long long ld_delta;
+    long long ld_delta, piece;
     int blocks;                       // workgroups a row
 };
 
-// What was kept to d, in place, 16 bytes a lane.  bfloat16, of exponentials: 2^(a L - m_tile + 15) * 2^(m_tile - 15 - m) * c / Z
-// - c eps / V.  float32, of products: as the logits' epilogue does it.
+// What was kept to d, 16 bytes of d a lane.  Of exponentials: 2^(a L - m_tile + 15) * 2^(m_tile - 15 - m) * c / Z - c eps / V.
+// Of products: as the logits' epilogue does it.
 template <typename T>
 __global__ __launch_bounds__(kRowThreads) void head_kept_kernel(const KeptArgs p)
 {
     constexpr int kVec = 16 / (int)sizeof(T);
-    typedef typename std::conditional<sizeof(T) == 4, float, f16_t>::type Kept;
     const int n = blockIdx.x / p.blocks;
     if (n >= *p.count) return;
     const int v = ((int)(blockIdx.x % p.blocks) * kRowThreads + (int)threadIdx.x) * kVec;
-    if (v >= p.ld_delta - kVec) return;
+    if (v >= p.piece) return;
     const HeadRow r = p.row[n];
-    u32x4 *at = (u32x4 *)((T *)p.delta + n * p.ld_delta + v);
-    union { u32x4 w; Kept e[kVec]; } x;
+    constexpr int kWords = kVec * (int)sizeof(Kept<T>) / 16;
+    union { u32x4 w[kWords]; Kept<T> e[kVec]; } x;
     union { u32x4 w; T d[kVec]; } o;
-    x.w = *at;
+    const u32x4 *from = (const u32x4 *)((const Kept<T> *)p.kept + n * p.ld_kept + v);
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) x.w[i] = from[i];
     float f = 0.0f;
-    if constexpr (sizeof(T) == 2) {
+    if constexpr (!__is_same(Kept<T>, float)) {
         const long long slot = (p.first + v) / p.each;
         const float m = slot < p.slots ? p.stat[n * p.slots + slot].x : -INFINITY;
         f = __builtin_amdgcn_exp2f(m - 15.0f - r.m) * r.pz;
@@ -696,12 +704,14 @@ __global__ __launch_bounds__(kRowThreads) void head_kept_kernel(const KeptArgs p
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
         float d;
-        if constexpr (sizeof(T) == 2) d = __builtin_fmaf((float)x.e[i], f, -r.smooth);
-        else d = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(x.e[i], p.l2, -r.m)), r.pz, -r.smooth);
+        if constexpr (__is_same(Kept<T>, float))
+            d = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(x.e[i], p.l2, -r.m)), r.pz, -r.smooth);
+        else
+            d = __builtin_fmaf((float)x.e[i], f, -r.smooth);
         if (v + i == lab) d = r.label;
         o.d[i] = (T)(v + i < p.classes ? d : 0.0f);
     }
-    *at = o.w;
+    *(u32x4 *)((T *)p.delta + n * p.ld_delta + v) = o.w;
 }
 
 // ----------------------------------------------------------------------- gradient products
@@ -884,14 +894,17 @@ struct HeadPlan {
     long long piece, ld_delta;        // classes a piece, and from one row of its d to the next
     int pieces;
     int dh_parts, dw_parts;
-    size_t o_few, o_blocks, o_rows, o_weight, o_row, o_label, o_count, o_scale, o_stat, o_sumz, o_zl, o_out, o_delta, o_dh, o_dw;
+    size_t o_few, o_blocks, o_rows, o_weight, o_row, o_label, o_count, o_scale, o_stat, o_sumz, o_zl, o_out, o_delta, o_kept, o_dh,
+        o_dw;
     size_t bytes;
 };
 
 constexpr size_t kDeltaBytes = (size_t)1 << 31;    // of one piece's d
-// Dimensions above which the last piece's exponentials are kept.  Measured (kept, taken again): 8192 x 131072 x 768 5.56,
-// 6.36 ms; 256 x 1000003 x 512 1.54, 1.71; 8192 x 50048 x 256 1.43, 1.43; 8192 x 50048 x 64 1.05, 0.92.
-constexpr int kKeepAbove = 256;
+
+// From which dim on something is kept.  Measured (rows x classes x dim, taken again, kept): bfloat16 1000 x 30000 x 128 140 141 us,
+// 60 x 200000 x 256 116 107, 256 x 1000003 x 512 1710 1540, 8192 x 131072 x 768 6360 5560;  float16 1000 x 30000 x 256 145 149, 300 x 100000 x 512 293 268, 4096 x 50000 x 2048 3127 2689;
+// float32 500 x 20000 x 64 138 130, 2000 x 30000 x 512 2029 1608: always.
+constexpr int kKeepAboveBf16 = 192, kKeepAboveF16 = 384;
 
 size_t put(size_t &at, size_t bytes)
 {
@@ -975,9 +988,11 @@ HeadPlan make_plan(long long rows, long long classes, long long dim, long long w
         // 256 bytes more than the piece, often a power of two: the rows that one store or load touches would otherwise all
         // lie in one channel of the L2 (d of 8192 x 65536: 2.2 -> 1.9 ms)
         q.ld_delta = q.piece + 256 / q.es;
-        // the pass over the kept exponentials and their stores move 6 bytes a logit, the products take 2 dim operations
-        q.keep = !q.few_parts && (dtype == SSDBOX_DTYPE_F32 ||
-                                 (dtype == SSDBOX_DTYPE_BF16 && q.tile == 2 && dim > kKeepAbove));
+        // The pass over what is kept and its stores move bytes, the products it spares take 2 dim operations a logit.
+        if (q.few_parts) q.keep = false;
+        else if (dtype == SSDBOX_DTYPE_F32) q.keep = true;
+        else if (dtype == SSDBOX_DTYPE_BF16) q.keep = dim > kKeepAboveBf16;
+        else q.keep = dim > kKeepAboveF16 && q.pieces == 1 && (size_t)(rows * q.ld_delta) * 4 <= kDeltaBytes;
     }
     size_t at = 0;
     q.o_few = put(at, (size_t)q.few_parts * rows * q.few_ld * 4);
@@ -993,6 +1008,7 @@ HeadPlan make_plan(long long rows, long long classes, long long dim, long long w
     q.o_sumz = put(at, smoothing != 0.0f && !q.few_parts ? (size_t)rows * q.slots * 4 : 0);
     q.o_weight = put(at, q.copy_weight ? (size_t)classes * q.pitch * q.es : 0);
     q.o_delta = put(at, grad ? (size_t)rows * q.ld_delta * q.es : 0);
+    q.o_kept = put(at, q.keep && dtype == SSDBOX_DTYPE_F16 ? (size_t)rows * q.ld_delta * 4 : 0);
     const long long wide = (dim + 3) / 4 * 4;
     if (grad_hidden) {
         cut_tile(dim, rows, (q.piece + bk - 1) / bk, q.es, false, q.dh_tile, q.dh_parts);
@@ -1037,10 +1053,8 @@ void launch_tiles(const HeadCall &c, const LogitArgs &a)
 template <typename T, int WHAT>
 void launch_logits(const HeadCall &c, int tile, const LogitArgs &a)
 {
-    if constexpr (WHAT != kStatKeep || sizeof(T) == 4) {
-        if (tile == 0) return launch_tiles<T, 128, 64, 4, 1, 2, WHAT>(c, a);
-        if (tile == 1) return launch_tiles<T, 128, 128, 2, 2, 2, WHAT>(c, a);
-    }
+    if (tile == 0) return launch_tiles<T, 128, 64, 4, 1, 2, WHAT>(c, a);
+    if (tile == 1) return launch_tiles<T, 128, 128, 2, 2, 2, WHAT>(c, a);
     if constexpr (sizeof(T) == 2) launch_tiles<T, 256, 256, 2, 4, 1, WHAT>(c, a);
 }
 
@@ -1136,6 +1150,7 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
     int *count = (int *)(c.ws + q.o_count), *row = (int *)(c.ws + q.o_row), *label = (int *)(c.ws + q.o_label);
     HeadScale *scale = (HeadScale *)(c.ws + q.o_scale);
     T *rows = (T *)(c.ws + q.o_rows);
+    void *kept = c.ws + (dtype == SSDBOX_DTYPE_F16 ? q.o_kept : q.o_delta);
 
     PrepArgs s = {};
     s.labels = c.labels;
@@ -1241,15 +1256,11 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
             if (c.classes < 4096) few(q.direct ? head_few_kernel<T, 256, true> : head_few_kernel<T, 256, false>, 256);
             else few(q.direct ? head_few_kernel<T, 1024, true> : head_few_kernel<T, 1024, false>, 1024);
         } else {
-            if constexpr (!__is_same(T, f16_t)) {
-                if (q.keep) {
-                    l.kept_from = (int)((q.pieces - 1) * q.piece);
-                    l.delta = c.ws + q.o_delta;
-                    l.ld_delta = q.ld_delta;
-                    launch_logits<T, kStatKeep>(c, q.tile, l);
-                } else {
-                    launch_logits<T, kStat>(c, q.tile, l);
-                }
+            if (q.keep) {
+                l.kept_from = (int)((q.pieces - 1) * q.piece);
+                l.delta = kept;
+                l.ld_delta = q.ld_delta;
+                launch_logits<T, kStatKeep>(c, q.tile, l);
             } else {
                 launch_logits<T, kStat>(c, q.tile, l);
             }
@@ -1280,8 +1291,11 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
             k.first = (int)first;
             k.classes = n_class;
             k.l2 = l.l2;
+            k.kept = kept;
+            k.ld_kept = q.ld_delta;
             k.delta = delta;
             k.ld_delta = q.ld_delta;
+            k.piece = q.piece;
             k.blocks = (int)((q.piece + kRowThreads * q.vec - 1) / (kRowThreads * q.vec));
             launch_stage(ctx, SSDBOX_STAGE_LOSS, head_kept_kernel<T>, dim3((unsigned)(c.rows * k.blocks)), dim3(kRowThreads), k);
         } else if (c.rows > 0) {

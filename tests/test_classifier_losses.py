@@ -132,7 +132,8 @@ HEAD_SIZES = [(1, 1, 1), (1, 2, 8), (3, 5, 7), (4, 1000, 128), (31, 257, 72), (3
               (130, 40, 1032), (300, 1500, 1024), (257, 515, 1030), (140, 700, 264), (4, 263, 1975), (2000, 44, 1216),
               (1, 9000, 600),
               # more logits than are written: statistics of tiles of every shape, d taken again or made of what was kept
-              (40, 16500, 24), (513, 16421, 24), (540, 16600, 270), (130, 65600, 40), (1030, 9001, 33), (5000, 2003, 72)]
+              (40, 16500, 24), (513, 16421, 24), (540, 16600, 270), (130, 65600, 40), (1030, 9001, 33), (5000, 2003, 72),
+              (300, 28001, 520), (41, 210001, 200)]
 
 
 @gpu
