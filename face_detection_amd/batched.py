@@ -359,7 +359,12 @@ def _row_floats(sess, x, name, shape):
     """A float32 array of the given shape on the device, or None."""
     if x is None:
         return None
-    t, _ = sess.put(x.detach() if _is_torch_tensor(x) and x.requires_grad else x, np.float32)
+    torch = _torch_if_loaded()
+    if (torch is not None and isinstance(x, torch.Tensor) and x.dtype is torch.float32 and x.is_cuda
+            and x.get_device() == sess.device and x.is_contiguous()):
+        t = x                                            # nothing to convert: most calls
+    else:
+        t, _ = sess.put(x.detach() if _is_torch_tensor(x) and x.requires_grad else x, np.float32)
     if tuple(t.shape) != shape:
         raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
     return t
@@ -375,7 +380,8 @@ def _aligned(t, ld, width):
 @_on_context_stream
 def linear_cross_entropy_batch(hidden, weight, labels, logit_scale=1.0, label_smoothing=0.0, grad_loss=None,
                                return_grad=False, weight_grad=True, context=None):
-    """Softmax cross entropy of a linear head over many classes; the logits are never stored whole.
+    """Softmax cross entropy of a linear head over many classes; of the logits and their gradient no
+    more than about 2 GiB each is ever stored.
 
     hidden (..., D) and weight (V,D) of one type (float32, float16, bfloat16); labels (...) int32 or
     int64.  logits = logit_scale * hidden weight^T.  A negative label leaves its row out: loss 0, no

@@ -33,6 +33,8 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.69314718055994530942;
 constexpr int kRowThreads = 256;
+constexpr long long kMostLd = 1 << 21;        // from one row of an operand to the next: a tile's rows in 32 bits of bytes
+constexpr long long kMostRows = (1 << 24) - 1;  // of workgroups of 256: a launch takes fewer than 2^32 threads
 constexpr int kRowsEach = 4;          // rows a workgroup places and copies
 constexpr int kCountRows = 1024;      // rows a workgroup counts, where there are many
 constexpr int kCountFrom = 4096;      // rows from which counting has a launch of its own: below, reading all labels before
@@ -1195,7 +1197,8 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
     }
     s.prep_blocks = (int)n_prep;
     s.stay = q.direct;
-    if (!q.direct || q.copy_weight || c.hidden_ld % q.vec != 0 || (uintptr_t)c.hidden % 16 != 0) {
+    // (rows as they are: 16-byte pieces, and a tile's rows within the 32 bits of its offsets)
+    if (!q.direct || q.copy_weight || c.hidden_ld % q.vec != 0 || (uintptr_t)c.hidden % 16 != 0 || c.hidden_ld > kMostLd) {
         launch_stage(ctx, SSDBOX_STAGE_LOSS, head_prep_kernel<T>, dim3(n_prep + n_pitch), dim3(kRowThreads), s);
         s.hidden = rows;
         s.ld = q.pitch;
@@ -1267,7 +1270,7 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
             } else {
                 launch_logits<T, kStat>(c, q.tile, l);
             }
-            if (q.slots < 2048)
+            if (q.slots < 2048 || c.rows > kMostRows / 4)
                 launch_stage(ctx, SSDBOX_STAGE_LOSS, head_row_kernel<256>, dim3((unsigned)c.rows), dim3(256), r);
             else
                 launch_stage(ctx, SSDBOX_STAGE_LOSS, head_row_kernel<1024>, dim3((unsigned)c.rows), dim3(1024), r);
@@ -1361,11 +1364,11 @@ int check_sizes(int64_t rows, int64_t classes, int64_t dim, int64_t weight_ld, i
 {
     SSD_REQUIRE(dtype == SSDBOX_DTYPE_F32 || dtype == SSDBOX_DTYPE_F16 || dtype == SSDBOX_DTYPE_BF16,
                 "linear_cross_entropy: dtype %d", dtype);
-    SSD_REQUIRE(rows >= 0 && rows <= (1 << 24), "linear_cross_entropy: %lld rows outside [0, 2^24]", (long long)rows);
+    SSD_REQUIRE(rows >= 0 && rows <= kMostRows, "linear_cross_entropy: %lld rows outside [0, 2^24)", (long long)rows);
     SSD_REQUIRE(classes >= 1 && classes <= (1 << 28), "linear_cross_entropy: %lld classes outside [1, 2^28]",
                 (long long)classes);
     SSD_REQUIRE(dim >= 1 && dim <= (1 << 20), "linear_cross_entropy: dim %lld outside [1, 2^20]", (long long)dim);
-    SSD_REQUIRE(weight_ld >= dim && weight_ld <= (1 << 21), "linear_cross_entropy: weight row stride %lld outside [%lld, 2^21]",
+    SSD_REQUIRE(weight_ld >= dim && weight_ld <= kMostLd, "linear_cross_entropy: weight row stride %lld outside [%lld, 2^21]",
                 (long long)weight_ld, (long long)dim);
     SSD_REQUIRE(smoothing >= 0.0f && smoothing < 1.0f, "linear_cross_entropy: label_smoothing %g outside [0, 1)", smoothing);
     return SSDBOX_OK;
@@ -1409,7 +1412,8 @@ extern "C" int ssdbox_linear_cross_entropy(ssdbox_ctx *ctx, const void *d_hidden
                     ((uintptr_t)d_grad_hidden % 16) == 0 && ((uintptr_t)d_grad_weight % 16) == 0,
                 "linear_cross_entropy: weight and gradients have to start at 16 bytes, the workspace at 256");
     SSD_REQUIRE(q.class_tiles * ((rows + q.bn - 1) / q.bn) < (1ll << 31) &&
-                    (q.pieces == 0 || (dim + q.bm - 1) / q.bm * ((rows + q.bn - 1) / q.bn) < (1ll << 31)),
+                    (q.pieces == 0 || (dim + 127) / 128 * ((rows + 63) / 64) * q.dh_parts < (1ll << 31)) &&
+                    (d_grad_hidden == nullptr || (dim + 255) / 256 * rows <= kMostRows * 4),
                 "linear_cross_entropy: %lld rows x %lld classes", (long long)rows, (long long)classes);
 
     DeviceGuard guard(ctx->device);

@@ -108,7 +108,7 @@ def test_workspace_refusals_and_sizes():
         return lib.ssdbox_linear_cross_entropy_workspace(rows, classes, dim, ld, dtype, smoothing, 1, 1, ctypes.byref(need))
     assert head() == _lib.OK and need.value > 0
     assert head(rows=0) == _lib.OK and head(rows=1, classes=1, dim=1, ld=1) == _lib.OK
-    for bad in ({"rows": -1}, {"rows": (1 << 24) + 1}, {"classes": 0}, {"classes": (1 << 28) + 1}, {"dim": 0},
+    for bad in ({"rows": -1}, {"rows": 1 << 24}, {"classes": 0}, {"classes": (1 << 28) + 1}, {"dim": 0},
                 {"dim": 17}, {"ld": 15}, {"ld": (1 << 21) + 1}, {"dtype": 3}, {"dtype": -1}, {"smoothing": 1.0},
                 {"smoothing": -0.1}, {"smoothing": float("nan")}):
         assert head(**bad) == _lib.ERR_INVALID, bad
@@ -271,6 +271,19 @@ def test_head_strides_and_alignment(n, v, dtype):
     flat = torch.empty(v * 40 + 1, device="cuda", dtype=dtype)
     flat[1:] = weight.reshape(-1)
     same(hidden, flat[1:].view(v, 40))                            # a base off any boundary
+
+
+@gpu
+def test_head_rows_far_apart():
+    """Rows of hidden whose distance passes 32 bits within one tile, read where they are or copied."""
+    import face_detection_amd as fda
+    hidden, weight, labels = head_inputs(3, 70, 40, torch.float16, seed=4, device="cuda")
+    want = fda.linear_cross_entropy_batch(hidden, weight, labels, return_grad=True)
+    for ld in (1 << 21, (1 << 21) + 8, 1 << 30):
+        far = torch.empty(2 * ld + 40, device="cuda", dtype=torch.float16).as_strided((3, 40), (ld, 1))
+        far.copy_(hidden)
+        got = fda.linear_cross_entropy_batch(far, weight, labels, return_grad=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 @gpu
@@ -499,10 +512,14 @@ def both_inputs(seed, n=96, v=5000, dim=64):
     return hidden, weight, labels, values, index
 
 
+BOTH_SIZES = [(96, 5000, 64), (600, 16390, 224), (40, 103000, 40)]     # few logits, tiles of them, rows beyond registers
+
+
 @gpu
-def test_both_losses_on_other_streams_and_contexts():
+@pytest.mark.parametrize("size", BOTH_SIZES, ids=str)
+def test_both_losses_on_other_streams_and_contexts(size):
     from face_detection_amd.runtime import Context
-    sets = [both_inputs(s) for s in range(3)]
+    sets = [both_inputs(s, *size) for s in range(3)]
     want = [both(*x) for x in sets]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in sets]
@@ -520,10 +537,11 @@ def test_both_losses_on_other_streams_and_contexts():
 
 
 @gpu
-def test_both_losses_in_captured_graphs():
+@pytest.mark.parametrize("size", BOTH_SIZES, ids=str)
+def test_both_losses_in_captured_graphs(size):
     """Two graphs of the same calls, replayed in turn with eager calls between: each has its own workspace."""
     import face_detection_amd as fda
-    sets = [both_inputs(s) for s in range(4)]
+    sets = [both_inputs(s, *size) for s in range(4)]
     want = [both(*x) for x in sets]
 
     def losses(x):
