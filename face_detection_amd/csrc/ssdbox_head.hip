@@ -833,8 +833,8 @@ struct JoinArgs {
     const int *row_of;
 };
 
-// The parts of a product over a long k, added in a fixed order: reads from the caches (128 parts of 256 x 512: 67 MB in 13 us).  Four values a lane, eight parts on their way at a time;
-// WAVES waves share the parts of one piece of 256 values.
+// The parts of a product over a long k, added in a fixed order: reads from the caches (128 parts of 256 x 512: 67 MB
+// in 13 us).  Four values a lane, eight parts on their way at a time; up to WAVES waves share the parts of 256 values.
 template <typename T, int WAVES>
 SSD_DEV void join(const JoinArgs &p, int block, f32x4 (&s_sum)[WAVES > 1 ? WAVES : 1][64])
 {
@@ -914,9 +914,10 @@ struct HeadPlan {
 
 constexpr size_t kDeltaBytes = (size_t)1 << 31;    // of one piece's d
 
-// From which dim on something is kept.  Measured (rows x classes x dim, taken again, kept): bfloat16 1000 x 30000 x 128 140 141 us,
-// 60 x 200000 x 256 116 107, 256 x 1000003 x 512 1710 1540, 8192 x 131072 x 768 6360 5560;  float16 1000 x 30000 x 256 145 149, 300 x 100000 x 512 293 268, 4096 x 50000 x 2048 3127 2689;
-// float32 500 x 20000 x 64 138 130, 2000 x 30000 x 512 2029 1608: always.
+// From which dim on something is kept.  Measured (rows x classes x dim, taken again, kept; us):
+//   bfloat16  1000 x 30000 x 128 140 141,  60 x 200000 x 256 116 107,  256 x 1000003 x 512 1710 1540,  8192 x 131072 x 768 6360 5560
+//   float16   1000 x 30000 x 256 145 149,  300 x 100000 x 512 293 268,  4096 x 50000 x 2048 3127 2689
+//   float32   500 x 20000 x 64 138 130,  2000 x 30000 x 512 2029 1608: always
 constexpr int kKeepAboveBf16 = 192, kKeepAboveF16 = 384;
 
 size_t put(size_t &at, size_t bytes)

@@ -321,6 +321,34 @@ def test_head_several_pieces(dim):
 
 
 @gpu
+def test_head_weight_beyond_32_bits():
+    """A weight, and its gradient, of more than 2^32 bytes."""
+    import face_detection_amd as fda
+    n, v, dim = 64, 1100001, 2048
+    weight = torch.randn(v, dim, device="cuda", dtype=torch.bfloat16) * (1.5 / math.sqrt(dim))
+    hidden = torch.randn(n, dim, device="cuda").bfloat16()
+    labels = torch.randint(v - 1000, v, (n,), device="cuda")
+    loss, gh, gw = fda.linear_cross_entropy_batch(hidden, weight, labels, return_grad=True)
+    z = torch.cat([hidden.double() @ weight[a:a + 50000].double().t() for a in range(0, v, 50000)], 1)
+    logp = torch.log_softmax(z, 1)
+    del z
+    within(loss, -logp.gather(1, labels[:, None])[:, 0], torch.full((n,), 1e-4), "loss")
+    p = logp.exp().scatter_add_(1, labels[:, None], torch.full((n, 1), -1.0, device="cuda", dtype=torch.float64)) / n
+    del logp
+    cols = torch.cat([torch.arange(0, 50), torch.arange(v - 1000, v)]).cuda()
+    want, size = p[:, cols].t() @ hidden.double(), p[:, cols].abs().t() @ hidden.double().abs()
+    # d to bfloat16 (through 16 bits of exponentials, 2^-11 more), the sum to float32, the result to bfloat16
+    # and 1e-4 for the logits: 2048 additions to sums of at most 8, each off by 2^-22 or less, as a random walk 1.1e-5
+    within(gw[cols], want, (2 ** -8 + 2 ** -11 + n * O.U + 1e-4) * size * 1.01 + 2 ** -8 * want.abs() + 1e-12, "grad_weight")
+    want, size = torch.zeros(n, dim, device="cuda", dtype=torch.float64), torch.zeros(n, dim, device="cuda", dtype=torch.float64)
+    for a in range(0, v, 50000):
+        w = weight[a:a + 50000].double()
+        want += p[:, a:a + 50000] @ w
+        size += p[:, a:a + 50000].abs() @ w.abs()
+    within(gh, want, (2 ** -8 + 2 ** -11 + 1e-4) * size * 1.01 + 2 ** -8 * want.abs() + 1e-12, "grad_hidden")
+
+
+@gpu
 def test_head_numpy_and_halves():
     import face_detection_amd as fda
     for dtype in (torch.float32, torch.float16):
@@ -460,6 +488,23 @@ def test_distill_strides_and_families():
         wide[:, 5:5 + v] = z
         got = fda.distill_topk_batch(wide[:, 5:5 + v], values, index, return_grad=True)
         assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@gpu
+def test_distill_beyond_32_bits():
+    """More than 2^31 logits: the rows behind the border as if they were alone."""
+    import face_detection_amd as fda
+    n, v, last = 55000, 40000, 700
+    z = torch.randn(n, v, device="cuda", dtype=torch.bfloat16)
+    values, index = torch.randn(n, 4, device="cuda"), torch.randint(0, v, (n, 4), device="cuda")
+    g = torch.rand(n, device="cuda")
+    loss, grad = fda.distill_topk_batch(z, values, index, temperature=2.0, grad_loss=g, return_grad=True)
+    alone = fda.distill_topk_batch(z[-last:].clone(), values[-last:], index[-last:], temperature=2.0, grad_loss=g[-last:],
+                                   return_grad=True)
+    assert torch.equal(loss[-last:], alone[0]) and torch.equal(grad[-last:], alone[1])
+    first = fda.distill_topk_batch(z[:last].clone(), values[:last], index[:last], temperature=2.0, grad_loss=g[:last],
+                                   return_grad=True)
+    assert torch.equal(loss[:last], first[0]) and torch.equal(grad[:last], first[1])
 
 
 @gpu
