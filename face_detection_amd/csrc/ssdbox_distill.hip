@@ -607,12 +607,31 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void distill_row_kernel(co
 }
 
 // ----------------------------------------------------------------------- few classes a row
-// G lanes a row, up to 4 classes a lane.  Latency of the entries' chain of loads (408000 x 2 x 2 float32: 11 us, 1.6 TB/s).
+// G lanes a row, up to 4 classes and every G-th entry a lane.  Latency of the entries' chain of loads (408000 x 2 x 2 float32: 11 us, 1.6 TB/s).
+// Joins by DPP: a lane's neighbour, the quad's other half, then the mirrored lane of eight and of sixteen, where the halves are
+// the same in all their lanes already.  Both sides of every join are the same two values: all lanes get the same bits.
+template <int CTRL>
+SSD_DEV float across(float x)
+{
+    return dpp<CTRL, 0xf>(x, x);
+}
+template <int CTRL>
+SSD_DEV double across(double x)
+{
+    return dpp<CTRL, 0xf>(x);
+}
+template <int CTRL>
+SSD_DEV int across(int x)
+{
+    return __builtin_amdgcn_update_dpp(0, x, CTRL, 0xf, 0xf, false);
+}
 template <int G, typename X, typename F>
 SSD_DEV X group(X x, F f)
 {
-#pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1) x = f(x, __shfl_xor(x, o));
+    if constexpr (G >= 2) x = f(x, across<0xB1>(x));
+    if constexpr (G >= 4) x = f(x, across<0x4E>(x));
+    if constexpr (G >= 8) x = f(x, across<0x141>(x));
+    if constexpr (G >= 16) x = f(x, across<0x140>(x));
     return x;
 }
 
@@ -635,32 +654,42 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const DistArgs p)
         x[i] = j < p.classes ? (float)z[j] : -INFINITY;
         m = fmaxf(m, x[i]);
     }
-    for (int k = 0; k < p.top; ++k) {
-        const Entry e = entry_of(p, row, k);
-        if (e.at < 0) continue;
-        ++entries;
-        t_top = fmaxf(t_top, e.t);
+    // Entries are dealt to the lanes, G at a time; what a class's own lane has to know of them comes by shuffles.
+    const int lane0 = (threadIdx.x & 63) - l;
+    const auto entry = [&](int k) { return k < p.top ? entry_of(p, row, k) : Entry{-1, -INFINITY}; };
+    for (int k0 = 0; k0 < p.top; k0 += G) {
+        const Entry e = entry(k0 + l);
+        if (e.at >= 0) {
+            ++entries;
+            t_top = fmaxf(t_top, e.t);
+        }
+        for (int j = 0; j < G && k0 + j < p.top; ++j) {
+            const int at = __shfl(e.at, lane0 + j);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (e.at == l + G * i) in |= 1u << i;
+            for (int i = 0; i < 4; ++i)
+                if (at == l + G * i) in |= 1u << i;
+        }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         if (!(in >> i & 1u)) mo = fmaxf(mo, x[i]);
     m = group<G>(m, more);
     mo = group<G>(mo, more);
+    t_top = group<G>(t_top, more);
+    entries = group<G>(entries | (int)__popc(in) << 16, [](int a, int b) { return a + b; });
+    const int inside = entries >> 16;
+    entries &= 0xFFFF;
     RowTerms f;
     f.l2 = (float)(kLog2eD / (double)p.tau);
     const float mref = m == -INFINITY ? 0.0f : m, oref = mo == -INFINITY ? 0.0f : mo;
-    double sum[3] = {0.0, 0.0, 0.0};
+    double sum[2] = {0.0, 0.0};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         sum[0] += (double)__builtin_amdgcn_exp2f((x[i] - mref) * f.l2);
         if (!(in >> i & 1u)) sum[1] += (double)__builtin_amdgcn_exp2f((x[i] - oref) * f.l2);
-        sum[2] += (double)(in >> i & 1u);
     }
 #pragma unroll
-    for (int i = 0; i < 3; ++i) sum[i] = group<G>(sum[i], plus);
+    for (int i = 0; i < 2; ++i) sum[i] = group<G>(sum[i], plus);
     T *g = (T *)p.grad + row * p.classes;
     if (entries == 0) {
         if (l == 0) p.loss[row] = 0.0f;
@@ -671,28 +700,40 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const DistArgs p)
         return;
     }
     double st = 0.0;
-    if (!p.teacher_lse)
-        for (int k = 0; k < p.top; ++k) {
-            const Entry e = entry_of(p, row, k);
+    if (!p.teacher_lse) {
+        for (int k0 = 0; k0 < p.top; k0 += G) {
+            const Entry e = entry(k0 + l);
             if (e.at >= 0) st += (double)__builtin_amdgcn_exp2f((e.t - t_top) * f.l2);
         }
+        st = group<G>(st, plus);
+    }
     f.sub = mref;
     f.off = 0.0f;
     f.inv_s = 1.0 / sum[0];
     f.ln_s = ln_of(sum[0]);
     terms_teacher(f, p, row, t_top, st);
     double of_entries[3] = {0.0, 0.0, 0.0}, q_at[4] = {0.0, 0.0, 0.0, 0.0};
-    const bool dup = entries > (int)sum[2];
-    for (int k = 0; k < p.top; ++k) {
-        const Entry e = entry_of(p, row, k);
-        if (e.at < 0) continue;
-        add_entry(of_entries, f, p, row, k, e, (float)z[e.at], dup);
+    const bool dup = entries > inside;
+    for (int k0 = 0; k0 < p.top; k0 += G) {
+        const Entry e = entry(k0 + l);
+        float q = 0.0f;
+        if (e.at >= 0) {
+            add_entry(of_entries, f, p, row, k0 + l, e, (float)z[e.at], dup);
+            q = f.q(e.t);
+        }
+        if (p.grad)
+            for (int j = 0; j < G && k0 + j < p.top; ++j) {
+                const int at = __shfl(e.at, lane0 + j);
+                const float of = __shfl(q, lane0 + j);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (e.at == l + G * i) q_at[i] += (double)f.q(e.t);
+                for (int i = 0; i < 4; ++i)
+                    if (at == l + G * i) q_at[i] += (double)of;
+            }
     }
+#pragma unroll
+    for (int i = 0; i < 3; ++i) of_entries[i] = group<G>(of_entries[i], plus);
     const double loss = terms_finish(f, p, row, of_entries[0], of_entries[1], of_entries[2], oref, sum[1],
-                                     (int)sum[2] < p.classes);
+                                     inside < p.classes);
     if (l == 0) p.loss[row] = (float)loss;
     if (!p.grad) return;
 #pragma unroll
