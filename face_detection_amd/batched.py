@@ -378,6 +378,13 @@ def _aligned(t, ld, width):
     return t.clone(memory_format=_torch().contiguous_format), width
 
 
+def _empty_like(sess, t, shape, dtype):
+    """A dense array of t's shape and type."""
+    if sess.use_torch and t.shape == shape and t.is_contiguous():
+        return _torch().empty_like(t)
+    return sess.empty(shape, dtype)
+
+
 @_on_context_stream
 def linear_cross_entropy_batch(hidden, weight, labels, logit_scale=1.0, label_smoothing=0.0, grad_loss=None,
                                return_grad=False, weight_grad=True, context=None):
@@ -411,8 +418,8 @@ def linear_cross_entropy_batch(hidden, weight, labels, logit_scale=1.0, label_sm
     need = _head_bytes(rows, classes, dim, ld_w, code, float(label_smoothing), int(bool(return_grad)),
                        int(bool(return_grad and weight_grad)))
     loss = sess.empty(lead)
-    gh = sess.empty(lead + (dim,), dtype) if return_grad else None
-    gw = sess.empty((classes, dim), dtype) if return_grad and weight_grad else None
+    gh = _empty_like(sess, h, lead + (dim,), dtype) if return_grad else None
+    gw = _empty_like(sess, w, (classes, dim), dtype) if return_grad and weight_grad else None
     work = sess.empty((need,), np.uint8)
     _lib.check(ctx.lib.ssdbox_linear_cross_entropy(
         ctx.handle, _at(h), ld_h, _at(w), ld_w, _at(lab), label_bytes, rows, classes, dim, code,
@@ -457,7 +464,7 @@ def distill_topk_batch(logits, teacher_values, teacher_index, temperature=1.0, t
     g = _row_floats(sess, grad_loss, "grad_loss", lead) if return_grad else None
     need = _distill_bytes(rows, classes, code)
     loss = sess.empty(lead)
-    grad = sess.empty(lead + (classes,), dtype) if return_grad else None
+    grad = _empty_like(sess, z, lead + (classes,), dtype) if return_grad else None
     work = sess.empty((need,), np.uint8) if need else None
     _lib.check(ctx.lib.ssdbox_distill_topk(
         ctx.handle, _at(z), ld, rows, classes, code, _at(values), _at(index), index_bytes, top, _at(lse),

@@ -173,12 +173,18 @@ def default_context(device=None, torch_stream=None):
     if cache is None:
         cache = _tls.contexts = {}
     if torch_stream:
-        stream = _torch().cuda.current_stream(device)
-        key = (device, stream.cuda_stream)
+        torch = _torch()
+        handle_of = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # (no Stream object: 0.1 us instead of 1)
+        stream = None
+        if handle_of is None or not torch.cuda.is_initialized():
+            stream = torch.cuda.current_stream(device)
+        key = (device, stream.cuda_stream if stream is not None else handle_of(device))
     else:
         stream, key = "own", (device, "own")
     ctx = cache.get(key)
     if ctx is None:
+        if stream is None:
+            stream = _torch().cuda.current_stream(device)
         ctx = cache[key] = Context(device, stream)
     return ctx
 
