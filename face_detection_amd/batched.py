@@ -445,7 +445,9 @@ def distill_topk_batch(logits, teacher_values, teacher_index, temperature=1.0, t
       teacher_lse (...), the log-sum-exp of all the teacher's logits / temperature:
       q = exp(teacher_values / temperature - teacher_lse), and the classes without an entry form one
       bucket of both.
-    A row without an entry has loss 0 and no gradient.  With return_grad also the (..., V) gradient
+    A row without an entry has loss 0 and no gradient.  The loss is +inf where the teacher gives
+    something to an entry, or to a bucket, whose logits are all -inf; of such a bucket (or one that
+    underflows) up to 2^-20 (1 + |lse|), the rounding of teacher_lse, counts as nothing.  With return_grad also the (..., V) gradient
     in the logits' type of sum(grad_loss * loss), or of mean(loss) when grad_loss (...) is None.
     The tensors' autograd graph is not extended: the gradient is what the call returns.
     """

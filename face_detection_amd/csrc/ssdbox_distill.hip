@@ -4,7 +4,7 @@
 //   without its log-sum-exp: q = softmax over the K of t / tau, no rest
 //   with it (at tau):        q = exp(t / tau - lse), q_r = 1 - sum q; the classes outside S are one bucket, p_r of p
 //   loss = tau^2 (sum_k q_k (log q_k - log p_k) + q_r (log q_r - log p_r))
-//   grad_j = g tau (p_j (Q + q_r) - q_j)  in S,   g tau p_j (Q + q_r - q_r / p_r)  outside,   Q = sum q
+//   grad_j = g tau (p_j (Q + q_r) - q_j)  in S,   g tau p_j (Q + q_r - q_r / p_r)  outside (0 where p_r is 0),   Q = sum q
 //
 // A row is read once, stays in registers for its maximum, its sum and its gradient, and is written once: 2 * V values a row
 // is all the HBM traffic there is, which bounds the kernel.  Rows of up to 64 classes: a few lanes a row, each with its
@@ -311,20 +311,24 @@ SSD_DEV double terms_finish(RowTerms &r, const DistArgs &p, long long row, doubl
     r.c = (float)(g * (double)p.tau);
     r.whole = sum_q;
     double loss = sum_loss, out = r.whole * r.inv_s;
-    if (p.teacher_lse) {
+    if (p.teacher_lse && outside) {
         double q_r = 1.0 - sum_q;
         if (q_r < 0.0) q_r = 0.0;
-        if (outside && so > 0.0) {
-            r.osub = osub;
+        // near 1 a bucket is what the entries leave of it, to their own relative error
+        const double ln_pr = sum_p < 0.5 ? ln_of(1.0 - sum_p)
+                                         : ((double)osub - (double)r.sub) * (double)r.l2 * kLn2 + ln_of(so) - r.ln_s;
+        // Where the student has nothing of the bucket that float32 holds (masked classes), a rest that is no more than the
+        // rounding of a float32 log-sum-exp is nothing too: times ln p_r, it would be all of the loss.  A larger one counts as
+        // defined: +inf where every class outside is -inf, whose shares of the bucket are then none.
+        if (!(ln_pr < -104.0 && q_r <= 0x1p-20 * (1.0 + fabs(r.ln_t)))) {
             r.whole = sum_q + q_r;
-            if (q_r > 0.0) {
-                // near 1 a bucket is what the entries leave of it, to their own relative error
-                const double ln_pr = sum_p < 0.5 ? ln_of(1.0 - sum_p)
-                                                 : ((double)osub - (double)r.sub) * (double)r.l2 * kLn2 + ln_of(so) - r.ln_s;
-                loss += q_r * (ln_of(q_r) - ln_pr);
+            if (q_r > 0.0) loss += q_r * (ln_of(q_r) - ln_pr);
+            out = 0.0;
+            if (so != 0.0) {
+                r.osub = osub;
+                const double down = (double)__builtin_amdgcn_exp2f((osub - r.sub) * r.l2);
+                out = r.whole * r.inv_s * down - q_r / so;
             }
-            const double down = (double)__builtin_amdgcn_exp2f((osub - r.sub) * r.l2);
-            out = r.whole * r.inv_s * down - q_r / so;
         }
     }
     r.out = (float)(out * (double)r.c);

@@ -319,7 +319,10 @@ int ssdbox_linear_cross_entropy(ssdbox_ctx *ctx, const void *d_hidden, int64_t h
  * d_teacher_lse (rows), the log-sum-exp of ALL the teacher's logits / temperature: q =
  *   exp(value / temperature - lse), and the classes without an entry form one bucket, which holds
  *   1 - sum q of the teacher and the sum of p there of the student.
- *   d_loss (rows): temperature^2 * KL(q || p) over the entries (and the bucket).
+ *   d_loss (rows): temperature^2 * KL(q || p) over the entries (and the bucket): +infinity where the
+ *   teacher gives something to an entry, or to a bucket, of -infinity alone.  (Of a bucket in which the
+ *   student has nothing that float32 holds, up to 2^-20 (1 + |lse|) of the teacher, which is no more
+ *   than the rounding of a float32 lse, counts as nothing.)  Such a bucket's classes have gradient 0.
  *   d_grad (rows, classes), dense, of `dtype`, or NULL: gradient of sum_n d_grad_loss[n] loss[n], with
  *   d_grad_loss NULL of the mean over the rows.
  * The same inputs give the same bits. */

@@ -84,16 +84,19 @@ def distill(logits, values, index, tau=1.0, lse=None, grad_loss=None):
     part = p * total + away
     if lse is not None:
         other = torch.where(inside, 0.0, p)
-        rest_p, rest_q = other.sum(1, keepdim=True), (1 - total).clamp(min=0)
-        use = (~inside).any(1, keepdim=True) & (rest_p > 0)
+        rest_q = (1 - total).clamp(min=0)
         ln_p = torch.logsumexp(torch.where(inside, -float("inf"), logp), 1)[:, None]
+        # a float32 log-sum-exp says no more of 1 - Q than this; where the student has nothing either, that is nothing
+        empty = (ln_p < -104) & (rest_q <= 2.0 ** -20 * (1 + whole.abs()[:, None]))
+        use = (~inside).any(1, keepdim=True) & ~empty
         rest = torch.where(use & (rest_q > 0), rest_q * (torch.log(rest_q.clamp(min=1e-300)) - ln_p), 0.0)
         loss, size = loss + rest[:, 0], size + (rest.abs() + 2 * rest_q * use)[:, 0]
-        factor = torch.where(use, rest_q / rest_p.clamp(min=1e-300), 0.0)
-        d = p * (total + rest_q * use) - away - other * factor
-        part = p * (total + rest_q * use) + away + other * factor
-        # q_r = 1 - Q is off by what Q is: by 2^-23 of the share at most, which the factor passes on
-        part = part + other / rest_p.clamp(min=1e-300) * use
+        # the classes' shares of the bucket; where the student has none of it, none
+        share = torch.softmax(torch.where(inside, -float("inf"), u), 1)
+        share = torch.where(inside | (ln_p == -float("inf")) | ~use, 0.0, share)
+        d = p * (total + rest_q * use) - away - share * rest_q
+        # q_r = 1 - Q is off by what Q is: by 2^-23 of the share at most, which the bucket's classes pass on
+        part = p * (total + rest_q * use) + away + share * (1 + rest_q)
     g = torch.full((n,), 1.0 / max(n, 1), dtype=torch.float64, device=u.device) if grad_loss is None else grad_loss.double()
     loss = torch.where(has, loss, 0.0) * tau ** 2
     d = torch.where(has[:, None], d, 0.0) * (g * tau)[:, None]

@@ -1,0 +1,86 @@
+"""The classifier losses where their definitions reach a limit: a rest bucket that the student masks whole, classes far above
+the teacher's, many rows, gradients in several pieces.  Bounds as in tests/test_classifier_losses.py."""
+import math
+
+import pytest
+import torch
+
+from oracle import classifier_oracle as O
+from test_classifier_losses import TYPES, distill_inputs, within
+
+gpu = pytest.mark.gpu
+INF = float("inf")
+
+
+# ------------------------------------------------------------------------------------------------ distillation: the bucket
+def masked_bucket(n, v, k, dtype, tau, device="cpu"):
+    """Rows whose classes outside the entries the student masks: 0 by -inf, of which the teacher has something there; 1 the same
+    by the type's lowest value; 2 and 3 as these, where the teacher has nothing there; 4 some of the entries too; 5 not masked;
+    6 all but the last class outside."""
+    z, values, index, lse = distill_inputs(n, v, k, dtype, seed=11, tau=tau, tail=True)
+    inside = torch.zeros(n, v, dtype=torch.bool).scatter_(1, index, True)
+    low = torch.finfo(dtype).min
+    lse = torch.maximum(lse, (values / tau).logsumexp(1) + 0.25)    # at least a fifth of the teacher lies outside
+    for row, mask in ((0, -INF), (1, low), (2, -INF), (3, low), (4, -INF)):
+        z[row] = torch.where(inside[row], z[row], torch.tensor(mask, dtype=dtype))
+    for row in (2, 3):                                              # 1 - sum q is what float32 rounds off
+        lse[row] = (values[row] / tau).logsumexp(0)
+    z[4, index[4, 0]] = -INF
+    last = int((~inside[6]).nonzero()[-1])
+    keep = inside[6].clone()
+    keep[last] = True
+    z[6] = torch.where(keep, z[6], torch.tensor(-INF, dtype=dtype))
+    return [x.to(device) for x in (z, values, index, lse)], inside.to(device)
+
+
+def test_masked_bucket_by_its_definition():
+    """The definition's sums written out, in 64 bits."""
+    tau = 2.0
+    (z, values, index, lse), inside = masked_bucket(7, 12, 3, torch.float32, tau)
+    (loss, grad), _ = O.distill(z, values, index, tau, lse, torch.ones(7))
+    for n in range(7):
+        u = z[n].double() / tau
+        lp = u - u.logsumexp(0)
+        q = (values[n].double() / tau - lse[n].double()).exp()
+        qr = 1 - float(q.sum())
+        kl = sum(float(a) * (math.log(float(a)) - float(lp[i])) for a, i in zip(q, index[n]))
+        lpr = float(lp[~inside[n]].logsumexp(0))
+        if n in (2, 3):
+            assert abs(qr) < 1e-6 and lpr < -1e30
+        else:
+            assert qr > 0.15
+            kl += qr * (math.log(qr) - lpr)
+        want = kl * tau ** 2
+        assert float(loss[n]) == want or abs(float(loss[n]) - want) < 1e-9 * (1 + abs(want)), n
+        assert (want == INF) == (n in (0, 4))
+        away = torch.zeros(12, dtype=torch.float64).scatter_add_(0, index[n], q)
+        whole = 1.0 if n not in (2, 3) else float(q.sum())
+        at = inside[n]
+        assert torch.allclose(grad[n][at], (tau * (lp.exp() * whole - away))[at], rtol=1e-9, atol=1e-12)
+        if n in (0, 2, 3, 4):
+            assert (grad[n][~at] == 0).all()
+
+
+# one to sixteen lanes a row, sixteen, a wave, workgroups of 256 and 512, rows longer than the registers, cut rows
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("n,v,k", [(7, 4, 2), (7, 7, 3), (7, 14, 3), (7, 30, 5), (7, 60, 5), (7, 200, 9), (7, 700, 40), (7, 700, 70),
+                                   (7, 3001, 5), (7, 9001, 5), (7, 30000, 8), (7, 60000, 8), (64, 140001, 6),
+                                   (64, 220001, 6), (7, 210001, 6)])
+def test_distill_bucket_masked_whole(n, v, k, dtype):
+    import face_detection_amd as fda
+    tau = 2.0
+    args, inside = masked_bucket(n, v, k, dtype, tau, "cuda")
+    z, values, index, lse = args
+    want, off = O.distill(z, values, index, tau, lse)
+    got = fda.distill_topk_batch(z, values, index, temperature=tau, teacher_lse=lse, return_grad=True)
+    # (row 1: tau^2 q_r 3.4e38 / tau, which float32 holds up to q_r = 1 / 2)
+    finite = torch.isfinite(want[0].float())
+    assert (got[0][~finite] == INF).all() and not finite[0] and not finite[4] and finite[[2, 3, 5, 6]].all()
+    within(got[0][finite], want[0][finite], off[0][finite], "loss")
+    off_g = torch.where(torch.isfinite(off[1]), off[1], 0.0)
+    within(got[1], want[1], off_g, "grad")
+    for row in (0, 2, 3, 4):
+        assert (got[1][row][~inside[row]] == 0).all()
+    alone = fda.distill_topk_batch(z, values, index, temperature=tau, teacher_lse=lse)
+    assert torch.equal(alone, got[0])
