@@ -248,7 +248,8 @@ struct RowTerms {
     double t_top, ln_t;               // log q = (t - t_top) / tau - ln_t
     double inv_tau;
     double whole;                     // Q + q_r
-    float osub, out;                  // outside: grad = 2^((z - osub) l2 - off) out
+    float osub;
+    double out;                       // outside: grad = 2^((z - osub) l2 - off) out
     float c;                          // g tau
 
     SSD_DEV double log_q(float t) const { return ((double)t - t_top) * inv_tau - ln_t; }
@@ -308,7 +309,8 @@ SSD_DEV double terms_finish(RowTerms &r, const DistArgs &p, long long row, doubl
 {
     r.osub = r.sub;
     const double g = p.grad_loss ? (double)p.grad_loss[row] : 1.0 / (double)p.rows;
-    r.c = (float)(g * (double)p.tau);
+    const double c = g * (double)p.tau;
+    r.c = (float)c;
     r.whole = sum_q;
     double loss = sum_loss, out = r.whole * r.inv_s;
     if (p.teacher_lse && outside) {
@@ -331,7 +333,7 @@ SSD_DEV double terms_finish(RowTerms &r, const DistArgs &p, long long row, doubl
             }
         }
     }
-    r.out = (float)(out * (double)r.c);
+    r.out = out * c;
     return loss * (double)p.tau * (double)p.tau;
 }
 
@@ -560,7 +562,11 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void distill_row_kernel(co
         const double loss = terms_finish(f, p, row, of_entries[0], of_entries[1], of_entries[2], osub, sum[0], outside);
         if (t == 0) p.loss[row] = n_inside > 0 ? (float)loss : 0.0f;      // a row without an entry teaches nothing
         T *g = (T *)p.grad + row * p.classes;
-        if (p.grad && !slow) {
+        // Against a reference that the row's largest exponential exceeds by up to 2^120, out is as small, and what g tau takes off it
+        // too may leave float32's range: such a row is read again, and the exponent of out is a factor of its own.
+        const float out = (float)f.out;
+        const bool in_range = (fabsf(out) >= 0x1p-100f && fabsf(out) <= 0x1p100f) || f.c == 0.0f;
+        if (p.grad && !slow && in_range) {
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 v.forget(r);
@@ -569,7 +575,7 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void distill_row_kernel(co
                     Piece<T> o;
 #pragma unroll
                     for (int j = 0; j < N; ++j)
-                        o.v[j] = (T)(__builtin_amdgcn_exp2f(__builtin_fmaf(v.value(r, j), f.l2, -off)) * f.out);
+                        o.v[j] = (T)(__builtin_amdgcn_exp2f(__builtin_fmaf(v.value(r, j), f.l2, -off)) * out);
                     o.store((T *)((char *)g + (unsigned)i * 16u), N);
                 }
                 if constexpr (kLoop) v.load(r, zn, limit);
@@ -581,15 +587,23 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void distill_row_kernel(co
                     Piece<T> o;
 #pragma unroll
                     for (int j = 0; j < N; ++j)
-                        o.v[j] = (T)(__builtin_amdgcn_exp2f(__builtin_fmaf(V::value(q.w, j), f.l2, -off)) * f.out);
+                        o.v[j] = (T)(__builtin_amdgcn_exp2f(__builtin_fmaf(V::value(q.w, j), f.l2, -off)) * out);
                     o.store((T *)((char *)g + (unsigned)i * 16u), N);
                 }
             if (t < v.more)
-                g[v.whole * N + t] = (T)(__builtin_amdgcn_exp2f(__builtin_fmaf(v.rest, f.l2, -off)) * f.out);
+                g[v.whole * N + t] = (T)(__builtin_amdgcn_exp2f(__builtin_fmaf(v.rest, f.l2, -off)) * out);
         } else {
-            if (p.grad)
-                for (int i = t; i < p.classes; i += TEAM)
-                    g[i] = (T)(n_inside > 0 ? __builtin_amdgcn_exp2f(((float)z[i] - f.osub) * f.l2) * f.out : 0.0f);
+            if (p.grad) {
+                const float from = slow ? f.osub : 0.0f;   // (off is 0 of a row that took its own maximum)
+                int e = (int)(__builtin_bit_cast(unsigned long long, f.out) >> 52 & 0x7FF) - 1023;
+                e = e < -252 ? -252 : (e > 252 ? 252 : e);
+                const float half = u2f((uint32_t)(127 + e / 2) << 23);
+                const float rest = (float)(f.out * __builtin_bit_cast(double, (unsigned long long)(1023 - e / 2) << 52));
+                for (int i = t; i < p.classes; i += TEAM) {
+                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf((float)z[i] - from, f.l2, -f.off));
+                    g[i] = (T)(n_inside > 0 ? x * half * rest : 0.0f);
+                }
+            }
             if constexpr (kLoop)
 #pragma unroll
                 for (int r = 0; r < R; ++r) v.load(r, zn, limit);
@@ -745,7 +759,7 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const DistArgs p)
         const int j = l + G * i;
         if (j >= p.classes) continue;
         const float o = (in >> i & 1u) ? (float)((double)f.c * ((double)f.share(x[i]) * f.whole - q_at[i]))
-                                       : __builtin_amdgcn_exp2f((x[i] - f.osub) * f.l2) * f.out;
+                                       : __builtin_amdgcn_exp2f((x[i] - f.osub) * f.l2) * (float)f.out;
         g[j] = (T)o;
     }
 }
@@ -922,13 +936,14 @@ __global__ __launch_bounds__(kSegThreads) void distill_segment_kernel(const Dist
                                      all.outside > 0);
     if (t == 0 && seg == 0) p.loss[row] = (float)loss;
     if (!p.grad) return;
+    const float out = (float)f.out;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const int at = (r * kSegThreads + t) * P::N;
         P o;
 #pragma unroll
         for (int i = 0; i < P::N; ++i)
-            o.v[i] = (T)(__builtin_amdgcn_exp2f(((float)x[r].v[i] - f.osub) * f.l2) * f.out);
+            o.v[i] = (T)(__builtin_amdgcn_exp2f(((float)x[r].v[i] - f.osub) * f.l2) * out);
         o.store(g + at, here - at);
     }
     __syncthreads();

@@ -84,3 +84,34 @@ def test_distill_bucket_masked_whole(n, v, k, dtype):
         assert (got[1][row][~inside[row]] == 0).all()
     alone = fda.distill_topk_batch(z, values, index, temperature=tau, teacher_lse=lse)
     assert torch.equal(alone, got[0])
+
+
+# ------------------------------------------------------------------------------- distillation: classes far from the teacher's
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("n,v,k", [(12, 7, 3), (12, 60, 5), (12, 200, 9), (12, 700, 70), (12, 3001, 5), (12, 9001, 5), (12, 30000, 8),
+                                   (64, 140001, 6), (12, 210001, 6)])
+def test_distill_classes_far_from_the_teachers(n, v, k, tail, dtype):
+    """A class that the teacher does not name 0 to 90 above those it does, or all of them far below, with rows' weights that
+    float32 holds and their products with such a row's largest exponential, or its inverse, does not."""
+    import face_detection_amd as fda
+    z, values, index, lse = distill_inputs(n, v, k, dtype, seed=5, tail=tail)
+    inside = torch.zeros(n, v, dtype=torch.bool).scatter_(1, index, True)
+    if tail:
+        lse = lse + 0.5
+    for row, above in enumerate((0, 40, 60, 75, 80, 83, 90)):
+        at = int((~inside[row]).nonzero()[-1 - row % 2])
+        z[row, at] = z[row, index[row]].max() + above
+    for row, below in ((7, 30), (8, 39), (9, 45)):
+        z[row] = torch.where(inside[row], z[row], z[row] - below)
+    z, values, index = z.cuda(), values.cuda(), index.cuda()
+    lse = lse.cuda() if tail else None
+    # float16 holds no gradients of the smallest weights, and none of the largest
+    for weight in (1.0, 2e-6, 1e-9, 1e-12, 1e-30) + (() if dtype == torch.float16 else (1e22, 3e37)):
+        g = torch.full((n,), weight, device="cuda")
+        want, off = O.distill(z, values, index, 1.0, lse, g)
+        got = fda.distill_topk_batch(z, values, index, teacher_lse=lse, grad_loss=g, return_grad=True)
+        within(got[0], want[0], off[0], "loss")
+        # 2^-126: an exponential below it is 0, relative to the row's largest one or to the teacher's classes'
+        within(got[1], want[1], off[1] + 2.0 ** -126 * weight, "grad at weight %g" % weight)
