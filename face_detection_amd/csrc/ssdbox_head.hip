@@ -831,16 +831,17 @@ struct JoinArgs {
     void *out;
     long long ldo;
     const int *row_of;
+    long long first;                  // the launch's first workgroup of the product's
 };
 
 // The parts of a product over a long k, added in a fixed order: reads from the caches (128 parts of 256 x 512: 67 MB
 // in 13 us).  Four values a lane, eight parts on their way at a time; up to WAVES waves share the parts of 256 values.
 template <typename T, int WAVES>
-SSD_DEV void join(const JoinArgs &p, int block, f32x4 (&s_sum)[WAVES > 1 ? WAVES : 1][64])
+SSD_DEV void join(const JoinArgs &p, long long block, f32x4 (&s_sum)[WAVES > 1 ? WAVES : 1][64])
 {
     constexpr int kPieces = WAVES < 4 ? 4 / WAVES : 1;
     const int across = (p.m + 255) / 256, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long id = (long long)block * kPieces + (WAVES > 1 ? 0 : wave);
+    const long long id = (block + p.first) * kPieces + (WAVES > 1 ? 0 : wave);
     const int n = (int)(id / across), m = ((int)(id % across) * 64 + lane) * 4;
     const bool in = n < (p.n_count ? *p.n_count : p.n) && m < p.m;
     f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -946,6 +947,7 @@ int whole_tile(long long m, long long n, int es)
 }
 
 constexpr int kPartBytes = 128 << 20;  // of a product's parts together
+constexpr long long kJoinBlocks = 1 << 20;    // workgroups of one join
 
 // The tile of a product whose k may be cut, and into how many parts: so that the chip is filled, at least eight stages each.
 // The largest tile does what it computes about 1.45 times as fast as the next one, so it may not compute more than that many
@@ -1121,24 +1123,54 @@ JoinArgs join_args(const GradArgs &a)
     return j;
 }
 
+// Workgroups of the whole join of a product by WAVES waves.
+template <int WAVES>
+long long join_blocks(const JoinArgs &j)
+{
+    const long long pieces = (long long)j.n * ((j.m + 255) / 256), each = WAVES < 4 ? 4 / WAVES : 1;
+    return (pieces + each - 1) / each;
+}
+
 template <typename T, int WAVES>
 void launch_join(const HeadCall &c, const JoinArgs &a, const JoinArgs &b)
 {
-    const auto blocks = [](const JoinArgs &j) {
-        const long long pieces = (long long)j.n * ((j.m + 255) / 256), each = WAVES < 4 ? 4 / WAVES : 1;
-        return (unsigned)((pieces + each - 1) / each);
-    };
-    launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_join_kernel<T, WAVES>, dim3(blocks(a) + blocks(b)),
-                 dim3(WAVES < 4 ? 256 : WAVES * 64), a, b, (int)blocks(a));
+    const unsigned blocks = (unsigned)join_blocks<WAVES>(a);
+    launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_join_kernel<T, WAVES>, dim3(blocks + (unsigned)join_blocks<WAVES>(b)),
+                 dim3(WAVES < 4 ? 256 : WAVES * 64), a, b, (int)blocks);
 }
 
-// One product's parts, or two's (b NULL: one's).
-template <typename T>
-void launch_join(const HeadCall &c, const GradArgs &a, const GradArgs *b)
+// One product's parts by themselves, so many workgroups a launch that it stays far below 2^32 threads.
+template <typename T, int WAVES>
+void launch_join(const HeadCall &c, JoinArgs a)
 {
-    const JoinArgs x = join_args(a), y = b ? join_args(*b) : JoinArgs{};
+    const long long all = join_blocks<WAVES>(a);
+    for (; a.first < all; a.first += kJoinBlocks) {
+        const unsigned blocks = (unsigned)(all - a.first < kJoinBlocks ? all - a.first : kJoinBlocks);
+        launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_join_kernel<T, WAVES>, dim3(blocks), dim3(WAVES < 4 ? 256 : WAVES * 64), a,
+                     JoinArgs{}, (int)blocks);
+    }
+}
+
+template <typename T>
+void launch_join(const HeadCall &c, const GradArgs &a)
+{
+    const JoinArgs x = join_args(a);
+    if (x.waves == 1) launch_join<T, 1>(c, x);
+    else if (x.waves == 4) launch_join<T, 4>(c, x);
+    else launch_join<T, 16>(c, x);
+}
+
+// Two products' parts, in one launch where it is no long one.
+template <typename T>
+void launch_join(const HeadCall &c, const GradArgs &a, const GradArgs &b)
+{
+    const JoinArgs x = join_args(a), y = join_args(b);
     const int waves = x.waves > y.waves ? x.waves : y.waves;
-    if (waves == 1) launch_join<T, 1>(c, x, y);
+    if (join_blocks<4>(x) + join_blocks<4>(y) > kJoinBlocks) {    // (a piece each: the most that any number of waves takes)
+        launch_join<T>(c, a);
+        launch_join<T>(c, b);
+    }
+    else if (waves == 1) launch_join<T, 1>(c, x, y);
     else if (waves == 4) launch_join<T, 4>(c, x, y);
     else launch_join<T, 16>(c, x, y);
 }
@@ -1159,14 +1191,15 @@ void launch_gradients(const HeadCall &c, const HeadPlan &q, GradArgs h, GradArgs
             launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_both_kernel<T, 64, 4, 1>, dim3(hb + wb), dim3(256), h, w, (int)hb);
         else
             launch_stage(c.ctx, SSDBOX_STAGE_LOSS, head_both_kernel<T, 128, 2, 2>, dim3(hb + wb), dim3(256), h, w, (int)hb);
-        if (join_h) launch_join<T>(c, h, join_w ? &w : nullptr);
-        else if (join_w) launch_join<T>(c, w, nullptr);
+        if (join_h && join_w) launch_join<T>(c, h, w);
+        else if (join_h) launch_join<T>(c, h);
+        else if (join_w) launch_join<T>(c, w);
         return;
     }
     if (want_h) launch_product<T, true, false>(c, q.dh_tile, h);
-    if (join_h) launch_join<T>(c, h, nullptr);
+    if (join_h) launch_join<T>(c, h);
     if (want_w) launch_product<T, true, true>(c, q.dw_tile, w);
-    if (join_w) launch_join<T>(c, w, nullptr);
+    if (join_w) launch_join<T>(c, w);
 }
 
 template <typename T>
@@ -1434,8 +1467,7 @@ extern "C" int ssdbox_linear_cross_entropy(ssdbox_ctx *ctx, const void *d_hidden
                     ((uintptr_t)d_grad_hidden % 16) == 0 && ((uintptr_t)d_grad_weight % 16) == 0,
                 "linear_cross_entropy: weight and gradients have to start at 16 bytes, the workspace at 256");
     SSD_REQUIRE(q.class_tiles * ((rows + q.bn - 1) / q.bn) < (1ll << 31) &&
-                    (q.pieces == 0 || (dim + 127) / 128 * ((rows + 63) / 64) * q.dh_parts < (1ll << 31)) &&
-                    (d_grad_hidden == nullptr || (dim + 255) / 256 * rows <= kMostRows * 4),
+                    (q.pieces == 0 || (dim + 127) / 128 * ((rows + 63) / 64) * q.dh_parts < (1ll << 31)),
                 "linear_cross_entropy: %lld rows x %lld classes", (long long)rows, (long long)classes);
 
     DeviceGuard guard(ctx->device);

@@ -17,8 +17,9 @@ def tiniest(dtype):
     return torch.finfo(dtype).smallest_normal * half_step(dtype)
 
 
-def head(hidden, weight, labels, scale=1.0, smoothing=0.0, grad_loss=None):
-    """loss, grad_hidden, grad_weight and a bound of each one's error (same shapes)."""
+def head(hidden, weight, labels, scale=1.0, smoothing=0.0, grad_loss=None, most=None, links=None):
+    """loss, grad_hidden, grad_weight and a bound of each one's error (same shapes).  Of some rows of a longer batch, the bounds
+    take the largest |grad_loss| of its counted rows (most) and the additions in a sum over its rows (links)."""
     dtype = hidden.dtype
     h, w = hidden.double(), weight.double()
     n, v, dim = h.shape[0], w.shape[0], h.shape[1]
@@ -46,12 +47,12 @@ def head(hidden, weight, labels, scale=1.0, smoothing=0.0, grad_loss=None):
     off_p = torch.where(one > 0, (1 - p), p) * (3 * spread + off_z + 16 * U).expm1() + 4 * U * smoothing
     off_d = off_p * c.abs()
     if dtype != torch.float32:
-        off_d = off_d * (1 + 2 * half_step(dtype)) + half_step(dtype) * d.abs() + 2.0 ** -38 * c.abs().amax()
+        off_d = off_d * (1 + 2 * half_step(dtype)) + half_step(dtype) * d.abs() + 2.0 ** -38 * (c.abs().amax() if most is None else most * scale)
     else:
         off_d = off_d + 4 * U * d.abs()
     gh, gw = d @ w, d.t() @ h
     off_h = off_d @ w.abs() + (v + 8) * U * ((d.abs() + off_d) @ w.abs())
-    off_w = off_d.t() @ h.abs() + (n + 8) * U * ((d.abs() + off_d).t() @ h.abs())
+    off_w = off_d.t() @ h.abs() + (n + 8 if links is None else links) * U * ((d.abs() + off_d).t() @ h.abs())
     off_h = off_h * (1 + 2 * half_step(dtype)) + half_step(dtype) * gh.abs() + tiniest(dtype)
     off_w = off_w * (1 + 2 * half_step(dtype)) + half_step(dtype) * gw.abs() + tiniest(dtype)
     return (loss, gh, gw), (off, off_h, off_w)

@@ -115,3 +115,49 @@ def test_distill_classes_far_from_the_teachers(n, v, k, tail, dtype):
         within(got[0], want[0], off[0], "loss")
         # 2^-126: an exponential below it is 0, relative to the row's largest one or to the teacher's classes'
         within(got[1], want[1], off[1] + 2.0 ** -126 * weight, "grad at weight %g" % weight)
+
+
+# ---------------------------------------------------------------------------------------------- head: many rows, many pieces
+def long_inputs(n, v, dim, dtype, seed=0, ignored=0.1):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    weight = (torch.randn(v, dim, generator=g, device="cuda") * (2.0 / math.sqrt(dim))).to(dtype)
+    hidden = torch.empty(n, dim, device="cuda", dtype=dtype)
+    for a in range(0, n, 1 << 19):
+        hidden[a:a + (1 << 19)] = torch.randn(min(1 << 19, n - a), dim, generator=g, device="cuda").to(dtype)
+    labels = torch.randint(0, v, (n,), generator=g, device="cuda")
+    weights = torch.rand(n, generator=g, device="cuda") + 0.5
+    labels[torch.rand(n, generator=g, device="cuda") < ignored] = -100
+    return hidden, weight, labels, weights
+
+
+def rows_against_the_oracle(got, hidden, weight, labels, weights, scale=1.0, smoothing=0.0, ends=None, logits=1 << 23):
+    """A long batch's results, some rows at a time; with ends only the loss and the hidden rows' gradient of so many rows at
+    either end."""
+    n, v = len(labels), len(weight)
+    step = max(1, logits // v)
+    # a sum over n rows: n additions, whose rounding errors go either way: sqrt(n) of them, eight times over
+    links = 8 * math.sqrt(n) + 64
+    most = float(weights[labels >= 0].abs().max())
+    want_w, off_w = torch.zeros(weight.shape, device="cuda", dtype=torch.float64), 0.0
+    for a in range(0, n, step):
+        b = min(a + step, n)
+        if ends is not None and ends <= a and b <= n - ends:
+            continue
+        (loss, gh, gw), (off, off_h, off_gw) = O.head(hidden[a:b], weight, labels[a:b], scale, smoothing, weights[a:b], most, links)
+        within(got[0][a:b], loss, off, "loss of rows %d to %d" % (a, b))
+        within(got[1][a:b], gh, off_h, "grad_hidden of rows %d to %d" % (a, b))
+        if ends is None:
+            want_w += gw
+            off_w = off_w + off_gw
+    if ends is None:
+        within(got[2], want_w, off_w, "grad_weight")
+
+
+@gpu
+@pytest.mark.parametrize("n,v,dim,ends", [(8500000, 300, 260, 200000), (1400000, 600, 770, None)])
+def test_head_joins_of_many_rows(n, v, dim, ends):
+    """Gradients of the hidden rows joined from parts or over pieces by more workgroups than one launch takes."""
+    import face_detection_amd as fda
+    hidden, weight, labels, weights = long_inputs(n, v, dim, torch.bfloat16)
+    got = fda.linear_cross_entropy_batch(hidden, weight, labels, grad_loss=weights, return_grad=True)
+    rows_against_the_oracle(got, hidden, weight, labels, weights, ends=ends)
