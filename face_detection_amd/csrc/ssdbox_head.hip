@@ -61,7 +61,8 @@ struct PrepArgs {
     int dim, pitch;
     int *block_count;                 // counted rows and largest |grad_loss| of every kCountRows rows, or NULL
     float *block_max;
-    int *place_count;                 // the number of counted rows
+    int *place_count;                 // the number of counted rows; behind it, of more than one chunk, each chunk's
+    int chunks, chunk_rows;
     int *row, *label;                 // per counted row: the row it was, its class
     HeadScale *scale;
     float *loss;
@@ -225,7 +226,12 @@ __global__ __launch_bounds__(kRowThreads) void head_prep_kernel(const PrepArgs p
                 p.loss[n] = lab < 0 ? 0.0f : u2f(0x7FC00000u);
             }
             if (t < kRowsEach) s_place[t] = counted ? at : -1;
-            if (t == 0 && first + kRowsEach >= p.rows) *p.place_count = before + __popcll(bal);
+            if (t == 0 && first + kRowsEach >= p.rows) {
+                const int all = before + __popcll(bal);
+                *p.place_count = all;
+                if (p.chunks > 1)
+                    for (int i = 0; i < p.chunks; ++i) p.place_count[1 + i] = min(max(all - i * p.chunk_rows, 0), p.chunk_rows);
+            }
         }
     }
     __syncthreads();
@@ -907,13 +913,16 @@ struct HeadPlan {
     long long class_tiles, slots;
     long long piece, ld_delta;        // classes a piece, and from one row of its d to the next
     int pieces;
+    int chunks;                       // of counted rows, whose d of a piece is there at a time
+    long long chunk_rows;
     int dh_parts, dw_parts;
     size_t o_few, o_blocks, o_rows, o_weight, o_row, o_label, o_count, o_scale, o_stat, o_sumz, o_zl, o_out, o_delta, o_kept, o_dh,
         o_dw;
     size_t bytes;
 };
 
-constexpr size_t kDeltaBytes = (size_t)1 << 31;    // of one piece's d
+constexpr size_t kDeltaBytes = (size_t)1 << 31;    // of one piece's d (its rows' padding, up to a quarter, comes on top)
+constexpr long long kChunkRow = 8192;              // bytes of a row of d at most, where rows are cut
 
 // From which dim on something is kept.  Measured (rows x classes x dim, taken again, kept; us):
 //   bfloat16  1000 x 30000 x 128 140 141,  60 x 200000 x 256 116 107,  256 x 1000003 x 512 1710 1540,  8192 x 131072 x 768 6360 5560
@@ -995,6 +1004,8 @@ HeadPlan make_plan(long long rows, long long classes, long long dim, long long w
     q.class_tiles = (classes + q.bm - 1) / q.bm;
     q.slots = q.class_tiles * (q.bm / q.each);
     const bool grad = grad_hidden || grad_weight;
+    q.chunks = 1;
+    q.chunk_rows = rows;
     if (grad) {
         const long long row_bytes = rows * q.es > 0 ? rows * q.es : 1;
         long long most = (long long)kDeltaBytes / row_bytes / 256 * 256;
@@ -1007,15 +1018,29 @@ HeadPlan make_plan(long long rows, long long classes, long long dim, long long w
         // 256 bytes more than the piece, often a power of two: the rows that one store or load touches would otherwise all
         // lie in one channel of the L2 (d of 8192 x 65536: 2.2 -> 1.9 ms)
         q.ld_delta = q.piece + 256 / q.es;
+        if (q.few_parts) {
+            if ((size_t)(rows * q.ld_delta) * q.es > kDeltaBytes) q.ld_delta = (classes + 63) / 64 * 64;
+        } else if (rows * (256 * q.es + 256) > (long long)kDeltaBytes) {
+            // So many rows that a piece of any width is too much: they are cut, too.  dW is added over the chunks, which costs
+            // less than dH over pieces, so pieces are wide again (ms, pieces of 256 classes of all rows, of 1024, 2048, 4096 of
+            // chunks:  2000000 x 4000 x 64 float32 70.2 67.4 67.8 77.6,  3000000 x 4000 x 64 bfloat16 43.9 37.5 35.7 33.6).
+            const long long widest = kChunkRow / q.es;
+            q.pieces = (int)((whole + widest - 1) / widest);
+            q.piece = ((whole + q.pieces - 1) / q.pieces + 255) / 256 * 256;
+            q.pieces = (int)((whole + q.piece - 1) / q.piece);
+            q.ld_delta = q.piece + 256 / q.es;
+            q.chunk_rows = (long long)kDeltaBytes / (q.ld_delta * q.es) / 256 * 256;
+            q.chunks = (int)((rows + q.chunk_rows - 1) / q.chunk_rows);
+        }
         // The pass over what is kept and its stores move bytes, the products it spares take 2 dim operations a logit.
-        if (q.few_parts) q.keep = false;
+        if (q.few_parts || q.chunks > 1) q.keep = false;
         else if (dtype == SSDBOX_DTYPE_F32) q.keep = true;
         else if (dtype == SSDBOX_DTYPE_BF16) q.keep = dim > kKeepAboveBf16;
         else q.keep = dim > kKeepAboveF16 && q.pieces == 1 && (size_t)(rows * q.ld_delta) * 4 <= kDeltaBytes;
     }
     size_t at = 0;
     q.o_few = put(at, (size_t)q.few_parts * rows * q.few_ld * 4);
-    q.o_count = put(at, 256);
+    q.o_count = put(at, (1 + (q.chunks > 1 ? q.chunks : 0)) * 4);
     q.o_scale = put(at, 256);
     q.o_blocks = put(at, rows > kCountFrom ? (rows + kCountRows - 1) / kCountRows * 8 : 0);
     q.o_row = put(at, rows * 4);
@@ -1026,13 +1051,13 @@ HeadPlan make_plan(long long rows, long long classes, long long dim, long long w
     q.o_stat = put(at, q.few_parts ? 0 : (size_t)rows * q.slots * sizeof(float2));
     q.o_sumz = put(at, smoothing != 0.0f && !q.few_parts ? (size_t)rows * q.slots * 4 : 0);
     q.o_weight = put(at, q.copy_weight ? (size_t)classes * q.pitch * q.es : 0);
-    q.o_delta = put(at, grad ? (size_t)rows * q.ld_delta * q.es : 0);
+    q.o_delta = put(at, grad ? (size_t)q.chunk_rows * q.ld_delta * q.es : 0);
     q.o_kept = put(at, q.keep && dtype == SSDBOX_DTYPE_F16 ? (size_t)rows * q.ld_delta * 4 : 0);
     const long long wide = (dim + 3) / 4 * 4, piece_classes = classes < q.piece ? classes : q.piece;
     if (grad) {
-        cut_tile(dim, rows, (q.piece + bk - 1) / bk, q.es, false, q.dh_tile, q.dh_parts);
-        cut_tile(dim, piece_classes, (rows + bk - 1) / bk, q.es, true, q.dw_tile, q.dw_parts);
-        const long long h = rows > 0 ? tiles(q.dh_tile, dim, rows) : 1, w = tiles(1, dim, piece_classes);
+        cut_tile(dim, q.chunk_rows, (q.piece + bk - 1) / bk, q.es, false, q.dh_tile, q.dh_parts);
+        cut_tile(dim, piece_classes, (q.chunk_rows + bk - 1) / bk, q.es, true, q.dw_tile, q.dw_parts);
+        const long long h = rows > 0 ? tiles(q.dh_tile, dim, q.chunk_rows) : 1, w = tiles(1, dim, piece_classes);
         if (q.dh_tile < 2 && q.dw_tile < 2 && w < 512) {
             // one launch for both, at two workgroups a compute unit: dW takes half, or its tiles, dH what is left (each cut as
             // if alone, 1000 x 1000 x 2048 bfloat16 takes 70 us and not 55, 61 x 10007 x 512 float32 64 and not 59)
@@ -1045,7 +1070,7 @@ HeadPlan make_plan(long long rows, long long classes, long long dim, long long w
         if (!grad_hidden) q.dh_parts = 0;
         if (!grad_weight) q.dw_parts = 0;
         q.o_dh = put(at, grad_hidden && (q.dh_parts > 1 || q.pieces > 1) ? (size_t)q.dh_parts * rows * wide * 4 : 0);
-        q.o_dw = put(at, q.dw_parts > 1 ? (size_t)q.dw_parts * q.piece * wide * 4 : 0);
+        q.o_dw = put(at, q.dw_parts > 1 || (q.dw_parts && q.chunks > 1) ? (size_t)q.dw_parts * q.piece * wide * 4 : 0);
     }
     q.bytes = at;
     return q;
@@ -1226,6 +1251,8 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
     s.dim = (int)c.dim;
     s.pitch = q.pitch;
     s.place_count = count;
+    s.chunks = q.chunks;
+    s.chunk_rows = (int)q.chunk_rows;
     s.row = row;
     s.label = label;
     s.scale = scale;
@@ -1334,10 +1361,13 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
     if (!grad) return SSDBOX_OK;
 
     const long long wide = (c.dim + 3) / 4 * 4;
-    for (int turn = 0; turn < q.pieces; ++turn) {
-        const int i = q.keep ? q.pieces - 1 - turn : turn;       // what is kept has to be used before its place is
-        const long long first = i * q.piece;
+    for (int turn = 0; turn < q.pieces * q.chunks; ++turn) {
+        const int piece = turn / q.chunks, chunk = turn % q.chunks;
+        const int i = q.keep ? q.pieces - 1 - piece : piece;     // what is kept has to be used before its place is
+        const long long first = i * q.piece, row0 = chunk * q.chunk_rows;
         const int n_class = (int)(c.classes - first < q.piece ? c.classes - first : q.piece);
+        const int n_rows = (int)(c.rows - row0 < q.chunk_rows ? c.rows - row0 : q.chunk_rows);
+        const int *counted = q.chunks > 1 ? count + 1 + chunk : count;
         T *delta = (T *)(c.ws + q.o_delta);
         if (q.few_parts) {
             // d is there: few tiles are one piece
@@ -1362,6 +1392,10 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
         } else if (c.rows > 0) {
             LogitArgs d = l;
             d.weight = weight + first * ldw;
+            d.rows = rows + row0 * q.pitch;
+            d.count = counted;
+            d.label = label + row0;
+            d.row = l.row + row0;
             d.classes = n_class;
             d.first = (int)first;
             d.tiles = (n_class + q.bm - 1) / q.bm;
@@ -1381,33 +1415,34 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
         if (want_h) {
             h.a = weight + first * ldw;
             h.lda = ldw;
-            h.n = (int)c.rows;
-            h.n_count = q.direct ? nullptr : count;
+            h.n = n_rows;
+            h.n_count = q.direct ? nullptr : counted;
             h.k = n_class;
             h.parts = q.dh_parts;
             h.out = c.grad_hidden;
-            h.row_of = row;
+            h.row_of = row + row0;
             if (q.dh_parts > 1 || q.pieces > 1) {
-                h.part = (float *)(c.ws + q.o_dh);
+                h.part = (float *)(c.ws + q.o_dh) + row0 * wide;
                 h.ld_part = wide;
                 h.part_stride = c.rows * wide;
-                h.add = turn > 0;
-                join_h = turn == q.pieces - 1;
+                h.add = piece > 0;
+                join_h = piece == q.pieces - 1;
             }
         }
         if (c.grad_weight) {
-            w.a = rows;
+            w.a = rows + row0 * q.pitch;
             w.lda = q.pitch;
             w.n = n_class;
-            w.k = (int)c.rows;
-            w.k_count = q.direct ? nullptr : count;
+            w.k = n_rows;
+            w.k_count = q.direct ? nullptr : counted;
             w.parts = q.dw_parts;
             w.out = (T *)c.grad_weight + first * c.dim;
-            if (q.dw_parts > 1) {
+            if (q.dw_parts > 1 || q.chunks > 1) {
                 w.part = (float *)(c.ws + q.o_dw);
                 w.ld_part = wide;
                 w.part_stride = q.piece * wide;
-                join_w = true;
+                w.add = chunk > 0;
+                join_w = chunk == q.chunks - 1;
             }
         }
         launch_gradients<T>(c, q, h, w, want_h, c.grad_weight != nullptr, join_h, join_w);

@@ -1,10 +1,12 @@
 """The classifier losses where their definitions reach a limit: a rest bucket that the student masks whole, classes far above
 the teacher's, many rows, gradients in several pieces.  Bounds as in tests/test_classifier_losses.py."""
+import ctypes
 import math
 
 import pytest
 import torch
 
+from face_detection_amd import _lib
 from oracle import classifier_oracle as O
 from test_classifier_losses import TYPES, distill_inputs, within
 
@@ -130,6 +132,15 @@ def long_inputs(n, v, dim, dtype, seed=0, ignored=0.1):
     return hidden, weight, labels, weights
 
 
+def within_there(got, want, off, what):
+    """within() on the GPU: such results are large.  Sums beyond float16's range are infinite there."""
+    assert got.shape == want.shape and not torch.isnan(got).any(), what
+    most = torch.finfo(got.dtype).max
+    over = torch.where((want.abs() + off > most) & (got == want.sign() * INF), 0.0, (got.double() - want).abs() - off)
+    assert not (over > 0).any(), "%s: %d of %d values off by more than the bound, the worst by %.3g" % (
+        what, int((over > 0).sum()), over.numel(), float(over.max()))
+
+
 def rows_against_the_oracle(got, hidden, weight, labels, weights, scale=1.0, smoothing=0.0, ends=None, logits=1 << 23):
     """A long batch's results, some rows at a time; with ends only the loss and the hidden rows' gradient of so many rows at
     either end."""
@@ -144,13 +155,13 @@ def rows_against_the_oracle(got, hidden, weight, labels, weights, scale=1.0, smo
         if ends is not None and ends <= a and b <= n - ends:
             continue
         (loss, gh, gw), (off, off_h, off_gw) = O.head(hidden[a:b], weight, labels[a:b], scale, smoothing, weights[a:b], most, links)
-        within(got[0][a:b], loss, off, "loss of rows %d to %d" % (a, b))
-        within(got[1][a:b], gh, off_h, "grad_hidden of rows %d to %d" % (a, b))
+        within_there(got[0][a:b], loss, off, "loss of rows %d to %d" % (a, b))
+        within_there(got[1][a:b], gh, off_h, "grad_hidden of rows %d to %d" % (a, b))
         if ends is None:
             want_w += gw
             off_w = off_w + off_gw
     if ends is None:
-        within(got[2], want_w, off_w, "grad_weight")
+        within_there(got[2], want_w, off_w, "grad_weight")
 
 
 @gpu
@@ -161,3 +172,39 @@ def test_head_joins_of_many_rows(n, v, dim, ends):
     hidden, weight, labels, weights = long_inputs(n, v, dim, torch.bfloat16)
     got = fda.linear_cross_entropy_batch(hidden, weight, labels, grad_loss=weights, return_grad=True)
     rows_against_the_oracle(got, hidden, weight, labels, weights, ends=ends)
+
+
+@pytest.mark.parametrize("dtype,size", [(_lib.DTYPE_F32, 4), (_lib.DTYPE_F16, 2), (_lib.DTYPE_BF16, 2)])
+def test_head_workspace_is_bounded(dtype, size):
+    """Of the logits' gradient 2 GiB, with their rows' padding 2.5, and of float16's products as much, however rows and classes
+    are distributed; beside them a copy of the rows, their statistics, and sums of a gradient in float32."""
+    need = ctypes.c_size_t()
+    for rows, classes, dim in ((4200000, 2, 8), ((1 << 24) - 1, 10, 8), (9000000, 300, 300), (1 << 23, 1, 8), ((1 << 23) // 65, 65, 16),
+                               (3000000, 5000, 64), (1700000, 40, 8), (1300000, 300, 8), (1 << 20, 1030, 64), (1 << 17, 1 << 18, 64),
+                               ((1 << 24) - 1, 1 << 15, 8), (600000, 2000, 512), (20000, 1000003, 512), (1, 1 << 28, 16)):
+        for grad_hidden, grad_weight in ((1, 1), (1, 0), (0, 1)):
+            _lib.check(_lib.load().ssdbox_linear_cross_entropy_workspace(rows, classes, dim, dim, dtype, 0.1, grad_hidden, grad_weight,
+                                                                         ctypes.byref(need)))
+            most = 2.5 * 2 ** 30 * (2 if dtype == _lib.DTYPE_F16 else 1)
+            most += rows * (dim * size + 32 + (classes / 32 + 8) * 12 + grad_hidden * (dim + 4) * 4) + 2 ** 29
+            assert need.value <= most, (rows, classes, dim, need.value / 2 ** 30, most / 2 ** 30)
+
+
+# one chunk's border within the batch's counted rows, or behind them; pieces and chunks; so few classes that nothing is cut
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("n,v,dim,ignored,smoothing", [(3400000, 270, 16, 0.1, 0.1), (3400000, 40, 33, 0.6, 0.0),
+                                                       (2900000, 4200, 8, 0.84, 0.0), (8000000, 1, 4, 0.1, 0.1)])
+def test_head_of_many_rows(n, v, dim, ignored, smoothing, dtype):
+    import face_detection_amd as fda
+    hidden, weight, labels, weights = long_inputs(n, v, dim, dtype, ignored=ignored)
+    # float16: so large that hidden rows' gradients are no subnormals, and so small that the weight's are finite
+    for factor in (2.0 ** 9, 2.0 ** -8) if dtype == torch.float16 else (1.0,):
+        weights *= factor
+        got = fda.linear_cross_entropy_batch(hidden, weight, labels, logit_scale=2.0, label_smoothing=smoothing, grad_loss=weights,
+                                             return_grad=True)
+        rows_against_the_oracle(got, hidden, weight, labels, weights, 2.0, smoothing)
+    assert dtype != torch.float16 or torch.isfinite(got[2]).any()
+    frozen = fda.linear_cross_entropy_batch(hidden, weight, labels, logit_scale=2.0, label_smoothing=smoothing, grad_loss=weights,
+                                            return_grad=True, weight_grad=False)
+    assert torch.equal(frozen[0], got[0]) and torch.equal(frozen[1], got[1])
