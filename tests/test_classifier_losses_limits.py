@@ -208,3 +208,26 @@ def test_head_of_many_rows(n, v, dim, ignored, smoothing, dtype):
     frozen = fda.linear_cross_entropy_batch(hidden, weight, labels, logit_scale=2.0, label_smoothing=smoothing, grad_loss=weights,
                                             return_grad=True, weight_grad=False)
     assert torch.equal(frozen[0], got[0]) and torch.equal(frozen[1], got[1])
+
+
+# largest tiles, with what is kept of them and without, and several pieces, of which float32 and bfloat16 above dim 192 keep the last
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("n,v,dim", [(600, 30000, 400), (600, 30000, 72), (1100, 33000, 137), (67000, 16700, 24), (40000, 30000, 130),
+                                     (67000, 16700, 520)])
+def test_head_large_tiles_and_pieces(n, v, dim, dtype):
+    import face_detection_amd as fda
+    hidden, weight, labels, weights = long_inputs(n, v, dim, dtype, ignored=0.2)
+    if dtype == torch.float16:
+        weights *= 64
+    hidden[labels < 0] = float("nan")
+    got = fda.linear_cross_entropy_batch(hidden, weight, labels, logit_scale=1.5, label_smoothing=0.1, grad_loss=weights,
+                                         return_grad=True)
+    rows_against_the_oracle(got, hidden, weight, labels, weights, 1.5, 0.1)
+    alone = fda.linear_cross_entropy_batch(hidden, weight, labels, logit_scale=1.5, label_smoothing=0.1)
+    frozen = fda.linear_cross_entropy_batch(hidden, weight, labels, logit_scale=1.5, label_smoothing=0.1, grad_loss=weights,
+                                            return_grad=True, weight_grad=False)
+    assert torch.equal(alone, got[0]) and torch.equal(frozen[0], got[0]) and torch.equal(frozen[1], got[1])
+    # the mean, without smoothing
+    plain = fda.linear_cross_entropy_batch(hidden, weight, labels, logit_scale=1.5, return_grad=True)
+    rows_against_the_oracle(plain, hidden, weight, labels, torch.full((n,), 1.0 / n, device="cuda"), 1.5)
