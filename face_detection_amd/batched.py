@@ -16,7 +16,7 @@ import math
 import numpy as np
 
 from . import _lib
-from .runtime import (AnchorGrid, Session, _is_tf_tensor, _is_torch_tensor, _ptr, _torch, _torch_device,
+from .runtime import (AnchorGrid, DevArray, Session, _is_tf_tensor, _is_torch_tensor, _ptr, _torch, _torch_device,
                       _torch_if_loaded)
 
 
@@ -294,12 +294,19 @@ def _distill_bytes(*sizes):
 def _float_rows(sess, x, name, max_ld=None):
     """A float32 / float16 / bfloat16 array as rows of its last axis: (array, family, rows, row stride,
     SSDBOX_DTYPE code, type).  Rows of a CUDA tensor may lie further apart than they are long."""
-    if _is_torch_tensor(x):
+    family, in_torch = "torch", _is_torch_tensor(x)
+    if not in_torch:
+        dtype = np.dtype(x.dtype.as_numpy_dtype) if _is_tf_tensor(x) else x.dtype if isinstance(x, np.ndarray) else None
+        if dtype is not None and dtype not in (np.dtype(np.float32), np.dtype(np.float16)):
+            raise ValueError("%s must be float32 or float16 (or a torch bfloat16 tensor), got %s" % (name, dtype))
+        x, family = sess.put(x)
+        in_torch = _is_torch_tensor(x)
+    if in_torch:
         torch, t = _torch(), x
         code = (_lib.DTYPE_F32 if t.dtype is torch.float32 else _lib.DTYPE_BF16 if t.dtype is torch.bfloat16
                 else _lib.DTYPE_F16 if t.dtype is torch.float16 else None)
-        if code is None:
-            raise ValueError("%s must be float32, float16 or bfloat16, got %s" % (name, x.dtype))
+        if code is None or (code == _lib.DTYPE_BF16 and family != "torch"):
+            raise ValueError("%s must be float32 or float16 (or a torch bfloat16 tensor), got %s" % (name, x.dtype))
         if t.dim() < 2:
             raise ValueError("%s must have at least 2 dimensions, got shape %s" % (name, tuple(x.shape)))
         if t.requires_grad:
@@ -309,30 +316,36 @@ def _float_rows(sess, x, name, max_ld=None):
         width = t.shape[-1]
         rows = t.numel() // width if width else math.prod(t.shape[:-1])
         if t.is_contiguous():
-            return t, "torch", rows, width, code, t.dtype
+            return t, family, rows, width, code, t.dtype
         try:
             t = t.view(rows, width)
         except RuntimeError:
             t = t.reshape(rows, width)
         if (t.stride(1) != 1 and width > 1) or (rows > 1 and not width <= t.stride(0) <= (max_ld or 1 << 62)):
             t = t.contiguous()
-        return t, "torch", rows, t.stride(0) if rows > 1 else width, code, t.dtype
-    dtype = np.dtype(getattr(x, "dtype", np.float32)) if not _is_tf_tensor(x) else np.dtype(x.dtype.as_numpy_dtype)
-    if dtype not in (np.dtype(np.float32), np.dtype(np.float16)):
-        raise ValueError("%s must be float32 or float16 (or a torch bfloat16 tensor), got %s" % (name, dtype))
-    t, family = sess.put(x, dtype if not sess.use_torch else None)
-    if len(t.shape) < 2:
-        raise ValueError("%s must have at least 2 dimensions, got shape %s" % (name, tuple(t.shape)))
-    rows = 1
-    for s in t.shape[:-1]:
-        rows *= int(s)
-    code = _lib.DTYPE_F32 if dtype == np.dtype(np.float32) else _lib.DTYPE_F16
-    return t, family, rows, int(t.shape[-1]), code, (t.dtype if sess.use_torch else dtype)
+        return t, family, rows, t.stride(0) if rows > 1 else width, code, t.dtype
+    if x.dtype not in (np.dtype(np.float32), np.dtype(np.float16)):
+        raise ValueError("%s must be float32 or float16, got %s" % (name, x.dtype))
+    if len(x.shape) < 2:
+        raise ValueError("%s must have at least 2 dimensions, got shape %s" % (name, x.shape))
+    return (x, family, math.prod(x.shape[:-1]), x.shape[-1],
+            _lib.DTYPE_F32 if x.dtype == np.dtype(np.float32) else _lib.DTYPE_F16, x.dtype)
 
 
 def _integers(sess, x, name, shape):
     """An int32 or int64 array of the given shape, dense on the device: (array, bytes a value)."""
-    if _is_torch_tensor(x):
+    in_torch = _is_torch_tensor(x)
+    if not in_torch and (isinstance(x, DevArray) or (hasattr(x, "__dlpack__") and not isinstance(x, np.ndarray)
+                                                     and not _is_tf_tensor(x))):
+        x, _ = sess.put(x)                               # another library's, read in place where it is on the GPU
+        in_torch = _is_torch_tensor(x)
+        if isinstance(x, DevArray):
+            if tuple(x.shape) != tuple(shape):
+                raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), x.shape))
+            if x.dtype in (np.dtype(np.int32), np.dtype(np.int64)):
+                return x, x.dtype.itemsize
+            x = x.numpy()
+    if in_torch:
         torch, t = _torch(), x
         if t.dtype is not torch.int64 and t.dtype is not torch.int32:
             if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
@@ -375,12 +388,12 @@ def _aligned(t, ld, width):
     """The same rows starting at a 16-byte boundary."""
     if t.data_ptr() % 16 == 0:
         return t, ld
-    return t.clone(memory_format=_torch().contiguous_format), width
+    return t.clone() if isinstance(t, DevArray) else t.clone(memory_format=_torch().contiguous_format), width
 
 
 def _empty_like(sess, t, shape, dtype):
     """A dense array of t's shape and type."""
-    if sess.use_torch and t.shape == shape and t.is_contiguous():
+    if _is_torch_tensor(t) and t.shape == shape and t.is_contiguous():
         return _torch().empty_like(t)
     return sess.empty(shape, dtype)
 
@@ -411,8 +424,7 @@ def linear_cross_entropy_batch(hidden, weight, labels, logit_scale=1.0, label_sm
         raise ValueError("weight must have shape (V, %d), got %s" % (dim, tuple(weight.shape)))
     if classes == 0 or dim == 0:
         raise ValueError("a head needs classes and values, got shape %s" % (tuple(weight.shape),))
-    if sess.use_torch:
-        w, ld_w = _aligned(w, ld_w, dim)
+    w, ld_w = _aligned(w, ld_w, dim)
     lab, label_bytes = _integers(sess, labels, "labels", lead)
     g = _row_floats(sess, grad_loss, "grad_loss", lead) if return_grad else None
     need = _head_bytes(rows, classes, dim, ld_w, code, float(label_smoothing), int(bool(return_grad)),

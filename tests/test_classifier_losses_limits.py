@@ -3,6 +3,7 @@ the teacher's, many rows, gradients in several pieces.  Bounds as in tests/test_
 import ctypes
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -231,3 +232,74 @@ def test_head_large_tiles_and_pieces(n, v, dim, dtype):
     # the mean, without smoothing
     plain = fda.linear_cross_entropy_batch(hidden, weight, labels, logit_scale=1.5, return_grad=True)
     rows_against_the_oracle(plain, hidden, weight, labels, torch.full((n,), 1.0 / n, device="cuda"), 1.5)
+
+
+# --------------------------------------------------------------------------------------------------- other libraries' arrays
+class Exported:
+    """What another library's array is to this one: DLPack, a shape and a numpy type."""
+
+    def __init__(self, t):
+        self.t, self.shape = t, tuple(t.shape)
+        self.dtype = np.dtype(str(t.dtype).replace("torch.", ""))
+
+    def __dlpack__(self, **kw):
+        return self.t.__dlpack__(**kw)
+
+    def __dlpack_device__(self):
+        return self.t.__dlpack_device__()
+
+    def __array__(self, *a, **kw):
+        raise TypeError("on the GPU")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16], ids=str)
+def test_losses_of_other_libraries_arrays(dtype):
+    import face_detection_amd as fda
+    from face_detection_amd.runtime import DevArray, default_context
+    n, v, dim = 37, 70, 24
+    hidden, weight, labels, weights = long_inputs(n, v, dim, dtype)
+    z, values, index, lse = [x.cuda() for x in distill_inputs(n, v, 5, dtype, tail=True)]
+    torch.cuda.synchronize()
+    head = fda.linear_cross_entropy_batch(hidden, weight, labels, grad_loss=weights, return_grad=True)
+    taught = fda.distill_topk_batch(z, values, index, teacher_lse=lse, grad_loss=weights, return_grad=True)
+
+    def same(got, want):
+        for a, b in zip(got, want):
+            assert isinstance(a, np.ndarray) and np.array_equal(a, b.cpu().numpy())
+
+    off = torch.empty(v * dim + 1, device="cuda", dtype=dtype)
+    off[1:] = weight.reshape(-1)
+    ctx = default_context(0, torch_stream=False)
+    dev = [DevArray.from_host(ctx, x.cpu().numpy()) for x in (labels, index, hidden)]
+    short = torch.where(labels < 0, labels, labels % 100).to(torch.int16)
+    for lab, ind in ((labels, index), (labels.int(), index.int()), (short, index.to(torch.int16))):
+        for w in (weight, off[1:].view(v, dim)):                       # (a base off any boundary)
+            torch.cuda.synchronize()
+            same(fda.linear_cross_entropy_batch(Exported(hidden), Exported(w), Exported(lab), grad_loss=Exported(weights),
+                                                return_grad=True), head)
+        same(fda.distill_topk_batch(Exported(z), Exported(values), Exported(ind), teacher_lse=Exported(lse),
+                                    grad_loss=Exported(weights), return_grad=True), taught)
+    same(fda.linear_cross_entropy_batch(dev[2], Exported(weight), dev[0], grad_loss=Exported(weights), return_grad=True), head)
+    same(fda.distill_topk_batch(Exported(z), Exported(values), dev[1], teacher_lse=Exported(lse), grad_loss=Exported(weights),
+                                return_grad=True), taught)
+    # some of torch's own among them
+    same(fda.linear_cross_entropy_batch(dev[2], weight, Exported(labels), grad_loss=weights, return_grad=True), head)
+    got = fda.linear_cross_entropy_batch(hidden, Exported(weight), dev[0], grad_loss=Exported(weights), return_grad=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, head))
+    for bad in (Exported(labels.float()), Exported(labels[:5])):
+        with pytest.raises(ValueError):
+            fda.linear_cross_entropy_batch(Exported(hidden), Exported(weight), bad)
+    with pytest.raises(ValueError):
+        fda.linear_cross_entropy_batch(Exported(hidden.double()), Exported(weight.double()), Exported(labels))
+
+
+@gpu
+def test_losses_of_empty_numpy_batches():
+    import face_detection_amd as fda
+    loss, gh, gw = fda.linear_cross_entropy_batch(np.empty((0, 8), np.float32), np.ones((10, 8), np.float32),
+                                                  np.empty(0, np.int64), return_grad=True)
+    assert loss.shape == (0,) and gh.shape == (0, 8) and gw.shape == (10, 8) and (gw == 0).all()
+    loss, grad = fda.distill_topk_batch(np.empty((0, 9), np.float16), np.empty((0, 3), np.float32), np.empty((0, 3), np.int64),
+                                        return_grad=True)
+    assert loss.shape == (0,) and grad.shape == (0, 9) and grad.dtype == np.float16
