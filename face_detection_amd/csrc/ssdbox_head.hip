@@ -1020,7 +1020,7 @@ HeadPlan make_plan(long long rows, long long classes, long long dim, long long w
         q.ld_delta = q.piece + 256 / q.es;
         if (q.few_parts) {
             if ((size_t)(rows * q.ld_delta) * q.es > kDeltaBytes) q.ld_delta = (classes + 63) / 64 * 64;
-        } else if (rows * (256 * q.es + 256) > (long long)kDeltaBytes) {
+        } else if (rows * q.es * 256 > (long long)kDeltaBytes) {
             // So many rows that a piece of any width is too much: they are cut, too.  dW is added over the chunks, which costs
             // less than dH over pieces, so pieces are wide again (ms, pieces of 256 classes of all rows, of 1024, 2048, 4096 of
             // chunks:  2000000 x 4000 x 64 float32 70.2 67.4 67.8 77.6,  3000000 x 4000 x 64 bfloat16 43.9 37.5 35.7 33.6).
@@ -1032,9 +1032,12 @@ HeadPlan make_plan(long long rows, long long classes, long long dim, long long w
             q.chunk_rows = (long long)kDeltaBytes / (q.ld_delta * q.es) / 256 * 256;
             q.chunks = (int)((rows + q.chunk_rows - 1) / q.chunk_rows);
         }
-        // The pass over what is kept and its stores move bytes, the products it spares take 2 dim operations a logit.
-        if (q.few_parts || q.chunks > 1) q.keep = false;
-        else if (dtype == SSDBOX_DTYPE_F32) q.keep = true;
+        // The pass over what is kept and its stores move bytes, the products it spares take 2 dim operations a logit.  Of chunks
+        // only float32 of one piece keeps them (kept, taken again, ms: 3000000 x 200 x 512 float32 28.6 33.8; 4500000 x 200 x 512
+        // bfloat16 18.1 17.0).
+        if (q.few_parts) q.keep = false;
+        else if (dtype == SSDBOX_DTYPE_F32) q.keep = q.chunks == 1 || q.pieces == 1;
+        else if (q.chunks > 1) q.keep = false;
         else if (dtype == SSDBOX_DTYPE_BF16) q.keep = dim > kKeepAboveBf16;
         else q.keep = dim > kKeepAboveF16 && q.pieces == 1 && (size_t)(rows * q.ld_delta) * 4 <= kDeltaBytes;
     }
@@ -1302,8 +1305,39 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
     l.slots = q.slots;
     l.z_label = (float *)(c.ws + q.o_zl);
     l.row = (const HeadRow *)(c.ws + q.o_out);
+    RowArgs r = {};
+    // Logits and rows of one chunk, or of all.
+    const auto logits_and_rows = [&](long long row0, long long n_rows, const int *counted) {
+        LogitArgs a = l;
+        a.rows = rows + row0 * q.pitch;
+        a.count = counted;
+        a.label = label + row0;
+        a.stat = l.stat + row0 * q.slots;
+        if (a.sum_z) a.sum_z += row0 * q.slots;
+        a.z_label = l.z_label + row0;
+        if (q.keep) {
+            a.kept_from = (int)((q.pieces - 1) * q.piece);
+            a.delta = kept;
+            a.ld_delta = q.ld_delta;
+            launch_logits<T, kStatKeep>(c, q.tile, a);
+        } else {
+            launch_logits<T, kStat>(c, q.tile, a);
+        }
+        RowArgs b = r;
+        b.count = counted;
+        b.row = row + row0;
+        b.label = a.label;
+        b.stat = a.stat;
+        b.sum_z = a.sum_z;
+        b.z_label = a.z_label;
+        if (b.out) b.out += row0;
+        if (q.slots < 2048 || n_rows > kMostRows / 4)
+            launch_stage(ctx, SSDBOX_STAGE_LOSS, head_row_kernel<256>, dim3((unsigned)n_rows), dim3(256), b);
+        else
+            launch_stage(ctx, SSDBOX_STAGE_LOSS, head_row_kernel<1024>, dim3((unsigned)n_rows), dim3(1024), b);
+    };
+    const bool keep_chunks = q.keep && q.chunks > 1;             // of one piece: what is kept of a chunk becomes its d at once
     if (c.rows > 0) {
-        RowArgs r = {};
         r.count = count;
         r.row = row;
         r.label = label;
@@ -1343,19 +1377,8 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
             };
             if (c.classes < 4096) few(q.direct ? head_few_kernel<T, 256, true> : head_few_kernel<T, 256, false>, 256);
             else few(q.direct ? head_few_kernel<T, 1024, true> : head_few_kernel<T, 1024, false>, 1024);
-        } else {
-            if (q.keep) {
-                l.kept_from = (int)((q.pieces - 1) * q.piece);
-                l.delta = kept;
-                l.ld_delta = q.ld_delta;
-                launch_logits<T, kStatKeep>(c, q.tile, l);
-            } else {
-                launch_logits<T, kStat>(c, q.tile, l);
-            }
-            if (q.slots < 2048 || c.rows > kMostRows / 4)
-                launch_stage(ctx, SSDBOX_STAGE_LOSS, head_row_kernel<256>, dim3((unsigned)c.rows), dim3(256), r);
-            else
-                launch_stage(ctx, SSDBOX_STAGE_LOSS, head_row_kernel<1024>, dim3((unsigned)c.rows), dim3(1024), r);
+        } else if (!keep_chunks) {
+            logits_and_rows(0, c.rows, count);
         }
     }
     if (!grad) return SSDBOX_OK;
@@ -1371,12 +1394,13 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
         T *delta = (T *)(c.ws + q.o_delta);
         if (q.few_parts) {
             // d is there: few tiles are one piece
-        } else if (c.rows > 0 && q.keep && turn == 0) {
+        } else if (c.rows > 0 && q.keep && (turn == 0 || keep_chunks)) {
+            if (keep_chunks) logits_and_rows(row0, n_rows, counted);
             KeptArgs k = {};
-            k.count = count;
-            k.label = label;
-            k.row = l.row;
-            k.stat = l.stat;
+            k.count = counted;
+            k.label = label + row0;
+            k.row = l.row + row0;
+            k.stat = l.stat + row0 * q.slots;
             k.slots = q.slots;
             k.each = q.each;
             k.first = (int)first;
@@ -1388,7 +1412,8 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
             k.ld_delta = q.ld_delta;
             k.piece = q.piece;
             k.blocks = (int)((q.piece + kRowThreads * q.vec - 1) / (kRowThreads * q.vec));
-            launch_stage(ctx, SSDBOX_STAGE_LOSS, head_kept_kernel<T>, dim3((unsigned)(c.rows * k.blocks)), dim3(kRowThreads), k);
+            launch_stage(ctx, SSDBOX_STAGE_LOSS, head_kept_kernel<T>, dim3((unsigned)((long long)n_rows * k.blocks)),
+                         dim3(kRowThreads), k);
         } else if (c.rows > 0) {
             LogitArgs d = l;
             d.weight = weight + first * ldw;
