@@ -921,7 +921,7 @@ struct HeadPlan {
     size_t bytes;
 };
 
-constexpr size_t kDeltaBytes = (size_t)1 << 31;    // of one piece's d (its rows' padding, up to a quarter, comes on top)
+constexpr size_t kDeltaBytes = (size_t)1 << 31;    // of one piece's d (256 bytes a row, half as much again at most, come on top)
 constexpr long long kChunkRow = 8192;              // bytes of a row of d at most, where rows are cut
 
 // From which dim on something is kept.  Measured (rows x classes x dim, taken again, kept; us):

@@ -291,8 +291,8 @@ int ssdbox_ssd_loss(ssdbox_ctx *ctx, const float *d_y_true, const float *d_y_pre
  * done, so that calls on several streams, or in several captured graphs, each have their own. */
 
 /* Softmax cross entropy of a linear head, logits = logit_scale * hidden weight^T: of the
- * (rows, classes) logits and their gradient no more than about 2 GiB each (2.5 with rows' padding) is
- * ever stored; up to there they may be stored whole.  d_hidden (rows, dim) and d_weight (classes, dim)
+ * (rows, classes) logits and their gradient no more than about 2 GiB each (with the rows' padding 3 at
+ * most) is ever stored; up to there they may be stored whole.  d_hidden (rows, dim) and d_weight (classes, dim)
  * of `dtype`, rows hidden_ld / weight_ld values apart; d_labels (rows) int32 or int64 (label_bytes
  * 4 or 8).  A row with a negative label is left out: loss 0, no gradient, and its hidden values
  * are not used.  A label >= classes gives loss NaN and no gradient.
