@@ -37,6 +37,7 @@ constexpr long long kMostLd = 1 << 21;        // from one row of an operand to t
 constexpr long long kMostRows = (1 << 24) - 1;  // of workgroups of 256: a launch takes fewer than 2^32 threads
 constexpr int kRowsEach = 4;          // rows a workgroup places and copies
 constexpr int kCountRows = 1024;      // rows a workgroup counts, where there are many
+constexpr int kMostShift = 10;        // of a row of float16's d, beyond the scale that all have (see row_finish)
 constexpr int kCountFrom = 4096;      // rows from which counting has a launch of its own: below, reading all labels before
                                       // a workgroup's rows again costs less than the launch
 
@@ -486,11 +487,35 @@ struct RowArgs {
     const HeadScale *scale;
     float *loss;
     HeadRow *out;
+    float *row_up;                    // float16 with rows' weights: 2^-shift of each counted row, and its values times that for
+    const void *values;               // dW (in their place, or not)
+    void *scaled;
+    int pitch;
 };
 
-// A row's loss and its gradient's terms: the others' exponentials sum to s * 2^m, the label's is 2^(z l2) with its product z.
-SSD_DEV HeadRow row_finish(const RowArgs &p, int n_in, float down, float m, double s, double sz, float z)
+// A counted row's values times 2^-shift, by a workgroup.
+template <typename T, int THREADS>
+SSD_DEV void scale_row(const T *from, T *to, int pitch, int shift)
 {
+    constexpr int kVec = 16 / (int)sizeof(T);
+    if (from == to && shift == 0) return;
+    const float f = u2f((uint32_t)(127 - shift) << 23);
+    for (int d = threadIdx.x * kVec; d < pitch; d += THREADS * kVec) {
+        union { u32x4 w; T v[kVec]; } x;
+        x.w = *(const u32x4 *)(from + d);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) x.v[i] = (T)((float)x.v[i] * f);
+        *(u32x4 *)(to + d) = x.w;
+    }
+}
+
+// A row's loss and its gradient's terms: the others' exponentials sum to s * 2^m, the label's is 2^(z l2) with its product z.
+// Float16 has few exponents: with one scale for all, p of a row whose weight is 10^6 times smaller than the largest would lie among
+// the subnormals.  Such a row's d is raised by 2^shift, which its dH gives back, and its values in dW's product.  What those lose
+// below 2^-14 is, with a shift of 10, less than their own rounding for values from 2^-4 on, and little beside other rows' terms.
+SSD_DEV HeadRow row_finish(const RowArgs &p, int n_in, float down, float m, double s, double sz, float z, int &shift)
+{
+    shift = 0;
     const double zl = (double)z * (double)p.l2;
     double nll = 0.0;
     if (s != 0.0) {
@@ -506,7 +531,12 @@ SSD_DEV HeadRow row_finish(const RowArgs &p, int n_in, float down, float m, doub
     HeadRow r = {0.0f, 0.0f, 0.0f, 0.0f};
     if (!p.out) return r;
     const double g = p.grad_loss ? (double)p.grad_loss[n_in] : 1.0 / (double)p.rows;
-    const double c = g * (double)p.logit_scale * (double)down;
+    double c = g * (double)p.logit_scale * (double)down;
+    if (p.row_up) {
+        const double v = fabs(c) * (1.0 - fmin((double)p.smoothing, 0.5));     // at most 32768 (1 - 1 / 128)
+        while (shift < kMostShift && v * (double)(2 << shift) <= 32512.0) ++shift;
+        c *= (double)(1 << shift);
+    }
     const float top = fmaxf(m, (float)zl);
     const double whole = (s != 0.0 ? s * exp2((double)m - (double)top) : 0.0) + exp2(zl - (double)top);
     const double share = (double)p.smoothing / (double)p.classes;
@@ -524,6 +554,7 @@ __global__ __launch_bounds__(THREADS) void head_row_kernel(const RowArgs p)
 {
     __shared__ float s_m[THREADS / 64];
     __shared__ double s_s[THREADS / 64], s_z[THREADS / 64];
+    __shared__ int s_shift;
     const int n = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
     if (n >= *p.count) return;
     const float2 *st = p.stat + (long long)n * p.slots;
@@ -558,17 +589,23 @@ __global__ __launch_bounds__(THREADS) void head_row_kernel(const RowArgs p)
         s_z[wave] = sz;
     }
     __syncthreads();
-    if (t != 0) return;
-    m = -INFINITY;
-    for (int w = 0; w < THREADS / 64; ++w) m = fmaxf(m, s_m[w]);
-    s = 0.0;
-    sz = 0.0;
-    for (int w = 0; w < THREADS / 64; ++w) {
-        s += m != -INFINITY ? s_s[w] * (double)__builtin_amdgcn_exp2f(s_m[w] - m) : s_s[w];
-        sz += s_z[w];
+    if (t == 0) {
+        m = -INFINITY;
+        for (int w = 0; w < THREADS / 64; ++w) m = fmaxf(m, s_m[w]);
+        s = 0.0;
+        sz = 0.0;
+        for (int w = 0; w < THREADS / 64; ++w) {
+            s += m != -INFINITY ? s_s[w] * (double)__builtin_amdgcn_exp2f(s_m[w] - m) : s_s[w];
+            sz += s_z[w];
+        }
+        const HeadRow r = row_finish(p, p.row[n], p.out ? p.scale->down : 1.0f, m, s, sz, p.z_label[n], s_shift);
+        if (p.out) p.out[n] = r;
+        if (p.row_up) p.row_up[n] = u2f((uint32_t)(127 - s_shift) << 23);
     }
-    const HeadRow r = row_finish(p, p.row[n], p.out ? p.scale->down : 1.0f, m, s, sz, p.z_label[n]);
-    if (p.out) p.out[n] = r;
+    if (!p.scaled) return;
+    __syncthreads();
+    scale_row<f16_t, THREADS>((const f16_t *)p.values + (long long)n * p.pitch, (f16_t *)p.scaled + (long long)n * p.pitch,
+                              p.pitch, s_shift);
 }
 
 // Few logits: their products (in parts, where k was cut) are joined in the parts' order a row at a time, with the row's
@@ -582,6 +619,7 @@ __global__ __launch_bounds__(THREADS) void head_few_kernel(const RowArgs p, cons
     __shared__ float s_m[THREADS / 64], s_g[THREADS / 64], s_label;
     __shared__ double s_s[THREADS / 64], s_z[THREADS / 64];
     __shared__ HeadRow s_row;
+    __shared__ int s_shift;
     const int n = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6, classes = (int)p.classes;
     int lab, n_in;
     float down = 1.0f;
@@ -659,11 +697,16 @@ __global__ __launch_bounds__(THREADS) void head_few_kernel(const RowArgs p, cons
             s_s[0] += s_s[w];
             s_z[0] += s_z[w];
         }
-        s_row = row_finish(p, n_in, down, m, s_s[0], s_z[0], s_label);
+        s_row = row_finish(p, n_in, down, m, s_s[0], s_z[0], s_label, s_shift);
+        if (p.row_up) p.row_up[n] = u2f((uint32_t)(127 - s_shift) << 23);
     }
     if (!p.out) return;
     __syncthreads();
     const HeadRow r = s_row;
+    if constexpr (__is_same(T, f16_t))
+        if (p.scaled)                 // (each lane what it has copied, if it has)
+            scale_row<T, THREADS>((const T *)p.values + (long long)n * p.pitch, (T *)p.scaled + (long long)n * p.pitch,
+                                  p.pitch, s_shift);
     T *d = delta + (long long)n * ld_delta;
     for (int v = t * 4; v < (classes + 63) / 64 * 64; v += THREADS * 4) {    // d has zeros behind the last class
         struct __align__(4 * sizeof(T)) { T v[4]; } o;
@@ -742,6 +785,7 @@ struct GradArgs {
     void *out;                        // [n][ldo], through row_of when given
     long long ldo;
     const int *row_of;
+    const float *row_up;              // what row n is multiplied by besides, or NULL
     float *part;                      // [part][n][ld_part] instead of out, or NULL
     long long ld_part, part_stride;
     int add;                          // to what part holds
@@ -792,6 +836,9 @@ SSD_DEV void product(const GradArgs &p, int block, int blocks, char *smem)
             } else {
                 const int to = in ? (p.row_of ? p.row_of[n] : n) : -1;
                 in = to >= 0;
+                float up_n = up;
+                if constexpr (__is_same(T, f16_t))
+                    if (p.row_up && in) up_n *= p.row_up[n];
                 T *o = (T *)p.out + (in ? (long long)to : 0) * p.ldo;
 #pragma unroll
                 for (int mi = 0; mi < S::MF; ++mi)
@@ -800,7 +847,7 @@ SSD_DEV void product(const GradArgs &p, int block, int blocks, char *smem)
                         const int m = u.m0 + em + mi * 32 + e * 2;
                         float d[2][4];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) d[i >> 2][i & 3] = acc[mi][nj][e + i] * up;
+                        for (int i = 0; i < 8; ++i) d[i >> 2][i & 3] = acc[mi][nj][e + i] * up_n;
                         store_pair<T>(o, m, d[0], d[1], p.m - m, in);
                     }
             }
@@ -837,6 +884,7 @@ struct JoinArgs {
     void *out;
     long long ldo;
     const int *row_of;
+    const float *row_up;
     long long first;                  // the launch's first workgroup of the product's
 };
 
@@ -874,7 +922,7 @@ SSD_DEV void join(const JoinArgs &p, long long block, f32x4 (&s_sum)[WAVES > 1 ?
     if (!in) return;
     const int to = p.row_of ? p.row_of[n] : n;
     if (to < 0) return;
-    const float up = p.scale->up;
+    const float up = p.row_up ? p.scale->up * p.row_up[n] : p.scale->up;
     T *o = (T *)p.out + to * p.ldo + m;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -916,7 +964,8 @@ struct HeadPlan {
     int chunks;                       // of counted rows, whose d of a piece is there at a time
     long long chunk_rows;
     int dh_parts, dw_parts;
-    size_t o_few, o_blocks, o_rows, o_weight, o_row, o_label, o_count, o_scale, o_stat, o_sumz, o_zl, o_out, o_delta, o_kept, o_dh,
+    bool scale_in_place;              // float16's rows times 2^-shift: nothing reads them as they were after their statistics
+    size_t o_few, o_blocks, o_rows, o_row_up, o_scaled, o_weight, o_row, o_label, o_count, o_scale, o_stat, o_sumz, o_zl, o_out, o_delta, o_kept, o_dh,
         o_dw;
     size_t bytes;
 };
@@ -1051,6 +1100,10 @@ HeadPlan make_plan(long long rows, long long classes, long long dim, long long w
     q.o_zl = put(at, rows * 4);
     q.o_out = put(at, rows * sizeof(HeadRow));
     q.o_rows = put(at, (size_t)rows * q.pitch * q.es);
+    q.scale_in_place = q.few_parts || (q.keep && q.pieces == 1);
+    const bool half = dtype == SSDBOX_DTYPE_F16 && grad;
+    q.o_row_up = put(at, half ? rows * 4 : 0);
+    q.o_scaled = put(at, half && grad_weight && !q.scale_in_place ? (size_t)rows * q.pitch * q.es : 0);
     q.o_stat = put(at, q.few_parts ? 0 : (size_t)rows * q.slots * sizeof(float2));
     q.o_sumz = put(at, smoothing != 0.0f && !q.few_parts ? (size_t)rows * q.slots * 4 : 0);
     q.o_weight = put(at, q.copy_weight ? (size_t)classes * q.pitch * q.es : 0);
@@ -1148,6 +1201,7 @@ JoinArgs join_args(const GradArgs &a)
     j.out = a.out;
     j.ldo = a.ldo;
     j.row_of = a.row_of;
+    j.row_up = a.row_up;
     return j;
 }
 
@@ -1238,6 +1292,8 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
     int *count = (int *)(c.ws + q.o_count), *row = (int *)(c.ws + q.o_row), *label = (int *)(c.ws + q.o_label);
     HeadScale *scale = (HeadScale *)(c.ws + q.o_scale);
     T *rows = (T *)(c.ws + q.o_rows);
+    float *row_up = dtype == SSDBOX_DTYPE_F16 && grad && c.grad_loss ? (float *)(c.ws + q.o_row_up) : nullptr;
+    T *scaled = row_up && !q.scale_in_place ? (T *)(c.ws + q.o_scaled) : rows;
     void *kept = c.ws + (dtype == SSDBOX_DTYPE_F16 ? q.o_kept : q.o_delta);
 
     PrepArgs s = {};
@@ -1331,6 +1387,9 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
         b.sum_z = a.sum_z;
         b.z_label = a.z_label;
         if (b.out) b.out += row0;
+        if (b.row_up) b.row_up += row0;
+        b.values = a.rows;
+        if (b.scaled) b.scaled = scaled + row0 * q.pitch;
         if (q.slots < 2048 || n_rows > kMostRows / 4)
             launch_stage(ctx, SSDBOX_STAGE_LOSS, head_row_kernel<256>, dim3((unsigned)n_rows), dim3(256), b);
         else
@@ -1354,6 +1413,10 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
         r.scale = scale;
         r.loss = c.loss;
         r.out = grad ? (HeadRow *)(c.ws + q.o_out) : nullptr;
+        r.row_up = row_up;
+        r.values = rows;
+        r.scaled = row_up && c.grad_weight ? scaled : nullptr;
+        r.pitch = q.pitch;
         if (q.few_parts) {
             GradArgs f = {};
             f.a = weight;
@@ -1446,6 +1509,7 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
             h.parts = q.dh_parts;
             h.out = c.grad_hidden;
             h.row_of = row + row0;
+            h.row_up = row_up ? row_up + row0 : nullptr;
             if (q.dh_parts > 1 || q.pieces > 1) {
                 h.part = (float *)(c.ws + q.o_dh) + row0 * wide;
                 h.ld_part = wide;
@@ -1455,7 +1519,7 @@ int run_head(const HeadCall &c, const HeadPlan &q, int dtype)
             }
         }
         if (c.grad_weight) {
-            w.a = rows + row0 * q.pitch;
+            w.a = scaled + row0 * q.pitch;
             w.lda = q.pitch;
             w.n = n_class;
             w.k = n_rows;

@@ -142,9 +142,10 @@ def within_there(got, want, off, what):
         what, int((over > 0).sum()), over.numel(), float(over.max()))
 
 
-def rows_against_the_oracle(got, hidden, weight, labels, weights, scale=1.0, smoothing=0.0, ends=None, logits=1 << 23):
+def rows_against_the_oracle(got, hidden, weight, labels, weights, scale=1.0, smoothing=0.0, ends=None, logits=1 << 23,
+                            extra=0.0):
     """A long batch's results, some rows at a time; with ends only the loss and the hidden rows' gradient of so many rows at
-    either end."""
+    either end.  extra: of the weight's gradient's bound."""
     n, v = len(labels), len(weight)
     left_out = (labels < 0).nonzero()[:, 0]
     assert (got[0][left_out] == 0).all() and (got[1][left_out] == 0).all()
@@ -166,7 +167,7 @@ def rows_against_the_oracle(got, hidden, weight, labels, weights, scale=1.0, smo
             want_w += gw
             off_w = off_w + off_gw
     if ends is None:
-        within_there(got[2], want_w, off_w, "grad_weight")
+        within_there(got[2], want_w, off_w + extra, "grad_weight")
 
 
 @gpu
@@ -309,3 +310,31 @@ def test_losses_of_empty_numpy_batches():
     loss, grad = fda.distill_topk_batch(np.empty((0, 9), np.float16), np.empty((0, 3), np.float32), np.empty((0, 3), np.int64),
                                         return_grad=True)
     assert loss.shape == (0,) and grad.shape == (0, 9) and grad.dtype == np.float16
+
+
+# few logits, with rows left where they are or placed; logits taken again, kept; one row's slots many; several pieces; chunks
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("n,v,dim", [(60, 700, 64), (60, 700, 61), (5000, 900, 64), (300, 40000, 72), (300, 40000, 400), (40, 280000, 64),
+                                     (67000, 16700, 24), (4300000, 270, 16)])
+def test_head_weights_far_apart(n, v, dim, dtype):
+    """Rows' weights over nine powers of ten: each row's own gradient keeps the accuracy that its weight alone would give it, but for
+    what lies below 2^-10 of the largest."""
+    import face_detection_amd as fda
+    hidden, weight, labels, _ = long_inputs(n, v, dim, dtype, ignored=0.1)
+    power = torch.arange(n, device="cuda") * 7 % 10
+    # (the largest so that dW of a hundred rows is within float16)
+    weights = (4000.0 if n < 10000 else 0.5) * 10.0 ** -power.float()
+    got = fda.linear_cross_entropy_batch(hidden, weight, labels, grad_loss=weights, return_grad=True)
+    most = float(weights.max())
+    for k in range(10):
+        at = ((power == k) & (labels >= 0)).nonzero()[:, 0][:2000]
+        own = most * 10.0 ** -k
+        (loss, gh, _), (off, off_h, _) = O.head(hidden[at], weight, labels[at], 1.0, 0.0, weights[at], max(own, most * 2.0 ** -10))
+        within_there(got[0][at], loss, off, "loss at 1e-%d" % k)
+        within_there(got[1][at], gh, off_h, "grad_hidden at 1e-%d" % k)
+    # values of rows that are less than half the largest are rounded at 2^-25 times what their d was raised by, float16's alone
+    extra = most * n * 2.0 ** -25 if dtype == torch.float16 else 0.0
+    rows_against_the_oracle(got, hidden, weight, labels, weights, extra=extra)
+    frozen = fda.linear_cross_entropy_batch(hidden, weight, labels, grad_loss=weights, return_grad=True, weight_grad=False)
+    assert torch.equal(frozen[1], got[1])
