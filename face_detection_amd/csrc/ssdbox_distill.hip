@@ -254,6 +254,7 @@ struct RowTerms {
 
     SSD_DEV double log_q(float t) const { return ((double)t - t_top) * inv_tau - ln_t; }
     SSD_DEV double log_p(float z) const { return (((double)z - (double)sub) * (double)l2 - (double)off) * kLn2 - ln_s; }
+    // (in float32, as p is, and as good as the gradient that it goes into; the loss's sums and logarithms are in 64 bits)
     SSD_DEV float q(float t) const { return __builtin_amdgcn_exp2f((float)(log_q(t) * kLog2eD)); }
     SSD_DEV float power(float z) const { return __builtin_amdgcn_exp2f(__builtin_fmaf(z - sub, l2, -off)); }
     SSD_DEV float share(float z) const { return (float)((double)power(z) * inv_s); }
@@ -346,7 +347,7 @@ SSD_DEV double terms_finish(RowTerms &r, const DistArgs &p, long long row, doubl
 // teacher's classes' logits is at hand before the row has arrived, so the row's maximum is taken, from memory again, only where
 // the sum says that the reference was far off (or a mask's lowest value overflowed the product).
 //
-// HBM bounds it: 8192 x 131072 bfloat16 with the rest bucket 935 us, 4.6 TB/s read and written; 3001 x 100003 float32 500 us, 4.8;
+// HBM bounds it: 8192 x 131072 bfloat16 with the rest bucket 931 us, 4.6 TB/s read and written; 3001 x 100003 float32 500 us, 4.8;
 // 2048 x 32000 the value alone 31 us, 4.3; one row of 32000 8 us, latency.  (A large copy: 4.96.)
 //
 // The registers are only ever loaded and read: a piece that holds one of the teacher's classes is summed without them where
@@ -1014,6 +1015,11 @@ void launch_distill(ssdbox_ctx *ctx, const DistArgs &a, const DistPlan &q, int r
         launch_stage(ctx, SSDBOX_STAGE_LOSS, distill_segment_kernel<T>, dim3((unsigned)rows * (a.grad ? q.segments : 1)),
                      dim3(kSegThreads), a);
     }
+    // as many lanes a row as leave each of them four classes; twice as many (rows x classes x K, us): 408000 x 4 x 2 float32 14.8, 16.4;
+    // 400000 x 8 x 3 bfloat16 24, 36;  400000 x 16 x 4 float32 35, 61;  300000 x 32 x 4 bfloat16 51, 91.  Against the sixteen lanes of
+    // the next kernel: 487435 x 23 x 6 float32 80, 109, its value alone 62, 103;  400000 x 20 x 2 bfloat16 55, 96; from 33 classes on they
+    // would be faster up to 64 entries (400000 x 60 x 2 float32 134, 122;  100000 x 40 x 8 float16 45, 37;  200000 x 60 x 30 bfloat16
+    // 151, 64), which this border leaves
     else if (a.classes <= 4) launch_small<T, 1>(ctx, a, rows);
     else if (a.classes <= 8) launch_small<T, 2>(ctx, a, rows);
     else if (a.classes <= 16) launch_small<T, 4>(ctx, a, rows);
@@ -1021,7 +1027,8 @@ void launch_distill(ssdbox_ctx *ctx, const DistArgs &a, const DistPlan &q, int r
     else if (a.classes <= 64) launch_small<T, 16>(ctx, a, rows);
     // short rows: sixteen lanes a row rather than a wave, as long as the registers hold the entries (rows x classes x K, us:
     // 113154 x 164 x 8 float32 39, a wave 113;  35660 x 74 x 15 float32 18, 40;  50000 x 400 x 64 float32 44, 66;
-    // 20000 x 1000 x 16 bfloat16 20, 31; past the registers' entries 20000 x 500 x 200 float32 133, 37)
+    // 20000 x 1000 x 16 bfloat16 20, 31; past the registers' entries 20000 x 500 x 200 float32 133, 37), in registers for no more
+    // pieces than there are (for 128 instead: 113154 x 100 x 8 float32 34, 40;  100000 x 200 x 8 44, 50;  60000 x 400 x 16 bfloat16 30, 32)
     else if (pieces <= 128 && a.top <= 16 * kEntries<16>) {
         if (pieces <= 32) launch_row<T, 16, 2>(ctx, a, rows);
         else if (pieces <= 64) launch_row<T, 16, 4>(ctx, a, rows);
@@ -1029,13 +1036,17 @@ void launch_distill(ssdbox_ctx *ctx, const DistArgs &a, const DistPlan &q, int r
     }
     // (479494 x 728 x 2 float32 485, a wave 620, its value alone 266, 475;  50000 x 1000 x 60 float32 111, 88)
     else if (pieces <= 256 && a.top <= 16) launch_row<T, 16, 16>(ctx, a, rows);
+    // (registers for 256 pieces instead: 60000 x 120 x 100 float32 72, 77;  60000 x 400 x 70 bfloat16 76, 80)
     else if (pieces <= 64) launch_row<T, 64, 1>(ctx, a, rows);
     else if (pieces <= 128) launch_row<T, 64, 2>(ctx, a, rows);
     else if (pieces <= 256) launch_row<T, 64, 4>(ctx, a, rows);
     // (a workgroup of 256 a row instead: 143928 x 2754 x 14 bfloat16 432 us, 852;  30000 x 8000 x 32 196, 224, its value alone
     // 84, 149;  100 x 2754 x 14 18.0, 17.2;  50000 x 4000 x 14 float32 315, 300)
+    // (registers for 1024 pieces instead: 20000 x 2000 x 14 float32 57, 66;  20000 x 3900 x 14 bfloat16 64, 74)
     else if (pieces <= 512) launch_row<T, 64, 8>(ctx, a, rows);
     else if (pieces <= 1024) launch_row<T, 64, 16>(ctx, a, rows);
+    // (a workgroup of 512 with registers for 8192 pieces instead: 8000 x 8000 x 14 float32 96, 135;  4000 x 16000 x 14 115, 119; and
+    // with registers for 25600 instead of 16384: 2000 x 50000 x 14 float32 194, 193;  2000 x 120000 x 14 bfloat16 228, 237)
     else if (pieces <= 2048) launch_row<T, 256, 8>(ctx, a, rows);
     else if (pieces <= 4096) launch_row<T, 512, 8>(ctx, a, rows);
     else if (pieces <= 8192) launch_row<T, 512, 16>(ctx, a, rows);

@@ -1,4 +1,5 @@
-// Cross entropy of a linear head over many classes, with its gradients, without the logits being kept.
+// Cross entropy of a linear head over many classes, with its gradients; of the logits and of d no more than about 2 GiB each is
+// stored at a time.
 //
 //   z = s H W^T (rows x classes), l = label, eps = label smoothing, V = classes
 //   nll = log sum_v exp z_v - z_l,   loss = (1 - eps) nll + eps (log sum_v exp z_v - mean_v z_v)
@@ -8,8 +9,8 @@
 // what its counted rows cost and nothing of a padded row (a NaN, say) reaches a sum over rows.  Then
 //   1  logits, a tile of classes x rows per workgroup; of each tile only (max, sum of exp) per row leave the chip
 //   2  per row: log-sum-exp, loss, and what the gradient needs (four floats a row)
-//   3  per piece of the classes: the logits again, turned into d in the epilogue and written in the operands' type;
-//      dH += d W_piece, dW_piece = d^T H.
+//   3  per piece of the classes (a d of 2 GiB: all of them, as a rule), and per chunk of the rows where 256 classes of all are more:
+//      the logits again, turned into d in the epilogue and written in the operands' type; dH += d W_piece, dW_piece = d^T H.
 // Recomputing the logits is 2 of the gradient's 8 rows * classes * dim operations.  The last piece need not be: while step 1
 // runs, what d can be made of waits for a pass that turns it into d.  float32: the products, in d's own place.  bfloat16: the
 // exponentials in 16 bits, relative to their tile's maximum, there too (float16's 11 bits round them finer than d's 8).
@@ -21,7 +22,8 @@
 // Exponentials are taken to base 2: exp(z_v - M) = 2^(a L - m) with a the product as summed, L = s log2(e) and m the row's
 // largest a L rounded once; m itself is what the rows' kernel adds back, so its rounding cancels.
 // Sums over k stay in float32 accumulators; over tiles and rows of partial results they are added in a fixed order, in
-// float64 for the exponentials.  d is rounded once, to the operands' type, which is what the matrix instructions read.
+// float64 for the exponentials.  d is rounded to the operands' type, which is what the matrix instructions read: once, but for
+// bfloat16's kept exponentials, whose first rounding to 11 bits is an eighth of the second one to 8.
 #include <math.h>
 
 #include <type_traits>
@@ -336,8 +338,8 @@ SSD_DEV void store_pair(T *row, int m, const float (&lo)[4], const float (&hi)[4
 
 // The logits by tiles: matrix instructions, and behind each tile its exponentials (one v_exp_f32 a logit, which the
 // stream's loads for the next tile run under).  Long dim: bound by the matrix instructions at the clock that the power limit leaves
-// (4096 x 32000 x 4096 bfloat16, value: 900 us, 1.19 PFLOP/s of 1.36 that the library's product alone reaches); short dim: by the
-// epilogue (1694 x 104936 x 16: 102 us, 1.7e12 exponentials a second).
+// (3891 x 32000 x 4096 bfloat16, value: 907 us, 1.12 PFLOP/s of 1.36 that the library's product alone reaches, matrix cores busy 74 %
+// of the time; 7782 x 131072 x 2048 with the exponentials stored: 4.06 ms, 1.03, 62 %); short dim: by the epilogue (1694 x 104936 x 16: 102 us, 1.7e12 exponentials a second).
 template <typename T, int BM, int BN, int WM, int WN, int BLOCKS, int WHAT>
 __global__ __launch_bounds__(WM * WN * 64, BLOCKS * WM * WN / 4) void head_logit_kernel(const LogitArgs p)
 {
@@ -792,8 +794,8 @@ struct GradArgs {
 };
 
 // A product whose result is written, or its parts: dH = d W, dW = d^T H, and few logits.  Matrix instructions at long k (7782 x
-// 131072 x 2048 bfloat16: dH 3.26 ms, 1.28 PFLOP/s, the library's 1.35; dW 3.34, 1.25 PFLOP/s, the library's 1.10); at short k HBM
-// (256 x 1000003 x 512: dW 463 us, 3.3 TB/s read and written).
+// 131072 x 2048 bfloat16: dH 3.29 ms, 1.27 PFLOP/s, the library's 1.35; dW 3.35, 1.25 PFLOP/s, the library's 1.10); at short k HBM
+// (256 x 1000003 x 512: dW 484 us, 3.3 TB/s read and written).
 template <typename T, int BM, int BN, int WM, int WN, bool A_KROWS, bool B_KROWS>
 SSD_DEV void product(const GradArgs &p, int block, int blocks, char *smem)
 {

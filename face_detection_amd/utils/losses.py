@@ -28,8 +28,8 @@ class SSDLoss:
 
 
 class LinearCrossEntropy:
-    """Softmax cross entropy of a linear head over many classes, logits = logit_scale * hidden weight^T, which are never
-    stored whole (an identity head's 10^5 classes, a vocabulary).  No counterpart in the reference, whose heads have two
+    """Softmax cross entropy of a linear head over many classes, logits = logit_scale * hidden weight^T, of which
+    about 2 GiB are stored at most (an identity head's 10^5 classes, a vocabulary).  No counterpart in the reference, whose heads have two
     classes; arguments and results as batched.linear_cross_entropy_batch."""
 
     def __init__(self, logit_scale=1.0, label_smoothing=0.0):
