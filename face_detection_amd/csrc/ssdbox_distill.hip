@@ -1015,11 +1015,11 @@ void launch_distill(ssdbox_ctx *ctx, const DistArgs &a, const DistPlan &q, int r
         launch_stage(ctx, SSDBOX_STAGE_LOSS, distill_segment_kernel<T>, dim3((unsigned)rows * (a.grad ? q.segments : 1)),
                      dim3(kSegThreads), a);
     }
-    // as many lanes a row as leave each of them four classes; twice as many (rows x classes x K, us): 408000 x 4 x 2 float32 14.8, 16.4;
-    // 400000 x 8 x 3 bfloat16 24, 36;  400000 x 16 x 4 float32 35, 61;  300000 x 32 x 4 bfloat16 51, 91.  Against the sixteen lanes of
-    // the next kernel: 487435 x 23 x 6 float32 80, 109, its value alone 62, 103;  400000 x 20 x 2 bfloat16 55, 96; from 33 classes on they
-    // would be faster up to 64 entries (400000 x 60 x 2 float32 134, 122;  100000 x 40 x 8 float16 45, 37;  200000 x 60 x 30 bfloat16
-    // 151, 64), which this border leaves
+    // as many lanes a row as leave each of them four classes; twice as many (rows x classes x K, us): 408000 x 4 x 2 float32
+    // 14.8, 16.4;  400000 x 8 x 3 bfloat16 24, 36;  400000 x 16 x 4 float32 35, 61;  300000 x 32 x 4 bfloat16 51, 91.  Against the
+    // sixteen lanes of the next kernel: 487435 x 23 x 6 float32 80, 109, its value alone 62, 103;  400000 x 20 x 2 bfloat16 55, 96;
+    // from 33 classes on they would be faster up to 64 entries (400000 x 60 x 2 float32 134, 122;  100000 x 40 x 8 float16 45, 37;
+    // 200000 x 60 x 30 bfloat16 151, 64), which this border leaves
     else if (a.classes <= 4) launch_small<T, 1>(ctx, a, rows);
     else if (a.classes <= 8) launch_small<T, 2>(ctx, a, rows);
     else if (a.classes <= 16) launch_small<T, 4>(ctx, a, rows);
@@ -1028,7 +1028,8 @@ void launch_distill(ssdbox_ctx *ctx, const DistArgs &a, const DistPlan &q, int r
     // short rows: sixteen lanes a row rather than a wave, as long as the registers hold the entries (rows x classes x K, us:
     // 113154 x 164 x 8 float32 39, a wave 113;  35660 x 74 x 15 float32 18, 40;  50000 x 400 x 64 float32 44, 66;
     // 20000 x 1000 x 16 bfloat16 20, 31; past the registers' entries 20000 x 500 x 200 float32 133, 37), in registers for no more
-    // pieces than there are (for 128 instead: 113154 x 100 x 8 float32 34, 40;  100000 x 200 x 8 44, 50;  60000 x 400 x 16 bfloat16 30, 32)
+    // pieces than there are (for 128 instead: 113154 x 100 x 8 float32 34, 40;  100000 x 200 x 8 44, 50;  60000 x 400 x 16 bfloat16
+    // 30, 32)
     else if (pieces <= 128 && a.top <= 16 * kEntries<16>) {
         if (pieces <= 32) launch_row<T, 16, 2>(ctx, a, rows);
         else if (pieces <= 64) launch_row<T, 16, 4>(ctx, a, rows);

@@ -339,7 +339,8 @@ SSD_DEV void store_pair(T *row, int m, const float (&lo)[4], const float (&hi)[4
 // The logits by tiles: matrix instructions, and behind each tile its exponentials (one v_exp_f32 a logit, which the
 // stream's loads for the next tile run under).  Long dim: bound by the matrix instructions at the clock that the power limit leaves
 // (3891 x 32000 x 4096 bfloat16, value: 907 us, 1.12 PFLOP/s of 1.36 that the library's product alone reaches, matrix cores busy 74 %
-// of the time; 7782 x 131072 x 2048 with the exponentials stored: 4.06 ms, 1.03, 62 %); short dim: by the epilogue (1694 x 104936 x 16: 102 us, 1.7e12 exponentials a second).
+// of the time; 7782 x 131072 x 2048 with the exponentials stored: 4.06 ms, 1.03, 62 %); short dim: by the epilogue (1694 x 104936 x
+// 16: 102 us, 1.7e12 exponentials a second).
 template <typename T, int BM, int BN, int WM, int WN, int BLOCKS, int WHAT>
 __global__ __launch_bounds__(WM * WN * 64, BLOCKS * WM * WN / 4) void head_logit_kernel(const LogitArgs p)
 {
@@ -967,8 +968,8 @@ struct HeadPlan {
     long long chunk_rows;
     int dh_parts, dw_parts;
     bool scale_in_place;              // float16's rows times 2^-shift: nothing reads them as they were after their statistics
-    size_t o_few, o_blocks, o_rows, o_row_up, o_scaled, o_weight, o_row, o_label, o_count, o_scale, o_stat, o_sumz, o_zl, o_out, o_delta, o_kept, o_dh,
-        o_dw;
+    size_t o_few, o_blocks, o_rows, o_row_up, o_scaled, o_weight, o_row, o_label, o_count, o_scale, o_stat, o_sumz, o_zl, o_out;
+    size_t o_delta, o_kept, o_dh, o_dw;
     size_t bytes;
 };
 

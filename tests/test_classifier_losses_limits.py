@@ -182,17 +182,17 @@ def test_head_joins_of_many_rows(n, v, dim, ends):
 
 @pytest.mark.parametrize("dtype,size", [(_lib.DTYPE_F32, 4), (_lib.DTYPE_F16, 2), (_lib.DTYPE_BF16, 2)])
 def test_head_workspace_is_bounded(dtype, size):
-    """Of the logits' gradient 2 GiB, with 256 bytes a row of padding 2.5 or 3, and of float16's products as much, however rows and classes
-    are distributed; beside them a copy of the rows (float16: two, one of them scaled), their statistics, and sums of a gradient in
-    float32."""
+    """Of the logits' gradient 2 GiB, with 256 bytes a row of padding 2.5 or 3, and of float16's products as much, however rows and
+    classes are distributed; beside them a copy of the rows (float16: two, one of them scaled), their statistics, and sums of a
+    gradient in float32."""
     need = ctypes.c_size_t()
     for rows, classes, dim in ((4200000, 2, 8), ((1 << 24) - 1, 10, 8), (9000000, 300, 300), (1 << 23, 1, 8), ((1 << 23) // 65, 65, 16),
                                (3000000, 5000, 64), (1700000, 40, 8), (1300000, 300, 8), (2090000, 200, 8),
                                (4190000, 200, 8), (1 << 20, 1030, 64), (1 << 17, 1 << 18, 64),
                                ((1 << 24) - 1, 1 << 15, 8), (600000, 2000, 512), (20000, 1000003, 512), (1, 1 << 28, 16)):
         for grad_hidden, grad_weight in ((1, 1), (1, 0), (0, 1)):
-            _lib.check(_lib.load().ssdbox_linear_cross_entropy_workspace(rows, classes, dim, dim, dtype, 0.1, grad_hidden, grad_weight,
-                                                                         ctypes.byref(need)))
+            _lib.check(_lib.load().ssdbox_linear_cross_entropy_workspace(rows, classes, dim, dim, dtype, 0.1, grad_hidden,
+                                                                         grad_weight, ctypes.byref(need)))
             most = {_lib.DTYPE_F32: 2.5, _lib.DTYPE_F16: 5.0, _lib.DTYPE_BF16: 3.0}[dtype] * 2 ** 30
             copies = 2 if dtype == _lib.DTYPE_F16 else 1
             most += rows * (copies * dim * size + 36 + (classes / 32 + 8) * 12 + grad_hidden * (dim + 4) * 4) + 2 ** 29
@@ -317,8 +317,8 @@ def test_losses_of_empty_numpy_batches():
 # few logits, with rows left where they are or placed; logits taken again, kept; one row's slots many; several pieces; chunks
 @gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-@pytest.mark.parametrize("n,v,dim", [(60, 700, 64), (60, 700, 61), (5000, 900, 64), (300, 40000, 72), (300, 40000, 400), (40, 280000, 64),
-                                     (67000, 16700, 24), (4300000, 270, 16)])
+@pytest.mark.parametrize("n,v,dim", [(60, 700, 64), (60, 700, 61), (5000, 900, 64), (300, 40000, 72), (300, 40000, 400),
+                                     (40, 280000, 64), (67000, 16700, 24), (4300000, 270, 16)])
 def test_head_weights_far_apart(n, v, dim, dtype):
     """Rows' weights over nine powers of ten: each row's own gradient keeps the accuracy that its weight alone would give it, but for
     what lies below 2^-10 of the largest."""
