@@ -340,3 +340,39 @@ def test_head_weights_far_apart(n, v, dim, dtype):
     rows_against_the_oracle(got, hidden, weight, labels, weights, extra=extra)
     frozen = fda.linear_cross_entropy_batch(hidden, weight, labels, grad_loss=weights, return_grad=True, weight_grad=False)
     assert torch.equal(frozen[1], got[1])
+
+
+@gpu
+@pytest.mark.parametrize("n,v,dim,dtype", [(60, 700, 64, torch.float16), (300, 40000, 72, torch.float16), (300, 40000, 400, torch.float16),
+                                           (4300000, 30, 16, torch.bfloat16), (2200000, 30, 16, torch.float32)], ids=str)
+def test_weighted_and_long_heads_in_captured_graphs(n, v, dim, dtype):
+    """Two graphs replayed in turn on new inputs, with eager calls between, on streams of their own."""
+    import face_detection_amd as fda
+
+    def call(x):
+        return fda.linear_cross_entropy_batch(*x[:3], label_smoothing=0.1, grad_loss=x[3], return_grad=True)
+    sets = [list(long_inputs(n, v, dim, dtype, seed=s)) for s in range(3)]
+    for x in sets:
+        x[3] *= 10.0 ** -(torch.arange(n, device="cuda") * 7 % 10).float()
+    want = [call(x) for x in sets]
+    held = [[t.clone() for t in sets[k]] for k in (0, 1)]
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in held]
+    for x in held:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(call(x))
+        graphs.append(graph)
+    torch.cuda.synchronize()
+    for turn in range(3):
+        for k in (0, 1):
+            for dst, src in zip(held[k], sets[(turn + k) % 3]):
+                dst.copy_(src)
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        eager = call(sets[(turn + 2) % 3])
+        torch.cuda.synchronize()
+        for k in (0, 1):
+            assert all(torch.equal(a, b) for a, b in zip(outs[k], want[(turn + k) % 3]))
+        assert all(torch.equal(a, b) for a, b in zip(eager, want[(turn + 2) % 3]))
