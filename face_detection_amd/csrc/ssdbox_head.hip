@@ -39,7 +39,7 @@ constexpr long long kMostLd = 1 << 21;        // from one row of an operand to t
 constexpr long long kMostRows = (1 << 24) - 1;  // of workgroups of 256: a launch takes fewer than 2^32 threads
 constexpr int kRowsEach = 4;          // rows a workgroup places and copies
 constexpr int kCountRows = 1024;      // rows a workgroup counts, where there are many
-constexpr int kMostShift = 10;        // of a row of float16's d, beyond the scale that all have (see row_finish)
+constexpr int kShiftFrom = 10, kMostShift = 10;   // of a row of float16's d, beyond the scale that all have (see row_finish)
 constexpr int kCountFrom = 4096;      // rows from which counting has a launch of its own: below, reading all labels before
                                       // a workgroup's rows again costs less than the launch
 
@@ -514,8 +514,9 @@ SSD_DEV void scale_row(const T *from, T *to, int pitch, int shift)
 
 // A row's loss and its gradient's terms: the others' exponentials sum to s * 2^m, the label's is 2^(z l2) with its product z.
 // Float16 has few exponents: with one scale for all, p of a row whose weight is 10^6 times smaller than the largest would lie among
-// the subnormals.  Such a row's d is raised by 2^shift, which its dH gives back, and its values in dW's product.  What those lose
-// below 2^-14 is, with a shift of 10, less than their own rounding for values from 2^-4 on, and little beside other rows' terms.
+// the subnormals.  The d of rows below 2^-10 of the largest is raised by 2^shift, so that it keeps 2^-28 of the row's weight, which
+// its dH gives back, and its values in dW's product.  Those lose what falls below 2^-24 there, in terms 2^-10 to 2^-20 of others':
+// rows of larger weights stay as they are, since their d needs nothing and hidden values may be small.
 SSD_DEV HeadRow row_finish(const RowArgs &p, int n_in, float down, float m, double s, double sz, float z, int &shift)
 {
     shift = 0;
@@ -537,7 +538,7 @@ SSD_DEV HeadRow row_finish(const RowArgs &p, int n_in, float down, float m, doub
     double c = g * (double)p.logit_scale * (double)down;
     if (p.row_up) {
         const double v = fabs(c) * (1.0 - fmin((double)p.smoothing, 0.5));     // at most 32768 (1 - 1 / 128)
-        while (shift < kMostShift && v * (double)(2 << shift) <= 32512.0) ++shift;
+        while (shift < kMostShift && v * (double)(2 << (kShiftFrom + shift)) <= 32512.0) ++shift;
         c *= (double)(1 << shift);
     }
     const float top = fmaxf(m, (float)zl);

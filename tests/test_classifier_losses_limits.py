@@ -320,8 +320,7 @@ def test_losses_of_empty_numpy_batches():
 @pytest.mark.parametrize("n,v,dim", [(60, 700, 64), (60, 700, 61), (5000, 900, 64), (300, 40000, 72), (300, 40000, 400),
                                      (40, 280000, 64), (67000, 16700, 24), (4300000, 270, 16)])
 def test_head_weights_far_apart(n, v, dim, dtype):
-    """Rows' weights over nine powers of ten: each row's own gradient keeps the accuracy that its weight alone would give it, but for
-    what lies below 2^-10 of the largest."""
+    """Rows' weights over nine powers of ten: d of each row keeps 2^-28 of its weight, not of the largest, down to 2^-20 of that."""
     import face_detection_amd as fda
     hidden, weight, labels, _ = long_inputs(n, v, dim, dtype, ignored=0.1)
     power = torch.arange(n, device="cuda") * 7 % 10
@@ -332,14 +331,27 @@ def test_head_weights_far_apart(n, v, dim, dtype):
     for k in range(10):
         at = ((power == k) & (labels >= 0)).nonzero()[:, 0][:2000]
         own = most * 10.0 ** -k
-        (loss, gh, _), (off, off_h, _) = O.head(hidden[at], weight, labels[at], 1.0, 0.0, weights[at], max(own, most * 2.0 ** -10))
+        (loss, gh, _), (off, off_h, _) = O.head(hidden[at], weight, labels[at], 1.0, 0.0, weights[at],
+                                               min(most, max(own * 2.0 ** 10, most * 2.0 ** -10)))
         within_there(got[0][at], loss, off, "loss at 1e-%d" % k)
         within_there(got[1][at], gh, off_h, "grad_hidden at 1e-%d" % k)
-    # values of rows that are less than half the largest are rounded at 2^-25 times what their d was raised by, float16's alone
-    extra = most * n * 2.0 ** -25 if dtype == torch.float16 else 0.0
+    # float16's values of rows whose d is raised are rounded at 2^-25 times that, and the weights of these are 2^-10 less the largest
+    extra = most * n * 2.0 ** -35 if dtype == torch.float16 else 0.0
     rows_against_the_oracle(got, hidden, weight, labels, weights, extra=extra)
     frozen = fda.linear_cross_entropy_batch(hidden, weight, labels, grad_loss=weights, return_grad=True, weight_grad=False)
     assert torch.equal(frozen[1], got[1])
+
+
+@gpu
+@pytest.mark.parametrize("n,v,dim", [(60, 700, 64), (300, 40000, 72), (300, 40000, 400)])
+def test_head_weights_of_three_powers_of_ten_and_small_rows(n, v, dim):
+    """Float16 rows near its subnormals: those of a thousandth of the largest weight are not lowered for the weight's gradient."""
+    import face_detection_amd as fda
+    hidden, weight, labels, _ = long_inputs(n, v, dim, torch.float16, ignored=0.1)
+    hidden *= 2.0 ** -10
+    weights = 30000.0 * 10.0 ** -(torch.arange(n, device="cuda") * 7 % 4).float()
+    got = fda.linear_cross_entropy_batch(hidden, weight, labels, grad_loss=weights, return_grad=True)
+    rows_against_the_oracle(got, hidden, weight, labels, weights)
 
 
 @gpu
